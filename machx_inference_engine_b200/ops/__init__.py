@@ -10,7 +10,8 @@ import functools
 
 from . import ref
 from .ref import ACT_GEGLU, ACT_GELU_TANH, ACT_NONE, ACT_RELU2, ACT_SWIGLU, ACT_SWIGLU_OAI, ACT_TANH, ACT_XIELU, MOE_TILE, BranchMean, ExpertSum, MoePacking, PoolPages, act_gated, moe_max_rows
-from .weights import QuantWeight, WFormat, from_dense, from_exl3, from_ggml
+from .fp8 import FP8Rows
+from .weights import QuantWeight, WFormat, from_dense, from_exl3, from_fp8, from_ggml
 from ..utils.profiler import profiler as _prof
 
 _NAMES = [
@@ -19,6 +20,7 @@ _NAMES = [
     "hadamard128", "group_norm", "kv_store", "mingru_scan", "dyt_norm", "latent_post", "head_linear", "latent_attention", "latent_attention_expanded",
     "qk_post", "token_shift", "stacked_linear", "decay_scan", "gated_group_norm", "sublayer_norm", "moe_scale_rows",
     "pool_blocks", "causal_conv", "rglru_scan", "rglru_step",
+    "fp8_rows", "expert_linear",
 ]
 
 
@@ -47,6 +49,8 @@ def _first_tensor(args, kwargs):
             return a.p0
         if isinstance(a, MoePacking):
             return a.packed_token
+        if isinstance(a, FP8Rows):
+            return a.codes
     raise TypeError("op called without a tensor argument")
 
 
@@ -82,5 +86,5 @@ def expert_chunk(w, rows_per_expert):
 for _n in _NAMES:
     globals()[_n] = _make(_n)
 
-__all__ = _NAMES + ["set_backend", "expert_chunk", "QuantWeight", "WFormat", "from_dense", "from_exl3", "from_ggml", "BranchMean", "ExpertSum", "MoePacking", "PoolPages", "moe_max_rows", "ACT_NONE", "ACT_SWIGLU",
+__all__ = _NAMES + ["set_backend", "expert_chunk", "QuantWeight", "WFormat", "from_dense", "from_exl3", "from_fp8", "from_ggml", "FP8Rows", "BranchMean", "ExpertSum", "MoePacking", "PoolPages", "moe_max_rows", "ACT_NONE", "ACT_SWIGLU",
                     "ACT_SWIGLU_OAI", "ACT_GEGLU", "ACT_XIELU", "ACT_GELU_TANH", "ACT_RELU2", "ACT_TANH", "act_gated", "MOE_TILE"]

@@ -14,6 +14,8 @@ import torch
 
 from .. import _lib
 from .ref import ACT_GEGLU, ACT_NONE, ACT_SWIGLU, ACT_SWIGLU_OAI, MOE_TILE, BranchMean, ExpertSum, MoePacking, PoolPages, act_gated, moe_max_rows
+from . import fp8 as _fp8
+from .fp8 import FP8Rows
 from .weights import QuantWeight, WFormat
 
 _vp = C.c_void_p
@@ -685,6 +687,8 @@ def _gemm_rows(x, w: QuantWeight, out, out_kind, bias, row_scale, act, act_alpha
 def linear(x, w: QuantWeight, bias=None, act=ACT_NONE, act_alpha=1.702, act_limit=7.0, out_f32=False, row_scale=None, out=None):
     """``out``: write into this [M, n_out] view (unit column stride; a column slice of a wider matrix is fine), so that projections
     whose weights differ in format can share one output without a concatenation."""
+    if w.fmt == WFormat.FP8 or isinstance(x, FP8Rows):
+        return _linear_fp8(x, w, bias, act, act_alpha, act_limit, out_f32, row_scale, out)
     if x.dtype == torch.float32:
         return _linear_f32(x, w, bias, act, act_alpha, act_limit, row_scale, out)
     assert x.dtype == torch.bfloat16 and x.is_contiguous() and x.shape[-1] == w.K and w.E == 1
@@ -825,6 +829,8 @@ def grouped_linear(xp, w: QuantWeight, tile_expert, num_tiles, bias=None, act=AC
     """``chunk`` > 0 (with ``tile_valid``, the live rows of every tile): the weight-streaming kernel over groups of that many rows, for experts of a few dozen
     rows each; rows past a tile's live ones are then not written.  ``tokens``: rows that one expert may have; tiles of more live rows than
     :func:`expert_rows_max` says go to the tcgen05 kernel after all.  ``out_dtype`` (bf16 / fp16 / fp32) overrides ``out_f32``; fp16 feeds a following MXFP4 GEMM without a cast."""
+    if w.fmt == WFormat.FP8:
+        raise ValueError("grouped_linear: FP8 banks take compact packings (expert_linear)")
     P = xp.shape[0]
     if xp.dtype == torch.float32:            # 32-bit models: every row in fp32 on the CUDA cores
         if w.fmt != WFormat.BF16 or bias is not None or out_dtype not in (None, torch.float32):
@@ -861,6 +867,11 @@ def expert_gemv(x, w: QuantWeight, slot_expert, x_div=1, bias=None, act=ACT_NONE
     """``w`` holds experts [e_lo, e_lo + w.E); slots routed to other experts produce zero rows (expert parallelism)."""
     S = slot_expert.numel()
     n_out = w.N // 2 if act_gated(act) else w.N
+    if w.fmt == WFormat.FP8:
+        _fp8.check_slots(x, w, slot_expert, x_div, bias, act_gated(act), slot_scale)
+        with _on(x.device):
+            out = torch.empty(S, n_out, dtype=torch.float32 if out_f32 else torch.bfloat16, device=x.device)
+            return _fp8_gemm(x, w, out, bias, slot_scale, act, act_alpha, act_limit, slot=slot_expert, x_div=x_div, e_lo=e_lo)
     out = torch.empty(S, n_out, dtype=torch.float32 if out_f32 else torch.bfloat16, device=x.device)
     fmt, p0, p1, p2, p3 = _planes(w)
     _check(_lib.cuda().mx_gemv_experts(fmt, p0, p1, p2, p3, _p(x), _p(out), _p(bias), w.N, w.K, int(out_f32), act, C.c_float(act_alpha),
@@ -868,6 +879,64 @@ def expert_gemv(x, w: QuantWeight, slot_expert, x_div=1, bias=None, act=ACT_NONE
            "expert gemv")
     _count()
     return out
+
+
+# ------------------------------------------------------------------ 8-bit floating point (see ops/fp8.py)
+class _Nothing:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+def _on(device):
+    """Launches and allocations go to ``device``, whichever is current."""
+    return _Nothing() if device.index is None or device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def fp8_rows(x, index=None) -> FP8Rows:
+    _fp8.check_rows(x, index)
+    with _on(x.device):
+        rows, K = x.shape[0] if index is None else index.numel(), x.shape[1]
+        kb = -(-K // _fp8.FP8_BLOCK)
+        q = FP8Rows(torch.empty(rows, kb * _fp8.FP8_BLOCK, dtype=torch.float8_e4m3fn, device=x.device), torch.empty(kb, rows, dtype=torch.float32, device=x.device), K)
+        if rows:
+            _check(_lib.cuda().mx_fp8_rows(_p(x), int(x.dtype == torch.float32), C.c_longlong(x.stride(0)), _p(index), x.shape[0], rows, K, _p(q.codes), _p(q.scale),
+                                           _stream()), "fp8_rows")
+            _count()
+    return q
+
+
+def _fp8_gemm(x, w: QuantWeight, out, bias, row_scale, act, act_alpha, act_limit, counts=None, seg=None, slot=None, x_div=1, e_lo=0, index=None):
+    M = out.shape[0]
+    if M == 0:
+        return out
+    q = x if isinstance(x, FP8Rows) else fp8_rows(x, index)
+    _check(_lib.cuda().mx_fp8_gemm(_p(q.codes), _p(q.scale), q.codes.shape[0], _p(w.p0), _p(w.p1), w.E, _p(out), C.c_longlong(out.stride(0)),
+                                   int(out.dtype == torch.float32), _p(bias), _p(row_scale), act, C.c_float(act_alpha), C.c_float(act_limit), M, w.N, w.p1.shape[2],
+                                   _p(counts), _p(seg), _p(slot), int(x_div), int(e_lo), _stream()), "fp8_gemm")
+    _count()
+    return out
+
+
+def _linear_fp8(x, w: QuantWeight, bias, act, act_alpha, act_limit, out_f32, row_scale, out):
+    M, n_out, odt = x.shape[0], w.N // 2 if act_gated(act) else w.N, torch.float32 if out_f32 else torch.bfloat16
+    _fp8.check_product(x, w, False, M, bias, act_gated(act), "linear")
+    _fp8.check_out(out, row_scale, M, n_out, odt, x.device)
+    with _on(x.device):
+        if out is None:
+            out = torch.empty(M, n_out, dtype=odt, device=x.device)
+        return _fp8_gemm(x, w, out, bias, row_scale, act, act_alpha, act_limit)
+
+
+def expert_linear(x, w: QuantWeight, pk: MoePacking, x_index=None, bias=None, act=ACT_NONE, act_alpha=1.702, act_limit=7.0, out_f32=False, e_lo=0):
+    P, n_out = pk.max_rows, w.N // 2 if act_gated(act) else w.N
+    _fp8.check_product(x, w, True, P, bias, act_gated(act), "expert_linear")
+    _fp8.check_packing(pk, w, x, x_index, e_lo)
+    with _on(x.device):
+        out = torch.empty(P, n_out, dtype=torch.float32 if out_f32 else torch.bfloat16, device=x.device)
+        return _fp8_gemm(x, w, out, bias, None, act, act_alpha, act_limit, counts=pk.counts[e_lo:], seg=pk.seg_start[e_lo:], index=None if x_index is None else x_index[:P])
 
 
 # ------------------------------------------------------------------ attention

@@ -12,7 +12,9 @@ from typing import Optional
 
 import torch
 
-from .weights import QuantWeight
+from . import fp8 as _fp8
+from .fp8 import FP8Rows
+from .weights import QuantWeight, WFormat
 
 ACT_NONE, ACT_SWIGLU, ACT_SWIGLU_OAI, ACT_GEGLU, ACT_XIELU, ACT_GELU_TANH, ACT_RELU2, ACT_TANH = 0, 1, 2, 3, 4, 5, 6, 7
 
@@ -143,14 +145,23 @@ def glu(x, act, alpha=1.702, limit=7.0):
 
 
 def linear(x, w: QuantWeight, bias=None, act=ACT_NONE, act_alpha=1.702, act_limit=7.0, out_f32=False, row_scale=None, out=None):
+    if w.fmt == WFormat.FP8:
+        _fp8.check_out(out, row_scale, x.shape[0], w.N // 2 if act_gated(act) else w.N, torch.float32 if out_f32 else torch.bfloat16, x.device)
     if out is not None:
         return out.copy_(linear(x, w, bias, act, act_alpha, act_limit, out_f32, row_scale))
-    y = _mm(x, _dense(w)[0])
+    if w.fmt == WFormat.FP8 or isinstance(x, FP8Rows):
+        _fp8.check_product(x, w, False, x.shape[0], bias, act_gated(act), "linear")
+        x = _fp8.values(x)
+        out_f32, y = out_f32 or None, _mm(x, _dense(w)[0])          # (None: bf16 whatever the type of the values)
+    else:
+        y = _mm(x, _dense(w)[0])
     if bias is not None:
         y = y + bias
     y = _epilogue_act(y, act, act_alpha, act_limit)
     if row_scale is not None:
         y = y * row_scale.unsqueeze(-1)
+    if out_f32 is None:
+        return y.to(torch.bfloat16)
     return y if (out_f32 or x.dtype == torch.float32) else y.to(torch.bfloat16)      # fp32 activations: the layer runs in fp32 throughout
 
 
@@ -173,6 +184,8 @@ def grouped_linear(xp, w: QuantWeight, tile_expert, num_tiles, bias=None, act=AC
                    out_dtype=None, tile_valid=None, chunk=0, tokens=0):
     """xp: packed rows [P,K]; tile t (rows 128t..128t+127) uses expert tile_expert[t] for t < num_tiles[0].  ``tile_valid`` (live rows of every tile),
     ``chunk`` and ``tokens`` choose a kernel on the GPU."""
+    if w.fmt == WFormat.FP8:
+        raise ValueError("grouped_linear: FP8 banks take compact packings (expert_linear)")
     W = _dense(w)
     P = xp.shape[0]
     n_out = w.N // 2 if act_gated(act) else w.N
@@ -194,8 +207,13 @@ def expert_gemv(x, w: QuantWeight, slot_expert, x_div=1, bias=None, act=ACT_NONE
     """y[s] = W[slot_expert[s] - e_lo] @ x[s // x_div]; slots whose expert lies outside [e_lo, e_lo + E) give zero rows."""
     W = _dense(w)
     S = slot_expert.numel()
+    if w.fmt == WFormat.FP8:
+        _fp8.check_slots(x, w, slot_expert, x_div, bias, act_gated(act), slot_scale)
     rows = torch.arange(S, device=x.device) // x_div
-    xe = x.to(torch.float32)[rows]
+    if w.fmt == WFormat.FP8:
+        xe, out_f32 = _fp8.values(x)[rows], out_f32 or None
+    else:
+        xe = x.to(torch.float32)[rows]
     se = slot_expert.long() - e_lo
     owned = (se >= 0) & (se < w.E)
     se = se.clamp(0, w.E - 1)
@@ -206,6 +224,8 @@ def expert_gemv(x, w: QuantWeight, slot_expert, x_div=1, bias=None, act=ACT_NONE
     y = y * owned.unsqueeze(-1)
     if slot_scale is not None:
         y = y * slot_scale.unsqueeze(-1)
+    if out_f32 is None:
+        return y.to(torch.bfloat16)
     return y if (out_f32 or x.dtype == torch.float32) else y.to(torch.bfloat16)
 
 
@@ -984,6 +1004,33 @@ def expert_group_gemv(x, w: QuantWeight, pk: MoePacking, x_index=None, bias=None
         y = _epilogue_act(y, act, act_alpha, act_limit)
         out[rows] = y
     return out.to(torch.bfloat16)
+
+
+def fp8_rows(x, index=None) -> FP8Rows:
+    """Rows of ``x`` (bf16 or fp32 [rows, K], any row stride) as e4m3 codes with a power-of-two scale per 128 elements (:mod:`ops.fp8`), for products with FP8
+    weights.  ``index`` (int32): row r of the result is row index[r] of ``x``; a negative entry gives zeros, one past the end NaN."""
+    return _fp8.round_rows(x, index)
+
+
+def expert_linear(x, w: QuantWeight, pk: MoePacking, x_index=None, bias=None, act=ACT_NONE, act_alpha=1.702, act_limit=7.0, out_f32=False, e_lo=0):
+    """y[r] = act(W[expert of packed row r] x[x_index[r] or r] + bias) over a compact packing (``moe_pack(..., tile=1)``), FP8 banks, any number of rows per
+    expert: [pk.max_rows, N_out].  ``w`` holds experts [e_lo, e_lo + w.E) of the packing; rows of other experts, and those behind the last one, are not
+    written (zeros here)."""
+    P, n_out = pk.max_rows, w.N // 2 if act_gated(act) else w.N
+    _fp8.check_product(x, w, True, P, bias, act_gated(act), "expert_linear")
+    _fp8.check_packing(pk, w, x, x_index, e_lo)
+    W, xf = _dense(w), _fp8.values(x)
+    out = torch.zeros(P, n_out, dtype=torch.float32, device=x.device)
+    for el in range(w.E):
+        c, s0 = int(pk.counts[e_lo + el]), int(pk.seg_start[e_lo + el])
+        if c == 0:
+            continue
+        rows = torch.arange(s0, s0 + c, device=x.device)
+        y = _mm(xf[x_index[rows].long()] if x_index is not None else xf[rows], W[el])
+        if bias is not None:
+            y = y + bias[el]
+        out[rows] = _epilogue_act(y, act, act_alpha, act_limit)
+    return out if out_f32 else out.to(torch.bfloat16)
 
 
 def moe_combine(yp, pk: MoePacking, w, out=None, accumulate=False):

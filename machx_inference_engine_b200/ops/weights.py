@@ -1,6 +1,6 @@
 """Runtime weight layouts and the load-time repack from ggml blocks.
 
-A :class:`QuantWeight` is a (stack of) [N, K] matrix stored in one of five runtime formats that
+A :class:`QuantWeight` is a (stack of) [N, K] matrix stored in one of the runtime formats that
 the sm_100a GEMV and GEMM kernels decode in registers:
 
 ========  =====================================================================================
@@ -20,6 +20,9 @@ MXF4T     the same codes cut into tiles of 192 rows x 128 elements, ``p0`` [E,FB
 EXL3      ``p0`` the trellis int16 [1,K/16,N/16,16*bits] as stored in the checkpoint, ``p1`` suh fp32 [1,K],
           ``p2`` svh fp32 [1,N]: y = had128(had128(x * suh) W_rot) * svh (see formats/exl3.py).  One matrix per
           weight (no expert stacks), never concatenated or sliced: every projection has its own rotation
+FP8       ``p0`` e4m3 codes [E,N,KB*128] (KB = ceil(K/128), zeros past K), ``p1`` fp32 scales [E,ceil(N/16),KB]: one for 16 rows by 128
+          elements, so that rows can be joined, cut and interleaved in runs of 16 whatever blocks a checkpoint has (128 x 128 as a rule).
+          The products multiply activations that are e4m3 too (ops/fp8.py)
 ========  =====================================================================================
 
 The rows of the small scale planes (Q8 ``p1``, Q6K ``p3``, MXFP4 ``p1``) are zero-padded to 16 bytes
@@ -49,6 +52,7 @@ class WFormat(IntEnum):
     MXFP4 = 4
     MXF4T = 5      # MXFP4 in 128 x 128 tiles for the block-scaled tensor-core kernel (see to_mxf4_tiles)
     EXL3 = 6       # trellis-coded weights with Hadamard rotations on both sides (formats/exl3.py)
+    FP8 = 7        # e4m3 codes with a scale per 16 x 128, multiplied with e4m3 activations (ops/fp8.py)
 
 
 def _pad_last(t: torch.Tensor, mult: int) -> torch.Tensor:
@@ -116,12 +120,33 @@ class QuantWeight:
         """Rows (output features) ``idx`` of every expert."""
         self._no_exl3("row-permuted")
         idx = idx.to(self.device)
+        if self.fmt == WFormat.FP8:
+            return self._select_fp8(idx.long())
         w = self._map_planes(lambda t: t.index_select(1, idx).contiguous())
         w.N = int(idx.numel())
         return w
 
+    def _select_fp8(self, idx: torch.Tensor) -> "QuantWeight":
+        """The codes unchanged where the rows of every new run of 16 have the same scales; otherwise that run is rounded again, to the largest of them."""
+        n = int(idx.numel())
+        groups = -(-n // FP8_ROWS)
+        codes = self.p0.view(torch.uint8).index_select(1, idx)
+        at = idx // FP8_ROWS
+        at = torch.cat([at, at[-1:].expand(groups * FP8_ROWS - n)])
+        t = self.p1.index_select(1, at).reshape(self.E, groups, FP8_ROWS, -1)
+        top = torch.gather(t, 2, t.abs().argmax(dim=2, keepdim=True))
+        w = QuantWeight(WFormat.FP8, n, self.K, self.E, codes.view(torch.float8_e4m3fn).contiguous(), top[:, :, 0].contiguous())
+        if not torch.equal(t, top.expand_as(t)):
+            same = (t == top).reshape(self.E, groups * FP8_ROWS, -1)[:, :n].repeat_interleave(FP8_BLOCK, dim=-1)
+            ratio = torch.where(top != 0, t / top, torch.zeros_like(t)).reshape(self.E, groups * FP8_ROWS, -1)[:, :n].repeat_interleave(FP8_BLOCK, dim=-1)
+            again = (w.p0.to(torch.float32) * ratio).to(torch.float8_e4m3fn)
+            w.p0 = torch.where(same, w.p0.view(torch.uint8), again.view(torch.uint8)).view(torch.float8_e4m3fn)
+        return w
+
     def slice_rows(self, lo: int, hi: int) -> "QuantWeight":
         self._no_exl3("sliced by rows")
+        if self.fmt == WFormat.FP8:
+            return self._select_fp8(torch.arange(lo, hi, device=self.device))
         w = self._map_planes(lambda t: t[:, lo:hi].contiguous())
         w.N = hi - lo
         return w
@@ -152,7 +177,7 @@ class QuantWeight:
         return w
 
     def k_granule(self) -> int:
-        return {WFormat.BF16: 8, WFormat.Q8: 32, WFormat.Q4K: 256, WFormat.Q6K: 256, WFormat.MXFP4: 32}[self.fmt]
+        return {WFormat.BF16: 8, WFormat.Q8: 32, WFormat.Q4K: 256, WFormat.Q6K: 256, WFormat.MXFP4: 32, WFormat.FP8: FP8_BLOCK}[self.fmt]
 
     def slice_k(self, lo: int, hi: int, requant: bool = False) -> "QuantWeight":
         """Input-dimension slice [lo, hi) (row-parallel shards).  Bounds must sit on block boundaries; with
@@ -160,14 +185,14 @@ class QuantWeight:
         else bf16) -- the case of a 256-element super-block format sharded finer than its blocks."""
         self._no_exl3("sliced along K")
         g = self.k_granule()
-        if lo % g or hi % g:
+        if lo % g or (hi % g and not (self.fmt == WFormat.FP8 and hi == self.K)):
             if not requant:
                 raise ValueError(f"K slice [{lo},{hi}) is not aligned to the {g}-element blocks of {self.fmt.name}")
             dense = self.dequantize(torch.float32)[:, :, lo:hi].contiguous()
             return from_dense(dense, WFormat.Q8 if (hi - lo) % 32 == 0 else WFormat.BF16)
         per_elem = {
             WFormat.BF16: (1, None, None, None), WFormat.Q8: (1, 32, None, None), WFormat.Q4K: (256 / 144, None, None, None),
-            WFormat.Q6K: (2, 4, 16, 256), WFormat.MXFP4: (2, 32, None, None),
+            WFormat.Q6K: (2, 4, 16, 256), WFormat.MXFP4: (2, 32, None, None), WFormat.FP8: (1, FP8_BLOCK, None, None),
         }[self.fmt]
         outs = []
         pads = _AUX_PAD.get(int(self.fmt), {})
@@ -176,6 +201,8 @@ class QuantWeight:
                 outs.append(None)
             else:
                 a, b = int(round(lo / div)), int(round(hi / div))
+                if self.fmt == WFormat.FP8 and hi == self.K:         # the last block's zeros with it
+                    b = t.shape[2]
                 sl = t[:, :, a:b]
                 outs.append(_pad_last(sl, pads[i][1]) if i in pads else sl.contiguous())
         w = QuantWeight(self.fmt, self.N, hi - lo, self.E, *outs)
@@ -186,6 +213,8 @@ class QuantWeight:
         f = ws[0]
         f._no_exl3("concatenated")
         assert all(w.fmt == f.fmt and w.K == f.K and w.E == f.E for w in ws), "cannot concatenate mixed formats"
+        if f.fmt == WFormat.FP8 and any(w.N % FP8_ROWS for w in ws[:-1]):
+            raise ValueError(f"FP8 matrices are joined in whole runs of {FP8_ROWS} rows, not {[w.N for w in ws]}")
         outs = []
         for i in range(4):
             ps = [w.planes()[i] for w in ws]
@@ -203,6 +232,8 @@ class QuantWeight:
             if a is None:
                 return None
             E, N = a.shape[0], a.shape[1]
+            if a.shape[1] != gate.N:                                 # FP8: one row of scales for 16 rows
+                return torch.stack([a, b], dim=2).reshape(E, 2 * N, -1).contiguous()
             a2 = a.reshape(E, N // 16, 16, -1)
             b2 = b.reshape(E, N // 16, 16, -1)
             return torch.cat([a2, b2], dim=2).reshape(E, 2 * N, -1).contiguous()
@@ -247,6 +278,9 @@ class QuantWeight:
             c = torch.stack([codes & 15, codes >> 4], dim=-1).reshape(E, N, K // 32, 32)
             vals = _E2M1.to(codes.device)[c]
             w = vals * _e8m0_to_f32(self.p1[..., :K // 32]).unsqueeze(-1)
+        elif self.fmt == WFormat.FP8:
+            t = self.p1.repeat_interleave(FP8_ROWS, dim=1)[:, :N].repeat_interleave(FP8_BLOCK, dim=2)
+            w = (self.p0.to(torch.float32) * t)[..., :K]
         else:  # pragma: no cover
             raise ValueError(self.fmt)
         return w.reshape(E, N, K).to(dtype)
@@ -496,9 +530,46 @@ def from_exl3(trellis: torch.Tensor, suh: torch.Tensor, svh: torch.Tensor) -> Qu
                        svh.to(dev, torch.float32).reshape(1, N).contiguous())
 
 
+FP8_BLOCK = 128     # elements of K per scale
+FP8_ROWS = 16       # rows per scale in the runtime layout
+
+
+def from_fp8(codes: torch.Tensor, scales: torch.Tensor, block=(128, 128)) -> QuantWeight:
+    """``codes`` e4m3 [N,K] or [E,N,K] and ``scales`` [.., ceil(N/block[0]), ceil(K/block[1])] (any float type; what a code is multiplied with) -> the runtime
+    weight.  ``block``: rows (a multiple of 16) and elements of K (a multiple of 128) that share a scale; None in either place: all of them."""
+    if codes.dtype != torch.float8_e4m3fn or codes.dim() not in (2, 3) or 0 in codes.shape:
+        raise ValueError(f"FP8 codes are float8_e4m3fn [N,K] or [E,N,K], not {codes.dtype} {tuple(codes.shape)}")
+    if codes.dim() == 2:
+        codes, scales = codes.unsqueeze(0), scales.unsqueeze(0)
+    E, N, K = codes.shape
+    rows, cols = (n if b is None else b for b, n in zip(block, (-(-N // FP8_ROWS) * FP8_ROWS, -(-K // FP8_BLOCK) * FP8_BLOCK)))
+    if rows < 1 or cols < 1 or rows % FP8_ROWS or cols % FP8_BLOCK:
+        raise ValueError(f"FP8 scales of blocks of {rows} x {cols}: whole multiples of {FP8_ROWS} x {FP8_BLOCK} are taken")
+    if not scales.is_floating_point() or tuple(scales.shape) != (E, -(-N // rows), -(-K // cols)):
+        raise ValueError(f"FP8 scales of a [{E},{N},{K}] weight in blocks of {rows} x {cols} are {[E, -(-N // rows), -(-K // cols)]}, not {scales.dtype} {list(scales.shape)}")
+    blocks, groups = -(-K // FP8_BLOCK), -(-N // FP8_ROWS)
+    t = scales.to(codes.device, torch.float32)
+    t = t.repeat_interleave(rows // FP8_ROWS, dim=1)[:, :groups].repeat_interleave(cols // FP8_BLOCK, dim=2)[:, :, :blocks]
+    p0 = _pad_last(codes.view(torch.uint8), FP8_BLOCK).view(torch.float8_e4m3fn)
+    return QuantWeight(WFormat.FP8, N, K, E, p0, t.contiguous())
+
+
+def quantize_fp8(w: torch.Tensor) -> QuantWeight:
+    """Round ``w`` [E,N,K] (or [N,K]) to e4m3 with one fp32 scale, the largest magnitude over 448, per block of 128 x 128."""
+    if w.dim() == 2:
+        w = w.unsqueeze(0)
+    E, N, K = w.shape
+    nb, kb = -(-N // 128), -(-K // FP8_BLOCK)
+    x = torch.nn.functional.pad(w.to(torch.float32), (0, kb * FP8_BLOCK - K, 0, nb * 128 - N)).view(E, nb, 128, kb, FP8_BLOCK)
+    t = x.abs().amax(dim=(2, 4)) / 448.0
+    t = torch.where(t > 0, t, torch.ones_like(t))
+    codes = (x / t[:, :, None, :, None]).clamp_(-448.0, 448.0).to(torch.float8_e4m3fn).reshape(E, nb * 128, kb * FP8_BLOCK)
+    return from_fp8(codes.view(torch.uint8)[:, :N, :K].contiguous().view(torch.float8_e4m3fn), t)
+
+
 def from_dense(w: torch.Tensor, fmt: WFormat) -> QuantWeight:
     if fmt == WFormat.BF16:
         if w.dim() == 2:
             w = w.unsqueeze(0)
         return QuantWeight(WFormat.BF16, w.shape[1], w.shape[2], w.shape[0], w.to(torch.bfloat16).contiguous())
-    return {WFormat.Q8: quantize_q8, WFormat.Q4K: quantize_q4k, WFormat.Q6K: quantize_q6k, WFormat.MXFP4: quantize_mxfp4}[fmt](w)
+    return {WFormat.Q8: quantize_q8, WFormat.Q4K: quantize_q4k, WFormat.Q6K: quantize_q6k, WFormat.MXFP4: quantize_mxfp4, WFormat.FP8: quantize_fp8}[fmt](w)
