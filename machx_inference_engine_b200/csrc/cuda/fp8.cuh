@@ -29,4 +29,67 @@ __device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d
   return (uint32_t)lo | ((uint32_t)hi << 16);
 }
 
+// D[tmem] (+)= A[smem] * B[smem], e4m3 inputs (K = 32 a step), fp32 accumulate; issued by one thread.
+__device__ __forceinline__ void umma_e4m3(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// kind::f8f6f4 instruction descriptor: e4m3 x e4m3 -> fp32, M x N tile, both operands K-major.
+__host__ __device__ constexpr uint32_t umma_idesc_e4m3(int M, int N) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }
+
+// two fp32 numbers in one register pair: d = a * b + c and a * b, each rounded once
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+template <int N> __device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[N]) {      // N columns of 32 lanes
+  static_assert(N == 16 || N == 32, "columns of one load");
+  if constexpr (N == 32) {
+    tmem_ld_32x32(taddr, r);
+  } else {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+          "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+  }
+}
+
+// What a product multiplies and writes.
+struct Fp8Params {
+  const __nv_bfloat16* xb;   // rows to be rounded on the way, `ldx` elements apart; null: codes and scales
+  long long ldx;
+  const int* x_index;        // experts: row of xb that packed row m reads (null: m)
+  const float* sx;           // [kb][x_rows]
+  int x_rows;
+  const float* sw;           // [E][ceil(N / 16)][kb]
+  void* C;
+  long long ldc;
+  int out_f32, M, N, K, kb, E;
+  const float* bias;         // [N] or [E][N]
+  const float* row_scale;    // [M]
+  int act;
+  float act_alpha, act_limit;
+  const int* counts;         // experts: rows of expert i of the bank, and the first of them
+  const int* seg;
+  const int* slot;           // slots: expert of output row m, whose input is row m / x_div
+  int x_div, e_lo;
+  float* part;               // partial sums of cut tiles
+  int* tickets;
+  int* status;
+};
+
 }  // namespace mx

@@ -1,8 +1,14 @@
-// Products of e4m3 rows with e4m3 weights, both with scales per 128 elements of K:
+// Products of many e4m3 rows with e4m3 weights, scales per 128 elements of K on both sides, on the tensor cores:
 //   y[m, n] = act(sum_b sx[b][m] sw[n / 16][b] sum_{k in b} x8[m][k] w8[n][k] + bias[n])
-// for dense layers, rows sorted by expert, and slots of one row and one expert.
+// for dense layers and for rows sorted by expert.
 //
-// The plainest form: tiles of 32 x 32 outputs, fp32 multiplications of decoded codes, a block of K at a time.
+// A block of K is one stage: 128 rows of x and BN of w, 128 bytes each, and four tcgen05.mma of K = 32.  Its sums have a scale of their own, so they cannot
+// stay in TMEM: eight warps read each block's 128 x BN sums and add s_x s_w times them to fp32 sums in registers, BN / 2 columns of a row per thread, while the
+// tensor cores fill the next accumulator.
+//   warp 0      TMA loads into a ring of NST stages
+//   warp 1      tcgen05.mma from one thread into a ring of 512 / BN accumulators
+//   warps 4-11  sums (warp & 3: rows, warp / 8: half of the columns); a finished tile goes through shared memory, so that rows are written in runs of 128 bytes
+// Every mbarrier wait is bounded.
 #include "act.cuh"
 #include "common.cuh"
 #include "fp8.cuh"
@@ -10,118 +16,315 @@
 
 namespace mx {
 
-struct Fp8Params {
-  const uint8_t* x;          // [rows][kb * 128]
-  const float* sx;           // [kb][x_rows]
-  const uint8_t* w;          // [E][N][kb * 128]
-  const float* sw;           // [E][ceil(N / 16)][kb]
-  void* C;
-  long long ldc;
-  int out_f32, M, N, kb, x_rows, E;
-  const float* bias;         // [N] or [E][N]
-  const float* row_scale;    // [M]
-  int act;
-  float act_alpha, act_limit;
-  const int* seg;            // experts: first packed row of expert e_lo + i, and how many
-  const int* counts;
-  const int* slot;           // slots: expert of output row m, whose input is row m / x_div
-  int x_div, e_lo;
+constexpr int FG_BM = 128, FG_THREADS = 384, FG_MAX_E = 1024;
+constexpr int FG_GROUP = 8;                                // m-tiles that are walked together: a wave shares bands of x and w in L2
+
+template <int BN> struct Fp8GemmShape {
+  static constexpr int A = FG_BM * FP8_BLOCK, B = BN * FP8_BLOCK, STAGE = A + B;
+  static constexpr int OUT = 8 * 4096;                     // 32 rows x 128 bytes for each warp
+  static constexpr int NST = 192 * 1024 / STAGE;
+  static constexpr int ACC = 512 / BN;
+  struct Small {                                           // what is not tiles, behind them
+    uint64_t bar[2 * NST + 2 * ACC];
+    int sum[12];
+    uint32_t tmem;
+    int abort;
+    uint16_t pre[FG_MAX_E + 1];                            // experts: m-tiles before expert i
+  };
+  static constexpr int SMEM = NST * STAGE + OUT + (int)sizeof(Small);
+  static_assert(SMEM <= 227 * 1024, "shared memory of a block");
 };
 
-__global__ void __launch_bounds__(256) fp8_gemm_kernel(const Fp8Params p) {
-  __shared__ float sa[32][FP8_BLOCK + 1], sb[32][FP8_BLOCK + 1], so[32][33];
-  __shared__ int s_tile[3];
-  pdl_prologue();
-  const int tid = threadIdx.x, n0 = blockIdx.x * 32;
+template <int BN>
+__global__ void __launch_bounds__(FG_THREADS, 1)
+fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, const Fp8Params p) {
+  using S = Fp8GemmShape<BN>;
+  constexpr int NST = S::NST, ACC = S::ACC;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  auto& small = *reinterpret_cast<typename S::Small*>(smem_raw + NST * S::STAGE + S::OUT);
+  auto& s_bar = small.bar;
+  auto& s_pre = small.pre;
+  auto& s_sum = small.sum;
+  uint32_t& s_tmem = small.tmem;
+  int& s_abort = small.abort;
+  const uint32_t base = smem_u32(smem_raw);
+  if (base & 1023) {                                       // (swizzled tiles start on 1 KiB; no static shared memory lies before them)
+    if (threadIdx.x == 0) atomicCAS(p.status, 0, ERR_BAD_ARGUMENT);
+    return;
+  }
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t bar_full = smem_u32(s_bar), bar_empty = bar_full + 8 * NST, bar_tfull = bar_empty + 8 * NST, bar_tempty = bar_tfull + 8 * ACC;
+  volatile int* abort_flag = &s_abort;
   if (tid == 0) {
-    int e = 0, row0 = blockIdx.y * 32, rows = min(32, p.M - row0);
-    if (p.slot) {
-      row0 = blockIdx.y; rows = 1;
-      e = p.slot[row0] - p.e_lo;
-    } else if (p.seg) {
-      int t = blockIdx.y;
-      rows = 0;
-      for (e = 0; e < p.E; ++e) {
-        const int c = p.counts[e], tiles = (c + 31) / 32;
-        if (t < tiles) { row0 = p.seg[e] + t * 32; rows = min(32, c - t * 32); break; }
-        t -= tiles;
+    for (int s = 0; s < NST; ++s) { mbar_init(bar_full + 8 * s, 1); mbar_init(bar_empty + 8 * s, 1); }
+    for (int a = 0; a < ACC; ++a) { mbar_init(bar_tfull + 8 * a, 1); mbar_init(bar_tempty + 8 * a, 8); }
+    s_abort = 0;
+    fence_mbar_init();
+  }
+  // tensor memory is taken when the launch before has ended: it may still want some, and would wait for a CTA that waits for it
+  pdl_wait();
+  if (warp == 1) { tmem_alloc(smem_u32(&s_tmem), 512); tmem_relinquish(); pdl_launch_dependents(); }
+
+  // ---- tiles: dense in groups of FG_GROUP m-tiles; experts one after the other, their m-tiles under each column of tiles
+  const bool banked = p.counts != nullptr;
+  const int n_tiles = (p.N + BN - 1) / BN;
+  int m_tiles = (p.M + FG_BM - 1) / FG_BM;
+  if (banked) {
+    int run = 0;
+    for (int e0 = 0; e0 < p.E; e0 += FG_THREADS) {
+      const int e = e0 + tid;
+      int incl = e < p.E ? (p.counts[e] + FG_BM - 1) / FG_BM : 0;
+      const int mine = incl;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += u;
       }
-      rows = min(rows, p.M - row0);
-    }
-    s_tile[0] = e; s_tile[1] = row0; s_tile[2] = rows;
-  }
-  __syncthreads();
-  const int e = s_tile[0], row0 = s_tile[1], rows = s_tile[2];
-  if (rows <= 0) return;
-  const bool owned = e >= 0 && e < p.E;
-  const int r = tid >> 3, c = tid & 7, groups = (p.N + FP8_ROWS - 1) / FP8_ROWS;
-  float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  auto in_row = [&](int i) { return p.slot ? (row0 + i) / p.x_div : row0 + i; };
-  for (int b = 0; b < p.kb && owned; ++b) {
-    __syncthreads();
-    for (int i = tid; i < 32 * FP8_BLOCK; i += 256) {
-      const int rr = i >> 7, k = i & 127;
-      __nv_fp8_e4m3 v;
-      v.__x = rr < rows ? p.x[(size_t)in_row(rr) * p.kb * FP8_BLOCK + b * FP8_BLOCK + k] : 0;
-      sa[rr][k] = float(v);
-      v.__x = n0 + rr < p.N ? p.w[((size_t)e * p.N + n0 + rr) * p.kb * FP8_BLOCK + b * FP8_BLOCK + k] : 0;
-      sb[rr][k] = float(v);
-    }
-    __syncthreads();
-    if (r < rows) {
-      const float sx = p.sx[(size_t)b * p.x_rows + in_row(r)];
+      if (lane == 31) s_sum[warp] = incl;
+      __syncthreads();
+      int before = run;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int n = n0 + c + 8 * j;
-        if (n >= p.N) continue;
-        float d = 0.f;
-        for (int k = 0; k < FP8_BLOCK; ++k) d = fmaf(sa[r][k], sb[c + 8 * j][k], d);
-        acc[j] = fmaf(d, sx * p.sw[((size_t)e * groups + n / FP8_ROWS) * p.kb + b], acc[j]);
+      for (int w = 0; w < FG_THREADS / 32; ++w) {
+        if (w < warp) before += s_sum[w];
+        run += s_sum[w];
       }
+      if (e < p.E) s_pre[e] = (uint16_t)(before + incl - mine);
+      __syncthreads();
     }
+    m_tiles = run;
+    if (tid == 0) s_pre[p.E] = (uint16_t)run;
   }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int n = n0 + c + 8 * j;
-    so[r][c + 8 * j] = acc[j] + (p.bias && owned && n < p.N ? p.bias[(size_t)e * p.N + n] : 0.f);
-  }
+  tc_fence_before();
   __syncthreads();
-  if (r >= rows) return;
-  const bool gated = act_gated(p.act);
-  const float rs = owned ? (p.row_scale ? p.row_scale[row0 + r] : 1.f) : 0.f;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int i = c + 8 * j;
-    float v = so[r][i];
-    int o = n0 + i, on = p.N;
-    if (gated) {
-      if (i >= 16) continue;
-      v = glu_apply(p.act, v, so[r][16 + i], p.act_alpha, p.act_limit);
-      o = n0 / 2 + i; on = p.N / 2;
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  const int tiles = m_tiles * n_tiles;
+  struct Tile { int e, row0, rows, nt; };
+  auto tile = [&](int t) {
+    Tile r;
+    if (banked) {
+      int lo = 0, hi = p.E - 1;                            // the expert with s_pre * n_tiles <= t < the next one's
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (s_pre[mid] * n_tiles <= t) lo = mid; else hi = mid - 1;
+      }
+      const int i = t - s_pre[lo] * n_tiles, mt = s_pre[lo + 1] - s_pre[lo];
+      r.e = lo;
+      r.nt = i / mt;
+      const int m = i - r.nt * mt;
+      r.row0 = p.seg[lo] + m * FG_BM;
+      r.rows = r.row0 < 0 ? 0 : min(min(FG_BM, p.counts[lo] - m * FG_BM), p.M - r.row0);
     } else {
-      v = act_unary<false>(p.act, v, p.act_alpha, p.act_limit);
+      const int full = FG_GROUP * n_tiles, g = t / full, i = t - g * full, gm = min(FG_GROUP, m_tiles - g * FG_GROUP);
+      r.e = 0;
+      r.nt = i / gm;
+      r.row0 = (g * FG_GROUP + i - r.nt * gm) * FG_BM;
+      r.rows = min(FG_BM, p.M - r.row0);
     }
-    if (o >= on) continue;
-    v = owned ? v * rs : 0.f;
-    if (p.out_f32) ((float*)p.C)[(row0 + r) * p.ldc + o] = v;
-    else ((__nv_bfloat16*)p.C)[(row0 + r) * p.ldc + o] = __float2bfloat16(v);
+    return r;
+  };
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    if (warp == 0 && lane == 0) {
+      prefetch_tmap(&tm_x); prefetch_tmap(&tm_w);
+      uint32_t s = 0, ph = 1;
+      bool ok = true;
+      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        const Tile at = tile(t);
+        for (int k = 0; k < p.kb; ++k) {
+          if (!(ok = mbar_wait(bar_empty + 8 * s, ph, p.status, ERR_MBAR_TIMEOUT_PRODUCER, abort_flag))) break;
+          const uint32_t dst = base + s * S::STAGE;
+          mbar_expect_tx(bar_full + 8 * s, S::STAGE);
+          tma_load_2d(dst, &tm_x, bar_full + 8 * s, k * (FP8_BLOCK / 2), at.row0);
+          tma_load_3d(dst + S::A, &tm_w, bar_full + 8 * s, k * (FP8_BLOCK / 2), at.nt * BN, at.e);
+          if (++s == NST) { s = 0; ph ^= 1; }
+        }
+      }
+    } else if (warp == 1 && lane == 0) {
+      constexpr uint32_t idesc = umma_idesc_e4m3(FG_BM, BN);
+      uint32_t s = 0, ph = 0, a = 0, aph = 1;
+      bool ok = true;
+      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x)
+        for (int k = 0; k < p.kb; ++k) {
+          if (!(ok = mbar_wait(bar_tempty + 8 * a, aph, p.status, ERR_MBAR_TIMEOUT_MMA, abort_flag))) break;
+          if (!(ok = mbar_wait(bar_full + 8 * s, ph, p.status, ERR_MBAR_TIMEOUT_MMA, abort_flag))) break;
+          tc_fence_after();
+          const uint64_t dx = umma_desc_k_sw128(base + s * S::STAGE), dw = umma_desc_k_sw128(base + s * S::STAGE + S::A);
+#pragma unroll
+          for (int kk = 0; kk < FP8_BLOCK / 32; ++kk) umma_e4m3(tmem + a * BN, dx + 2 * kk, dw + 2 * kk, idesc, kk != 0);
+          umma_commit(bar_empty + 8 * s);
+          umma_commit(bar_tfull + 8 * a);
+          if (++s == NST) { s = 0; ph ^= 1; }
+          if (++a == ACC) { a = 0; aph ^= 1; }
+        }
+    }
+    __syncwarp();
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    constexpr int HC = BN / 2, G = HC / FP8_ROWS;          // columns of a thread, and the scales that they have
+    const int q = warp & 3, half = (warp - 4) >> 2, sw_groups = (p.N + FP8_ROWS - 1) / FP8_ROWS;
+    uint8_t* const stage = smem_raw + NST * S::STAGE + (warp - 4) * 4096;
+    const bool gated = act_gated(p.act);
+    const int on = gated ? p.N >> 1 : p.N, esz = p.out_f32 ? 4 : 2;
+    const bool wide = (((uintptr_t)p.C) & 15) == 0 && (p.ldc * esz) % 16 == 0;
+    uint32_t a = 0, aph = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      const Tile at = tile(t);
+      const int mine = q * 32 + lane, col0 = at.nt * BN + half * HC;
+      const float* sxp = p.sx + min(at.row0 + mine, p.x_rows - 1);
+      const float* swp[G];
+#pragma unroll
+      for (int g = 0; g < G; ++g) swp[g] = p.sw + ((size_t)at.e * sw_groups + min(col0 / FP8_ROWS + g, sw_groups - 1)) * p.kb;
+      auto fetch_x = [&](int k) { return __ldg(sxp + (size_t)min(k, p.kb - 1) * p.x_rows); };
+      float wv[G], x0 = fetch_x(0), x1 = fetch_x(1), x2 = fetch_x(2);
+      float2 acc[HC / 2];
+#pragma unroll
+      for (int j = 0; j < HC / 2; ++j) acc[j] = make_float2(0.f, 0.f);
+      for (int k = 0; k < p.kb; ++k) {
+        if ((k & 31) == 0) {
+#pragma unroll
+          for (int g = 0; g < G; ++g) wv[g] = __ldg(swp[g] + min(k + lane, p.kb - 1));
+        }
+        const float sx = x0;
+        x0 = x1; x1 = x2; x2 = fetch_x(k + 3);
+        if (!(ok = mbar_wait(bar_tfull + 8 * a, aph, p.status, ERR_MBAR_TIMEOUT_EPILOGUE, abort_flag))) break;
+        tc_fence_after();
+#pragma unroll
+        for (int c0 = 0; c0 < HC; c0 += 32) {
+          uint32_t r[32];
+          tmem_ld_32x32(tmem + ((uint32_t)(q * 32) << 16) + a * BN + half * HC + c0, r);
+          const float s0 = sx * __shfl_sync(0xffffffffu, wv[c0 / 16], k & 31), s1 = sx * __shfl_sync(0xffffffffu, wv[c0 / 16 + 1], k & 31);
+          tmem_ld_wait();
+          if (c0 + 32 == HC) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_tempty + 8 * a);
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float sc = j < 8 ? s0 : s1;
+            acc[c0 / 2 + j] = fma2(make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), make_float2(sc, sc), acc[c0 / 2 + j]);
+          }
+        }
+        if (++a == ACC) { a = 0; aph ^= 1; }
+      }
+      if (!ok) break;
+
+      // ---- the tile: 32 sums at a time to 32 or 16 outputs, collected until a row has 128 bytes
+      const float rs = p.row_scale && mine < at.rows ? p.row_scale[at.row0 + mine] : 1.f;
+      const float* bias = p.bias ? p.bias + (size_t)at.e * p.N : nullptr;
+      int fill = 0, out0 = gated ? col0 >> 1 : col0;
+#pragma unroll
+      for (int g = 0; g < HC / 32; ++g) {
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) { v[2 * j] = acc[16 * g + j].x; v[2 * j + 1] = acc[16 * g + j].y; }
+        if (bias) {
+          const int c = col0 + 32 * g;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] += __ldg(bias + min(c + j, p.N - 1));
+        }
+        if (gated) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] = glu_apply(p.act, v[j], v[16 + j], p.act_alpha, p.act_limit);
+        } else if (p.act) {
+          act_unary_run<false>(p.act, v, p.act_alpha, p.act_limit);
+        }
+        const int n = gated ? 16 : 32;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] *= rs;
+        uint8_t* row = stage + lane * 128;
+        if (p.out_f32) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 4)
+            if (j < n) *reinterpret_cast<float4*>(row + (((fill / 16 + j / 4) ^ (lane & 7)) << 4)) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; j += 8)
+            if (j < n)
+              *reinterpret_cast<uint4*>(row + (((fill / 16 + j / 8) ^ (lane & 7)) << 4)) =
+                  make_uint4(pack_bf16(v[j], v[j + 1]), pack_bf16(v[j + 2], v[j + 3]), pack_bf16(v[j + 4], v[j + 5]), pack_bf16(v[j + 6], v[j + 7]));
+        }
+        fill += n * esz;
+        if (fill == 128 || g + 1 == HC / 32) {
+          __syncwarp();
+          const int n_el = fill / esz;
+          uint8_t* const c = (uint8_t*)p.C + ((size_t)(at.row0 + q * 32) * p.ldc + out0) * esz;
+          const int live = at.rows - q * 32;
+          if (wide && out0 + n_el <= on) {
+            const int per_row = fill / 16, step = 32 / per_row;
+            const int ch = lane % per_row;
+            for (int r = lane / per_row; r < 32; r += step)
+              if (r < live) *reinterpret_cast<uint4*>(c + (size_t)r * p.ldc * esz + ch * 16) = *reinterpret_cast<const uint4*>(stage + r * 128 + ((ch ^ (r & 7)) << 4));
+          } else {
+            for (int r = 0; r < min(32, live); ++r)
+              for (int j = lane; j < n_el && out0 + j < on; j += 32) {
+                const uint8_t* src = stage + r * 128 + (((j * esz / 16) ^ (r & 7)) << 4) + (j * esz) % 16;
+                if (p.out_f32) reinterpret_cast<float*>(c)[(size_t)r * p.ldc + j] = *reinterpret_cast<const float*>(src);
+                else reinterpret_cast<uint16_t*>(c)[(size_t)r * p.ldc + j] = *reinterpret_cast<const uint16_t*>(src);
+              }
+          }
+          __syncwarp();
+          out0 += n_el;
+          fill = 0;
+        }
+      }
+    }
   }
+  if (*abort_flag)                                         // a wait ran out: copies still in flight land before shared memory is released
+    for (int i = 0; i < 200; ++i) __nanosleep(1000);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem, 512); }
+}
+
+template <int BN> static int launch_gemm(const CUtensorMap& tx, const CUtensorMap& tw, const Fp8Params& p, long long tiles, cudaStream_t st) {
+  using S = Fp8GemmShape<BN>;
+  auto kern = fp8_gemm_kernel<BN>;
+  static DeviceOnce configured;
+  if (configured.pending()) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    if (e != cudaSuccess) return (int)e;
+    configured.mark();
+  }
+  launch_pdl(kern, dim3(tiles < sm_count() ? (unsigned)tiles : sm_count()), dim3(FG_THREADS), S::SMEM, st, tx, tw, p);
+  return (int)cudaGetLastError();
 }
 
 }  // namespace mx
 
 using namespace mx;
 
-// M rows of output (dense: rows of x; experts: rows of the packing; slots: slots).  counts / seg: those of the bank's first expert on.
+// Dense (M rows) or experts (counts / seg: from the bank's first expert on; M rows of the packing).  bn: 128 or 256 columns a tile.
 MX_HOST_API int mx_fp8_gemm(const void* x, const float* sx, int x_rows, const void* w, const float* sw, int E, void* c, long long ldc, int out_f32, const float* bias,
-                            const float* row_scale, int act, float act_alpha, float act_limit, int M, int N, int kb, const int* counts, const int* seg, const int* slot,
-                            int x_div, int e_lo, cudaStream_t st) {
+                            const float* row_scale, int act, float act_alpha, float act_limit, int M, int N, int K, const int* counts, const int* seg, int bn,
+                            cudaStream_t st) {
   if (M <= 0 || N <= 0) return 0;
-  if (kb < 1 || x_div < 1 || E < 1) return -101;
+  const int kb = (K + FP8_BLOCK - 1) / FP8_BLOCK;
+  if (K < 1 || E < 1 || E > FG_MAX_E || x_rows < 1 || (bn != 128 && bn != 256)) return -101;
   if (act_gated(act) && N % 32) return -104;
-  Fp8Params p{(const uint8_t*)x, sx, (const uint8_t*)w, sw, c, ldc, out_f32, M, N, kb, x_rows, E, bias, row_scale, act, act_alpha, act_limit, seg, counts, slot, x_div, e_lo};
-  const int tiles = slot ? M : (M + 31) / 32 + (seg ? (E < M ? E : M) : 0);
-  if (tiles > 65535) return -106;
-  launch_pdl(fp8_gemm_kernel, dim3((N + 31) / 32, tiles), dim3(256), 0, st, p);
-  return (int)cudaGetLastError();
+  if (((uintptr_t)x | (uintptr_t)w) & 15) return -114;
+  if (counts && (M + FG_BM - 1) / FG_BM + E > 65535) return -106;
+  const long long tiles = ((M + FG_BM - 1) / FG_BM + (counts ? (E < M ? E : M) : 0)) * (long long)((N + bn - 1) / bn);
+  if (tiles >= 1ll << 31) return -106;
+  Fp8Params p{};
+  p.sx = sx; p.x_rows = x_rows; p.sw = sw; p.C = c; p.ldc = ldc; p.out_f32 = out_f32; p.M = M; p.N = N; p.K = K; p.kb = kb; p.E = E; p.bias = bias; p.row_scale = row_scale;
+  p.act = act; p.act_alpha = act_alpha; p.act_limit = act_limit; p.counts = counts; p.seg = seg; p.x_div = 1; p.status = status_word();
+  CUtensorMap tx, tw;
+  const uint64_t row = (uint64_t)kb * FP8_BLOCK;               // codes travel as two-byte elements: the tile is bytes either way
+  {
+    uint64_t dims[2] = {row / 2, (uint64_t)x_rows}, strides[1] = {row};
+    uint32_t box[2] = {FP8_BLOCK / 2, FG_BM};
+    int r = make_tmap_bf16(&tx, x, 2, dims, strides, box, 1);
+    if (r) return r;
+  }
+  {
+    uint64_t dims[3] = {row / 2, (uint64_t)N, (uint64_t)E}, strides[2] = {row, row * (uint64_t)N};
+    uint32_t box[3] = {FP8_BLOCK / 2, (uint32_t)bn, 1};
+    int r = make_tmap_bf16(&tw, w, 3, dims, strides, box, 1);
+    if (r) return r;
+  }
+  return bn == 256 ? launch_gemm<256>(tx, tw, p, tiles, st) : launch_gemm<128>(tx, tw, p, tiles, st);
 }

@@ -1,0 +1,494 @@
+// Products of a few e4m3 rows (up to 128 together) with e4m3 weights, bound by reading the weights: a dense layer of a decode batch, an expert's few rows, a slot's one row.
+//   y[m, n] = act(sum_b sx[b][m] sw[n / 16][b] sum_{k in b} x8[m][k] w8[n][k] + bias[n])
+//
+// The weights are the M side of tcgen05.mma (128 weight rows x 128 bytes: one block of K, one TMA box) and the rows its N side, padded to NT = 16 to 128
+// columns; the tensor cores need a small part of the time that the box takes to arrive, whatever NT.  Every block has scales of its own, so its sums go from
+// TMEM to registers, where a thread owns a weight row and adds s_x s_w times them to NT sums in fp32.
+//   warp 0      TMA: weight boxes (and boxes of codes, where the rows have been rounded before) into a ring of NST stages
+//   warp 1      tcgen05.mma from one thread into a ring of ACC accumulators
+//   warps 2-5   32 weight rows each: scale and add, epilogue
+//   warps 6-    the rows' side of a stage: bf16 rows are read ahead into registers, rounded to e4m3 and put into the swizzled tile with their scales, so that a
+//               decode step needs no launch for it; rows that have been rounded: their scales
+// The work is the list of (group of rows, 128 weight rows, block of K) laid end to end, of which every CTA takes an equal run.  A tile that is cut leaves fp32
+// partials (at most two per CTA); the warp that arrives last adds them in the order of the CTAs, so results do not depend on timing.
+// Every mbarrier wait is bounded.
+#include "act.cuh"
+#include "common.cuh"
+#include "fp8.cuh"
+#include "host_util.h"
+
+namespace mx {
+
+constexpr int FS_TILE = 128;             // weight rows per tile
+constexpr int FS_W = FS_TILE * FP8_BLOCK;
+constexpr int FS_MAX_E = 1024;
+constexpr int FS_MAX_GRID = CUT_TICKETS / 4;
+
+template <int NT, bool ROUND> struct Fp8StreamShape {
+  static constexpr int X = NT * FP8_BLOCK;
+  static constexpr int STAGE = FS_W + X;
+  // up to 64 columns the next launch's CTA fits beside this one's and fetches its first weights while this one drains
+  static constexpr int LIMIT = (NT <= 64 ? 108 : 200) * 1024;
+  static constexpr int NST = LIMIT / STAGE < 8 ? LIMIT / STAGE : 8;
+  static constexpr int SMEM = NST * STAGE + 1024;
+  static constexpr int ACC = NT <= 32 ? 4 : NT == 64 ? 4 : 2;
+  static constexpr int TMEM = NT * ACC;  // 64, 128, 256, 256 columns
+  // warps of the rows' side.  Registers are shared out by the warps of a quarter of the SM, so eight warps leave an epilogue thread 255 of them (twice eight: 128),
+  // and ten only 168
+  static constexpr int RW = !ROUND ? 1 : NT <= 32 ? 2 : 4;
+  static constexpr int THREADS = 192 + 32 * RW;
+  static constexpr int AHEAD = NT <= 16 ? 4 : NT <= 32 ? 2 : 1;      // units whose bf16 rows are in registers ahead of their use
+};
+
+// A run of `per` units for every CTA; shorter runs would cost more in partial sums than they gain.
+__host__ __device__ inline int fp8_run(int total, int grid) {
+  const int per = (total - 1) / grid + 1;
+  return per < 2 ? 2 : per;
+}
+
+template <int NT, bool ROUND>
+__global__ void __launch_bounds__(Fp8StreamShape<NT, ROUND>::THREADS, NT <= 32 ? 2 : 1)
+fp8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const Fp8Params p) {
+  using S = Fp8StreamShape<NT, ROUND>;
+  constexpr int NST = S::NST, ACC = S::ACC, RW = S::RW, FS_THREADS = S::THREADS;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t s_bar[2 * NST + 2 * ACC];
+  __shared__ __align__(16) float s_sx[NST][NT];
+  __shared__ uint16_t s_pre[FS_MAX_E + 1];
+  __shared__ int s_sum[FS_THREADS / 32];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_abort;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* const smem = smem_raw + (base - smem_u32(smem_raw));
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t bar_full = smem_u32(s_bar), bar_empty = bar_full + 8 * NST, bar_tfull = bar_empty + 8 * NST, bar_tempty = bar_tfull + 8 * ACC;
+  volatile int* abort_flag = &s_abort;
+  if (tid == 0) {
+    for (int s = 0; s < NST; ++s) {
+      mbar_init(bar_full + 8 * s, 1 + RW);             // the TMA thread, the row warps
+      mbar_init(bar_empty + 8 * s, 1 + 4);             // the products, four epilogue warps (they read the scales)
+    }
+    for (int a = 0; a < ACC; ++a) { mbar_init(bar_tfull + 8 * a, 1); mbar_init(bar_tempty + 8 * a, 4); }
+    s_abort = 0;
+    fence_mbar_init();
+  }
+  if (ROUND) {                                         // rows that no group fills stay zero
+    for (int i = tid; i < NST * S::X / 16; i += FS_THREADS)
+      *reinterpret_cast<uint4*>(smem + (i / (S::X / 16)) * S::STAGE + FS_W + (i % (S::X / 16)) * 16) = make_uint4(0, 0, 0, 0);
+    fence_proxy_async();
+  }
+  for (int i = tid; i < NST * NT; i += FS_THREADS) (&s_sx[0][0])[i] = 0.f;
+
+  // ---- the list of work
+  const bool banked = p.counts != nullptr;
+  const int n_tiles = (p.N + FS_TILE - 1) / FS_TILE;
+  int groups = p.slot ? p.M : 1;
+  if (banked) {
+    pdl_wait();
+    int run = 0;
+    for (int e0 = 0; e0 < p.E; e0 += FS_THREADS) {
+      const int e = e0 + tid;
+      int incl = e < p.E ? (p.counts[e] + NT - 1) / NT : 0;
+      const int mine = incl;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += u;
+      }
+      if (lane == 31) s_sum[warp] = incl;
+      __syncthreads();
+      int before = run;
+#pragma unroll
+      for (int w = 0; w < FS_THREADS / 32; ++w) {
+        if (w < warp) before += s_sum[w];
+        run += s_sum[w];
+      }
+      if (e < p.E) s_pre[e] = (uint16_t)(before + incl - mine);
+      __syncthreads();
+    }
+    groups = run;
+    if (tid == 0) s_pre[p.E] = (uint16_t)run;
+  }
+  __syncthreads();
+  const int total = groups * n_tiles * p.kb;
+  const int per = fp8_run(total, (int)gridDim.x);
+  const int my0 = min((long long)total, (long long)blockIdx.x * per), my1 = min(total, my0 + per);
+
+  // a unit of the list: group (expert e, output rows row0 .. row0 + rows - 1), tile nt, block k
+  struct Place { int g, e, row0, rows, nt, k; };
+  auto group = [&](Place& r) {                         // what r.g is
+    if (p.slot) {
+      r.row0 = r.g; r.rows = 1;
+      r.e = p.slot[r.g] - p.e_lo;
+    } else if (banked) {
+      int lo = 0, hi = p.E - 1;                        // the expert with s_pre <= g < the next one's
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (s_pre[mid] <= r.g) lo = mid; else hi = mid - 1;
+      }
+      const int c = r.g - s_pre[lo];
+      r.e = lo;
+      r.row0 = p.seg[lo] + c * NT;
+      r.rows = r.row0 < 0 ? 0 : min(min(NT, p.counts[lo] - c * NT), p.M - r.row0);
+    } else {
+      r.e = 0; r.row0 = 0; r.rows = p.M;
+    }
+  };
+  auto place = [&](int pos) {
+    Place r;
+    const int t = pos / p.kb;
+    r.k = pos - t * p.kb;
+    r.g = t / n_tiles;
+    r.nt = t - r.g * n_tiles;
+    group(r);
+    return r;
+  };
+  auto next_tile = [&](Place& r, bool any) {           // (any: there is one)
+    r.k = 0;
+    if (++r.nt == n_tiles) {
+      r.nt = 0; ++r.g;
+      if (any) group(r);
+    }
+  };
+  const bool early = !banked && !p.slot;               // which weights are read does not depend on the launch before
+
+  if (warp == 0) {
+    // ------------------------------------------------ TMA
+    if (lane == 0 && my0 < my1) {
+      prefetch_tmap(&tm_w);
+      if (!ROUND) prefetch_tmap(&tm_x);
+      if (!early && !banked) pdl_wait();
+      auto load_w = [&](int s, const Place& at) {
+        mbar_expect_tx(bar_full + 8 * s, ROUND ? FS_W : S::STAGE);
+        tma_load_3d(base + s * S::STAGE, &tm_w, bar_full + 8 * s, at.k * (FP8_BLOCK / 2), at.nt * FS_TILE, min(max(at.e, 0), p.E - 1));
+      };
+      Place at = place(my0), w = at;
+      int ahead = 0, pos = my0;
+      auto next = [&](Place& r, int i) {
+        if (++r.k == p.kb) next_tile(r, i + 1 < my1);
+      };
+      if (early) {
+        for (; ahead < NST && my0 + ahead < my1; ++ahead) { load_w(ahead, w); next(w, my0 + ahead); }
+        pdl_wait();
+      }
+      uint32_t s = 0, ph = 1;
+      for (; pos < my1; ++pos) {
+        if (pos - my0 >= ahead) {
+          if (!mbar_wait(bar_empty + 8 * s, ph, p.status, ERR_MBAR_TIMEOUT_PRODUCER, abort_flag)) break;
+          load_w(s, at);
+        }
+        if (!ROUND) tma_load_2d(base + s * S::STAGE + FS_W, &tm_x, bar_full + 8 * s, at.k * (FP8_BLOCK / 2), p.slot ? at.row0 / p.x_div : at.row0);
+        if (++s == NST) { s = 0; ph ^= 1; }
+        next(at, pos);
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------ products
+    // Tensor memory is taken when the launch before has ended: it may still want some, and would wait for a CTA that waits for it.  For the same reason the next
+    // launch's CTAs may come only now.
+    if (!banked) pdl_wait();
+    tmem_alloc(smem_u32(&s_tmem), S::TMEM);
+    tmem_relinquish();
+    pdl_launch_dependents();
+    tc_fence_before();
+    asm volatile("bar.sync 1, 160;" ::: "memory");
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    if (lane == 0) {
+      constexpr uint32_t idesc = umma_idesc_e4m3(FS_TILE, NT);
+      uint32_t s = 0, ph = 0, a = 0, aph = 1;
+      for (int pos = my0; pos < my1; ++pos) {
+        if (!mbar_wait(bar_tempty + 8 * a, aph, p.status, ERR_MBAR_TIMEOUT_MMA, abort_flag)) break;
+        if (!mbar_wait(bar_full + 8 * s, ph, p.status, ERR_MBAR_TIMEOUT_MMA, abort_flag)) break;
+        tc_fence_after();
+        const uint64_t dw = umma_desc_k_sw128(base + s * S::STAGE), dx = umma_desc_k_sw128(base + s * S::STAGE + FS_W);
+#pragma unroll
+        for (int kk = 0; kk < FP8_BLOCK / 32; ++kk) umma_e4m3(tmem + a * NT, dw + 2 * kk, dx + 2 * kk, idesc, kk != 0);
+        umma_commit(bar_empty + 8 * s);
+        umma_commit(bar_tfull + 8 * a);
+        if (++s == NST) { s = 0; ph ^= 1; }
+        if (++a == ACC) { a = 0; aph ^= 1; }
+      }
+    }
+  } else if (warp < 6) {
+    // ------------------------------------------------ scales, sums, epilogue: a thread owns weight row `n`
+    const int q = warp & 3, sw_groups = (p.N + FP8_ROWS - 1) / FP8_ROWS;
+    asm volatile("bar.sync 1, 160;" ::: "memory");
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    if (!banked) pdl_wait();
+    uint32_t s = 0, ph = 0, a = 0, aph = 0;
+    bool ok = true;
+    Place at;
+    if (my0 < my1) at = place(my0);
+    for (int pos = my0; ok && pos < my1;) {
+      const int first = at.k, n_units = min(my1 - pos, p.kb - at.k);
+      const int n = at.nt * FS_TILE + q * 32 + lane;
+      const int e = min(max(at.e, 0), p.E - 1);
+      // scales of 16 blocks at a time, one per lane of the half-warp that shares a group of rows
+      const float* swp = p.sw + ((size_t)e * sw_groups + min(n / FP8_ROWS, sw_groups - 1)) * p.kb;
+      auto fetch = [&](int k) { return __ldg(swp + min(k + (lane & 15), p.kb - 1)); };
+      float wv = fetch(first), wn = first + 16 < p.kb ? fetch(first + 16) : 0.f;
+      float2 acc[NT / 2];
+#pragma unroll
+      for (int j = 0; j < NT / 2; ++j) acc[j] = make_float2(0.f, 0.f);
+      for (int i = 0; i < n_units; ++i) {
+        if (i && (i & 15) == 0) {
+          wv = wn;
+          if (i + 16 < n_units) wn = fetch(first + i + 16);
+        }
+        const float sw = __shfl_sync(0xffffffffu, wv, (lane & 16) | (i & 15));
+        // the scales of the rows: written by the row warps before they arrived at the stage's barrier
+        if (!(ok = mbar_wait(bar_full + 8 * s, ph, p.status, ERR_MBAR_TIMEOUT_EPILOGUE, abort_flag))) break;
+        if (!(ok = mbar_wait(bar_tfull + 8 * a, aph, p.status, ERR_MBAR_TIMEOUT_EPILOGUE, abort_flag))) break;
+        tc_fence_after();
+        const float4* sx = reinterpret_cast<const float4*>(s_sx[s]);
+        constexpr int C = NT < 32 ? NT : 32;
+#pragma unroll
+        for (int c0 = 0; c0 < NT; c0 += C) {
+          uint32_t r[C];
+          tmem_ld_cols<C>(tmem + ((uint32_t)(q * 32) << 16) + a * NT + c0, r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < C; j += 4) {
+            const float4 t = sx[(c0 + j) / 4];
+            float2& u = acc[(c0 + j) / 2];
+            float2& v = acc[(c0 + j) / 2 + 1];
+            u = fma2(make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), mul2(make_float2(t.x, t.y), make_float2(sw, sw)), u);
+            v = fma2(make_float2(__uint_as_float(r[j + 2]), __uint_as_float(r[j + 3])), mul2(make_float2(t.z, t.w), make_float2(sw, sw)), v);
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) { mbar_arrive(bar_tempty + 8 * a); mbar_arrive(bar_empty + 8 * s); }
+        if (++s == NST) { s = 0; ph ^= 1; }
+        if (++a == ACC) { a = 0; aph ^= 1; }
+      }
+      if (!ok) break;
+
+      // ---- a cut tile: partials, and the last warp to arrive adds them up
+      bool mine_to_finish = true;
+      if (n_units < p.kb) {
+        const int t0 = pos - first, c0 = t0 / per, c1 = (t0 + p.kb - 1) / per;
+        float4* part = reinterpret_cast<float4*>(p.part);
+        auto slab = [&](int c) { return part + (((size_t)c * 2 + (c == c0 ? 1 : 0)) * 4 + q) * (NT / 4 * 32) + lane; };
+        float4* mine = slab(blockIdx.x);
+#pragma unroll
+        for (int j = 0; j < NT / 4; ++j)
+          if (4 * j < at.rows) mine[j * 32] = make_float4(acc[2 * j].x, acc[2 * j].y, acc[2 * j + 1].x, acc[2 * j + 1].y);
+        __threadfence();
+        __syncwarp();
+        int prev = 0;
+        if (lane == 0) {
+          prev = atomicAdd(p.tickets + c0 * 4 + q, 1);
+          if (prev == c1 - c0) p.tickets[c0 * 4 + q] = 0;
+        }
+        prev = __shfl_sync(0xffffffffu, prev, 0);
+        mine_to_finish = prev == c1 - c0;
+        if (mine_to_finish) {
+          __threadfence();
+#pragma unroll
+          for (int j = 0; j < NT / 2; ++j) acc[j] = make_float2(0.f, 0.f);
+          for (int c = c0; c <= c1; ++c) {
+            const float4* src = slab(c);
+#pragma unroll
+            for (int j = 0; j < NT / 4; ++j)
+              if (4 * j < at.rows) {
+                const float4 v = __ldcg(src + j * 32);
+                acc[2 * j].x += v.x; acc[2 * j].y += v.y; acc[2 * j + 1].x += v.z; acc[2 * j + 1].y += v.w;
+              }
+          }
+        }
+      }
+      if (mine_to_finish) {
+        // ---- epilogue: gate rows are lanes 0-15, their up rows lanes 16-31
+        const bool gated = act_gated(p.act), owned = at.e >= 0 && at.e < p.E;
+        const float bias = p.bias && n < p.N ? p.bias[(size_t)e * p.N + n] : 0.f;
+        const int on = gated ? p.N >> 1 : p.N, o = gated ? at.nt * (FS_TILE / 2) + q * 16 + (lane & 15) : n;
+        const bool write = o < on && (!gated || lane < 16);
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+          if (j < at.rows) {
+            float v = (j & 1 ? acc[j / 2].y : acc[j / 2].x) + bias;
+            if (gated) v = glu_apply(p.act, v, __shfl_down_sync(0xffffffffu, v, 16), p.act_alpha, p.act_limit);
+            else if (p.act) v = act_unary<false>(p.act, v, p.act_alpha, p.act_limit);
+            const int row = at.row0 + j;
+            if (p.row_scale) v *= p.row_scale[row];
+            if (!owned) v = 0.f;
+            if (write) {
+              if (p.out_f32) ((float*)p.C)[row * p.ldc + o] = v;
+              else ((__nv_bfloat16*)p.C)[row * p.ldc + o] = __float2bfloat16(v);
+            }
+          }
+      }
+      pos += n_units;
+      next_tile(at, pos < my1);
+    }
+  } else {
+    // ------------------------------------------------ the rows' side of the stages
+    const int rw = warp - 6;
+    if (!banked) pdl_wait();
+    if (my0 < my1) {
+      uint32_t s = 0, ph = 1;
+      if constexpr (ROUND) {
+        constexpr int R = NT / RW, D = S::AHEAD;         // rows of a warp: rw, rw + RW, ..
+        const bool vec = p.ldx % 4 == 0 && ((uintptr_t)p.xb & 7) == 0;
+        uint2 raw[D][R];
+        auto row_of = [&](const Place& r, int j) { return p.slot ? r.row0 / p.x_div : p.x_index ? p.x_index[r.row0 + j] : r.row0 + j; };
+        const int skip = 4 * lane;
+        auto load = [&](uint2 (&v)[R], const Place& r) {
+#pragma unroll
+          for (int j = 0; j < R; ++j) {
+            v[j] = make_uint2(0, 0);
+            if (rw + RW * j >= r.rows) continue;
+            const int src = row_of(r, rw + RW * j);
+            if (src < 0) continue;
+            if (src >= p.x_rows) { v[j] = make_uint2(0x7fc07fc0u, 0x7fc07fc0u); continue; }       // no such row: NaN
+            const __nv_bfloat16* at = p.xb + src * p.ldx + r.k * FP8_BLOCK + skip;
+            const int left = p.K - r.k * FP8_BLOCK - skip;
+            if (vec && left >= 4) {
+              v[j] = __ldg(reinterpret_cast<const uint2*>(at));
+            } else {
+              const uint16_t* h = reinterpret_cast<const uint16_t*>(at);
+              const uint32_t a = left > 0 ? h[0] : 0, b = left > 1 ? h[1] : 0, c = left > 2 ? h[2] : 0, d = left > 3 ? h[3] : 0;
+              v[j] = make_uint2(a | b << 16, c | d << 16);
+            }
+          }
+        };
+        Place at = place(my0), pf = at;
+        int pf_pos = my0;
+        auto advance = [&](Place& r, int pos) { if (++r.k == p.kb) next_tile(r, pos + 1 < my1); };
+#pragma unroll
+        for (int d = 0; d < D; ++d)
+          if (pf_pos < my1) { load(raw[d], pf); advance(pf, pf_pos); ++pf_pos; }
+        bool ok = true;
+        for (int pos = my0; ok && pos < my1;) {
+#pragma unroll
+          for (int d = 0; d < D; ++d) {
+            if (!ok || pos >= my1) continue;
+            if (!(ok = mbar_wait(bar_empty + 8 * s, ph, p.status, ERR_MBAR_TIMEOUT_DEQUANT, abort_flag))) continue;
+            uint8_t* tile = smem + s * S::STAGE + FS_W;
+#pragma unroll
+            for (int j = 0; j < R; ++j) {
+              const int r = rw + RW * j;
+              if (r >= at.rows) continue;
+              const float v0 = bf16_lo(raw[d][j].x), v1 = bf16_hi(raw[d][j].x), v2 = bf16_lo(raw[d][j].y), v3 = bf16_hi(raw[d][j].y);
+              const uint32_t m = __reduce_max_sync(0xffffffffu, max(max(fp8_mag(v0), fp8_mag(v1)), max(fp8_mag(v2), fp8_mag(v3))));
+              float inv;
+              const float sc = fp8_scale(__uint_as_float(m), &inv);
+              const uint32_t word = m >= 0x7f800000u ? 0u : fp8_pack4(v0 * inv, v1 * inv, v2 * inv, v3 * inv);
+              *reinterpret_cast<uint32_t*>(tile + sw128_offset(r, lane >> 2) + (lane & 3) * 4) = word;
+              if (lane == 0) s_sx[s][r] = sc;
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_full + 8 * s);
+            if (++s == NST) { s = 0; ph ^= 1; }
+            advance(at, pos);
+            ++pos;
+            if (pf_pos < my1) { load(raw[d], pf); advance(pf, pf_pos); ++pf_pos; }
+          }
+        }
+      } else {
+        // scales of the rows: columns lane, lane + 32, .. of the stage
+        constexpr int D = 4, C = (NT + 31) / 32;
+        Place at = place(my0), pf = at;
+        int pf_pos = my0;
+        float v[D][C];
+        auto advance = [&](Place& r, int pos) { if (++r.k == p.kb) next_tile(r, pos + 1 < my1); };
+        auto load = [&](float (&t)[C], const Place& r) {
+#pragma unroll
+          for (int c = 0; c < C; ++c) {
+            const int j = c * 32 + lane;
+            t[c] = j < r.rows ? __ldg(p.sx + (size_t)r.k * p.x_rows + (p.slot ? r.row0 / p.x_div : r.row0 + j)) : 0.f;
+          }
+        };
+#pragma unroll
+        for (int d = 0; d < D; ++d)
+          if (pf_pos < my1) { load(v[d], pf); advance(pf, pf_pos); ++pf_pos; }
+        bool ok = true;
+        for (int pos = my0; ok && pos < my1;) {
+#pragma unroll
+          for (int d = 0; d < D; ++d) {
+            if (!ok || pos >= my1) continue;
+            if (!(ok = mbar_wait(bar_empty + 8 * s, ph, p.status, ERR_MBAR_TIMEOUT_DEQUANT, abort_flag))) continue;
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+              if (c * 32 + lane < NT) s_sx[s][c * 32 + lane] = v[d][c];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_full + 8 * s);
+            if (++s == NST) { s = 0; ph ^= 1; }
+            ++pos;
+            if (pf_pos < my1) { load(v[d], pf); advance(pf, pf_pos); ++pf_pos; }
+          }
+        }
+      }
+    }
+  }
+  if (*abort_flag)                                         // a wait ran out: copies still in flight land before shared memory is released
+    for (int i = 0; i < 200; ++i) __nanosleep(1000);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) { tc_fence_after(); tmem_dealloc(s_tmem, S::TMEM); }
+}
+
+template <int NT, bool ROUND> static int launch_stream(const CUtensorMap& tw, const CUtensorMap& tx, const Fp8Params& p, cudaStream_t st) {
+  using S = Fp8StreamShape<NT, ROUND>;
+  auto kern = fp8_stream_kernel<NT, ROUND>;
+  static DeviceOnce configured;
+  if (configured.pending()) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    if (e != cudaSuccess) return (int)e;
+    configured.mark();
+  }
+  const int grid = sm_count() < FS_MAX_GRID ? sm_count() : FS_MAX_GRID;
+  launch_pdl(kern, dim3(grid), dim3(S::THREADS), S::SMEM, st, tw, tx, p);
+  return (int)cudaGetLastError();
+}
+
+}  // namespace mx
+
+using namespace mx;
+
+// Floats of scratch (16-byte aligned) that mx_fp8_stream wants for groups of up to `nt` rows.
+MX_HOST_API int mx_fp8_stream_scratch(int nt) { return FS_MAX_GRID * 2 * FS_TILE * nt; }
+
+// Whether the units of a launch can be counted: `groups` is the most there can be.
+MX_HOST_API int mx_fp8_stream_takes(long long groups, int N, int kb, int E) {
+  return E <= FS_MAX_E && groups < 65536 && groups * ((N + FS_TILE - 1) / FS_TILE) * kb < (1ll << 30);
+}
+
+// Dense (M <= nt), experts (counts / seg: from the bank's first expert on) or slots (slot).  nt 16, 32, 64 or 128: rows of a group, padded.  xb: bf16 rows, rounded on the
+// way (nt <= 64); null: codes x and scales sx of x_rows rows.  tickets: see host_util.h.
+MX_HOST_API int mx_fp8_stream(const void* x, const float* sx, const void* xb, long long ldx, const int* x_index, int x_rows, const void* w, const float* sw, int E, void* c,
+                              long long ldc, int out_f32, const float* bias, const float* row_scale, int act, float act_alpha, float act_limit, int M, int N, int K,
+                              const int* counts, const int* seg, const int* slot, int x_div, int e_lo, int nt, float* scratch, int* tickets, cudaStream_t st) {
+  if (M <= 0 || N <= 0) return 0;
+  const int kb = (K + FP8_BLOCK - 1) / FP8_BLOCK;
+  if (K < 1 || x_div < 1 || E < 1 || x_rows < 1) return -101;
+  if (act_gated(act) && N % 32) return -104;
+  const long long groups = slot ? M : counts ? (long long)M / nt + (E < M ? E : M) + 1 : 1;
+  if (!mx_fp8_stream_takes(groups, N, kb, E) || (!slot && !counts && M > nt) || (xb && nt > 64)) return -106;
+  if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)scratch) & 15) return -114;
+  Fp8Params p{(const __nv_bfloat16*)xb, ldx, x_index, sx, x_rows, sw, c, ldc, out_f32, M, N, K, kb, E, bias, row_scale, act, act_alpha, act_limit, counts, seg, slot, x_div,
+              e_lo, scratch, tickets, status_word()};
+  CUtensorMap tw, tx;
+  const uint64_t row = (uint64_t)kb * FP8_BLOCK;               // codes travel as two-byte elements: the tile is bytes either way
+  {
+    uint64_t dims[3] = {row / 2, (uint64_t)N, (uint64_t)E}, strides[2] = {row, row * (uint64_t)N};
+    uint32_t box[3] = {FP8_BLOCK / 2, FS_TILE, 1};
+    int r = make_tmap_bf16(&tw, w, 3, dims, strides, box, 1);
+    if (r) return r;
+  }
+  tx = tw;
+  if (!xb) {
+    uint64_t dims[2] = {row / 2, (uint64_t)x_rows}, strides[1] = {row};
+    uint32_t box[2] = {FP8_BLOCK / 2, (uint32_t)nt};
+    int r = make_tmap_bf16(&tx, x, 2, dims, strides, box, 1);
+    if (r) return r;
+  }
+#define MX_FS(NT_) if (nt == NT_) return xb ? launch_stream<NT_, NT_ <= 64>(tw, tx, p, st) : launch_stream<NT_, false>(tw, tx, p, st)
+  MX_FS(16); MX_FS(32); MX_FS(64); MX_FS(128);
+#undef MX_FS
+  return -106;
+}

@@ -871,7 +871,7 @@ def expert_gemv(x, w: QuantWeight, slot_expert, x_div=1, bias=None, act=ACT_NONE
         _fp8.check_slots(x, w, slot_expert, x_div, bias, act_gated(act), slot_scale)
         with _on(x.device):
             out = torch.empty(S, n_out, dtype=torch.float32 if out_f32 else torch.bfloat16, device=x.device)
-            return _fp8_gemm(x, w, out, bias, slot_scale, act, act_alpha, act_limit, slot=slot_expert, x_div=x_div, e_lo=e_lo)
+            return _fp8_product(x, w, out, bias, slot_scale, act, act_alpha, act_limit, slot=slot_expert, x_div=x_div, e_lo=e_lo)
     out = torch.empty(S, n_out, dtype=torch.float32 if out_f32 else torch.bfloat16, device=x.device)
     fmt, p0, p1, p2, p3 = _planes(w)
     _check(_lib.cuda().mx_gemv_experts(fmt, p0, p1, p2, p3, _p(x), _p(out), _p(bias), w.N, w.K, int(out_f32), act, C.c_float(act_alpha),
@@ -908,16 +908,54 @@ def fp8_rows(x, index=None) -> FP8Rows:
     return q
 
 
-def _fp8_gemm(x, w: QuantWeight, out, bias, row_scale, act, act_alpha, act_limit, counts=None, seg=None, slot=None, x_div=1, e_lo=0, index=None):
+FP8_STREAM_ROWS = (16, 32, 64, 128)      # rows of a group in the weight-streaming kernel
+FP8_ROUND_ROWS = 64                      # bf16 rows are rounded inside it up to groups of this many
+
+
+def _fp8_stream(x, w: QuantWeight, out, bias, row_scale, act, act_alpha, act_limit, nt, counts=None, seg=None, slot=None, x_div=1, e_lo=0, index=None):
+    """The weight-streaming kernel (csrc/cuda/fp8_stream.cu) with groups of up to ``nt`` rows."""
+    lib = _lib.cuda()
+    if not isinstance(x, FP8Rows) and nt > FP8_ROUND_ROWS:
+        x, index = fp8_rows(x, index), None
+    rounded = isinstance(x, FP8Rows)
+    scratch = torch.empty(lib.mx_fp8_stream_scratch(nt), dtype=torch.float32, device=out.device)
+    tickets = _tickets(out.device)
+    null = _vp(0)
+    _check(lib.mx_fp8_stream(_p(x.codes) if rounded else null, _p(x.scale) if rounded else null, null if rounded else _p(x), C.c_longlong(0 if rounded else x.stride(0)),
+                             _p(index), x.shape[0], _p(w.p0), _p(w.p1), w.E, _p(out), C.c_longlong(out.stride(0)), int(out.dtype == torch.float32), _p(bias), _p(row_scale),
+                             act, C.c_float(act_alpha), C.c_float(act_limit), out.shape[0], w.N, w.K, _p(counts), _p(seg), _p(slot), int(x_div), int(e_lo), nt, _p(scratch),
+                             tickets[1], tickets[2]), "fp8_stream")
+    _count()
+    return out
+
+
+def _fp8_tiles(x, w: QuantWeight, out, bias, row_scale, act, act_alpha, act_limit, bn, counts=None, seg=None, index=None):
+    """The tiled kernel (csrc/cuda/fp8_gemm.cu) with ``bn`` columns a tile."""
+    q = x if isinstance(x, FP8Rows) else fp8_rows(x, index)
+    _check(_lib.cuda().mx_fp8_gemm(_p(q.codes), _p(q.scale), q.codes.shape[0], _p(w.p0), _p(w.p1), w.E, _p(out), C.c_longlong(out.stride(0)), int(out.dtype == torch.float32),
+                                   _p(bias), _p(row_scale), act, C.c_float(act_alpha), C.c_float(act_limit), out.shape[0], w.N, w.K, _p(counts), _p(seg), bn, _stream()),
+           "fp8_gemm")
+    _count()
+    return out
+
+
+def _fp8_bn(M: int, N: int) -> int:
+    sms = sm_count()
+    waves = lambda bn: -(-(-(-M // 128) * -(-N // bn)) // sms)
+    return 256 if 1.9 * waves(256) < waves(128) else 128
+
+
+def _fp8_product(x, w: QuantWeight, out, bias, row_scale, act, act_alpha, act_limit, counts=None, seg=None, slot=None, x_div=1, e_lo=0, index=None):
     M = out.shape[0]
     if M == 0:
         return out
-    q = x if isinstance(x, FP8Rows) else fp8_rows(x, index)
-    _check(_lib.cuda().mx_fp8_gemm(_p(q.codes), _p(q.scale), q.codes.shape[0], _p(w.p0), _p(w.p1), w.E, _p(out), C.c_longlong(out.stride(0)),
-                                   int(out.dtype == torch.float32), _p(bias), _p(row_scale), act, C.c_float(act_alpha), C.c_float(act_limit), M, w.N, w.p1.shape[2],
-                                   _p(counts), _p(seg), _p(slot), int(x_div), int(e_lo), _stream()), "fp8_gemm")
-    _count()
-    return out
+    if slot is not None:
+        return _fp8_stream(x, w, out, bias, row_scale, act, act_alpha, act_limit, 16, slot=slot, x_div=x_div, e_lo=e_lo)
+    rows = M if counts is None else 2 * M / w.E
+    nt = next((n for n in FP8_STREAM_ROWS if rows <= n), 0)
+    if nt:
+        return _fp8_stream(x, w, out, bias, row_scale, act, act_alpha, act_limit, nt, counts=counts, seg=seg, index=index)
+    return _fp8_tiles(x, w, out, bias, row_scale, act, act_alpha, act_limit, _fp8_bn(M, w.N), counts=counts, seg=seg, index=index)
 
 
 def _linear_fp8(x, w: QuantWeight, bias, act, act_alpha, act_limit, out_f32, row_scale, out):
@@ -927,7 +965,7 @@ def _linear_fp8(x, w: QuantWeight, bias, act, act_alpha, act_limit, out_f32, row
     with _on(x.device):
         if out is None:
             out = torch.empty(M, n_out, dtype=odt, device=x.device)
-        return _fp8_gemm(x, w, out, bias, row_scale, act, act_alpha, act_limit)
+        return _fp8_product(x, w, out, bias, row_scale, act, act_alpha, act_limit)
 
 
 def expert_linear(x, w: QuantWeight, pk: MoePacking, x_index=None, bias=None, act=ACT_NONE, act_alpha=1.702, act_limit=7.0, out_f32=False, e_lo=0):
@@ -936,7 +974,7 @@ def expert_linear(x, w: QuantWeight, pk: MoePacking, x_index=None, bias=None, ac
     _fp8.check_packing(pk, w, x, x_index, e_lo)
     with _on(x.device):
         out = torch.empty(P, n_out, dtype=torch.float32 if out_f32 else torch.bfloat16, device=x.device)
-        return _fp8_gemm(x, w, out, bias, None, act, act_alpha, act_limit, counts=pk.counts[e_lo:], seg=pk.seg_start[e_lo:], index=None if x_index is None else x_index[:P])
+        return _fp8_product(x, w, out, bias, None, act, act_alpha, act_limit, counts=pk.counts[e_lo:], seg=pk.seg_start[e_lo:], index=None if x_index is None else x_index[:P])
 
 
 # ------------------------------------------------------------------ attention

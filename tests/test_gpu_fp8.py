@@ -105,6 +105,50 @@ def test_dense_over_many_tiles(M, N, K):
     assert O.rel(ops.linear(x, w), want) < tolerance(K, bf16=True)
 
 
+def K_():
+    from machx_inference_engine_b200.ops import cuda
+    return cuda
+
+
+@pytest.mark.parametrize("M", [1, 15, 64, 128, 129, 300])
+@pytest.mark.parametrize("N,K", [(1, 1), (257, 2880), (1000, 1024), (544, 515), (4096, 128)])
+def test_each_kernel_at_every_tile_size(M, N, K):
+    """The kernels that the dense layers choose between, at sizes that the choice would give to the other one too."""
+    x, w = acts(M, K), bank(N, K)
+    want = O.row_values(x) @ O.weight_values(w)[0].T
+    bias, rs = torch.randn(N, generator=gen(1)).to(DEV), torch.rand(M, generator=gen(2)).to(DEV)
+    full = (want + bias.cpu().double()) * rs.cpu().double()[:, None]
+    q = ops.fp8_rows(x)
+    for rows in (x, q):
+        for nt in (n for n in K_().FP8_STREAM_ROWS if n >= M):
+            out = torch.empty(M, N, device=DEV)
+            assert O.rel(K_()._fp8_stream(rows, w, out, None, None, 0, 0.0, 0.0, nt), want) < tolerance(K), nt
+            assert O.rel(K_()._fp8_stream(rows, w, out, bias, rs, 0, 0.0, 0.0, nt), full) < tolerance(K), nt
+        for bn in (128, 256):
+            out = torch.empty(M, N, device=DEV)
+            assert O.rel(K_()._fp8_tiles(rows, w, out, None, None, 0, 0.0, 0.0, bn), want) < tolerance(K), bn
+            assert O.rel(K_()._fp8_tiles(rows, w, out, bias, rs, 0, 0.0, 0.0, bn), full) < tolerance(K), bn
+
+
+@pytest.mark.parametrize("act", ["none", "geglu"])
+@pytest.mark.parametrize("T,E,k", [(7, 4, 2), (200, 6, 2), (500, 3, 2), (90, 40, 5)])
+def test_each_kernel_over_experts(T, E, k, act):
+    H, F = 392, 320
+    x, w = acts(T, H), bank(F, H, E)
+    idx = routing(T, E, k, "skewed")
+    pk = ops.moe_pack(idx.to(DEV), E, tile=1)
+    want = O.activate(torch.einsum("pk,pnk->pn", O.row_values(x).repeat_interleave(k, 0), O.weight_values(w)[idx.reshape(-1).long()]), act)
+    kw = dict(counts=pk.counts, seg=pk.seg_start)
+    n = F // 2 if act != "none" else F
+    for rows, index in ((x, pk.packed_token), (ops.fp8_rows(x, index=pk.packed_token), None)):
+        for nt in K_().FP8_STREAM_ROWS:
+            got = K_()._fp8_stream(rows, w, torch.empty(T * k, n, device=DEV), None, None, ACTS[act], 1.702, 7.0, nt, index=index, **kw)
+            assert O.rel(got[pk.pair_to_packed.long()], want) < tolerance(H, act), nt
+        for bn in (128, 256):
+            got = K_()._fp8_tiles(rows, w, torch.empty(T * k, n, device=DEV), None, None, ACTS[act], 1.702, 7.0, bn, index=index, **kw)
+            assert O.rel(got[pk.pair_to_packed.long()], want) < tolerance(H, act), bn
+
+
 @pytest.mark.parametrize("act", ["swiglu", "swiglu_oai", "geglu", "relu2"])
 @pytest.mark.parametrize("M", [1, 8, 19, 64, 130, 513])
 def test_epilogues(M, act):
