@@ -1,6 +1,7 @@
 // Rounding of activations to e4m3 with a power-of-two scale per 128 elements, shared by the quantiser and the products that round their rows themselves.
 #pragma once
 #include "common.cuh"
+#include "host_util.h"
 #include <cuda_fp8.h>
 
 namespace mx {
@@ -68,17 +69,18 @@ template <int N> __device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, ui
   }
 }
 
+// 4 bytes from global to shared memory, asynchronously; `arrive_copies`: the barrier is arrived at when this thread's copies so far have landed.
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory"); }
+__device__ __forceinline__ void arrive_copies(uint32_t bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }
+
 // What a product multiplies and writes.
 struct Fp8Params {
-  const __nv_bfloat16* xb;   // rows to be rounded on the way, `ldx` elements apart; null: codes and scales
-  long long ldx;
-  const int* x_index;        // experts: row of xb that packed row m reads (null: m)
   const float* sx;           // [kb][x_rows]
   int x_rows;
   const float* sw;           // [E][ceil(N / 16)][kb]
   void* C;
   long long ldc;
-  int out_f32, M, N, K, kb, E;
+  int out_f32, M, N, kb, E;
   const float* bias;         // [N] or [E][N]
   const float* row_scale;    // [M]
   int act;
@@ -91,5 +93,13 @@ struct Fp8Params {
   int* tickets;
   int* status;
 };
+
+// Boxes of `rows` rows by one block of codes [E][n][kb * 128] (E = 0: [n][kb * 128]).  Codes travel as two-byte elements: the tile is bytes either way.
+inline int fp8_tmap(CUtensorMap* out, const void* codes, int kb, int n, int E, int rows) {
+  const uint64_t row = (uint64_t)kb * FP8_BLOCK;
+  uint64_t dims[3] = {row / 2, (uint64_t)n, (uint64_t)E}, strides[2] = {row, row * (uint64_t)n};
+  uint32_t box[3] = {FP8_BLOCK / 2, (uint32_t)rows, 1};
+  return make_tmap_bf16(out, codes, E ? 3 : 2, dims, strides, box, 1);
+}
 
 }  // namespace mx

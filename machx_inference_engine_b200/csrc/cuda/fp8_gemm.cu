@@ -7,7 +7,9 @@
 // tensor cores fill the next accumulator.
 //   warp 0      TMA loads into a ring of NST stages
 //   warp 1      tcgen05.mma from one thread into a ring of 512 / BN accumulators
-//   warps 4-11  sums (warp & 3: rows, warp / 8: half of the columns); a finished tile goes through shared memory, so that rows are written in runs of 128 bytes
+//   warps 2, 3  asynchronous copies of the block's scales (128 of the rows, BN / 16 of the weights) into a ring.  Loads into registers would be waited for one block
+//               ahead at most, whatever the distance: they share the counters by which a warp waits
+//   warps 4-11  sums (warp & 3: rows, warp / 8: half of the columns); a finished tile goes through shared memory, so that rows are written in runs of 64 bytes
 // Every mbarrier wait is bounded.
 #include "act.cuh"
 #include "common.cuh"
@@ -21,10 +23,13 @@ constexpr int FG_GROUP = 8;                                // m-tiles that are w
 
 template <int BN> struct Fp8GemmShape {
   static constexpr int A = FG_BM * FP8_BLOCK, B = BN * FP8_BLOCK, STAGE = A + B;
-  static constexpr int OUT = 8 * 4096;                     // 32 rows x 128 bytes for each warp
+  static constexpr int OUT = 8 * 2048;                     // 32 rows x 64 bytes for each warp
   static constexpr int NST = 192 * 1024 / STAGE;
   static constexpr int ACC = 512 / BN;
+  // A slot of scales is free again when the products of the block NST before are done, since they waited for the sums of the block ACC before them.
+  static constexpr int RING = NST + ACC, SC = FG_BM + BN / FP8_ROWS;
   struct Small {                                           // what is not tiles, behind them
+    alignas(16) float scale[RING][SC];
     uint64_t bar[2 * NST + 2 * ACC];
     int sum[12];
     uint32_t tmem;
@@ -56,8 +61,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
   const uint32_t bar_full = smem_u32(s_bar), bar_empty = bar_full + 8 * NST, bar_tfull = bar_empty + 8 * NST, bar_tempty = bar_tfull + 8 * ACC;
   volatile int* abort_flag = &s_abort;
   if (tid == 0) {
-    for (int s = 0; s < NST; ++s) { mbar_init(bar_full + 8 * s, 1); mbar_init(bar_empty + 8 * s, 1); }
-    for (int a = 0; a < ACC; ++a) { mbar_init(bar_tfull + 8 * a, 1); mbar_init(bar_tempty + 8 * a, 8); }
+    for (int s = 0; s < NST; ++s) { mbar_init(bar_full + 8 * s, 1 + 64); mbar_init(bar_empty + 8 * s, 1); }
+    for (int a = 0; a < ACC; ++a) { mbar_init(bar_tfull + 8 * a, 2); mbar_init(bar_tempty + 8 * a, 8); }
     s_abort = 0;
     fence_mbar_init();
   }
@@ -98,7 +103,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
-  const int tiles = m_tiles * n_tiles;
+  const int tiles = m_tiles * n_tiles, sw_groups = (p.N + FP8_ROWS - 1) / FP8_ROWS;
   struct Tile { int e, row0, rows, nt; };
   auto tile = [&](int t) {
     Tile r;
@@ -154,48 +159,67 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
 #pragma unroll
           for (int kk = 0; kk < FP8_BLOCK / 32; ++kk) umma_e4m3(tmem + a * BN, dx + 2 * kk, dw + 2 * kk, idesc, kk != 0);
           umma_commit(bar_empty + 8 * s);
+          mbar_arrive(bar_tfull + 8 * a);                  // (what this thread has seen arrive, the scales among it, is seen by who waits here)
           umma_commit(bar_tfull + 8 * a);
           if (++s == NST) { s = 0; ph ^= 1; }
           if (++a == ACC) { a = 0; aph ^= 1; }
         }
+    } else if (warp >= 2) {
+      uint32_t s = 0, ph = 1, r = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        const Tile at = tile(t);
+        // warp 2: rows lane, lane + 32, ..; warp 3: runs of 16 weight rows.  What lies past the matrix has a neighbour's scale
+        const float* from[4];
+        if (warp == 2) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) from[i] = p.sx + min(max(at.row0, 0) + lane + 32 * i, p.x_rows - 1);
+        } else {
+          from[0] = p.sw + ((size_t)at.e * sw_groups + min(at.nt * (BN / FP8_ROWS) + lane, sw_groups - 1)) * p.kb;
+        }
+        for (int k = 0; k < p.kb; ++k) {
+          if (!(ok = mbar_wait(bar_empty + 8 * s, ph, p.status, ERR_MBAR_TIMEOUT_PRODUCER, abort_flag))) break;
+          const uint32_t to = smem_u32(small.scale[r]) + 4 * lane;
+          if (warp == 2) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) copy4(to + 128 * i, from[i] + (size_t)k * p.x_rows);
+          } else if (lane < BN / FP8_ROWS) {
+            copy4(to + 4 * FG_BM, from[0] + k);
+          }
+          arrive_copies(bar_full + 8 * s);
+          if (++s == NST) { s = 0; ph ^= 1; }
+          if (++r == S::RING) r = 0;
+        }
+      }
     }
     __syncwarp();
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     constexpr int HC = BN / 2, G = HC / FP8_ROWS;          // columns of a thread, and the scales that they have
-    const int q = warp & 3, half = (warp - 4) >> 2, sw_groups = (p.N + FP8_ROWS - 1) / FP8_ROWS;
-    uint8_t* const stage = smem_raw + NST * S::STAGE + (warp - 4) * 4096;
+    const int q = warp & 3, half = (warp - 4) >> 2;
+    uint8_t* const stage = smem_raw + NST * S::STAGE + (warp - 4) * 2048;
     const bool gated = act_gated(p.act);
     const int on = gated ? p.N >> 1 : p.N, esz = p.out_f32 ? 4 : 2;
     const bool wide = (((uintptr_t)p.C) & 15) == 0 && (p.ldc * esz) % 16 == 0;
-    uint32_t a = 0, aph = 0;
+    uint32_t a = 0, aph = 0, ring = 0;
     bool ok = true;
     for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
       const Tile at = tile(t);
       const int mine = q * 32 + lane, col0 = at.nt * BN + half * HC;
-      const float* sxp = p.sx + min(at.row0 + mine, p.x_rows - 1);
-      const float* swp[G];
-#pragma unroll
-      for (int g = 0; g < G; ++g) swp[g] = p.sw + ((size_t)at.e * sw_groups + min(col0 / FP8_ROWS + g, sw_groups - 1)) * p.kb;
-      auto fetch_x = [&](int k) { return __ldg(sxp + (size_t)min(k, p.kb - 1) * p.x_rows); };
-      float wv[G], x0 = fetch_x(0), x1 = fetch_x(1), x2 = fetch_x(2);
       float2 acc[HC / 2];
 #pragma unroll
       for (int j = 0; j < HC / 2; ++j) acc[j] = make_float2(0.f, 0.f);
       for (int k = 0; k < p.kb; ++k) {
-        if ((k & 31) == 0) {
-#pragma unroll
-          for (int g = 0; g < G; ++g) wv[g] = __ldg(swp[g] + min(k + lane, p.kb - 1));
-        }
-        const float sx = x0;
-        x0 = x1; x1 = x2; x2 = fetch_x(k + 3);
         if (!(ok = mbar_wait(bar_tfull + 8 * a, aph, p.status, ERR_MBAR_TIMEOUT_EPILOGUE, abort_flag))) break;
         tc_fence_after();
+        const float sx = small.scale[ring][mine];
+        const float2* swp = reinterpret_cast<const float2*>(&small.scale[ring][FG_BM + half * G]);
 #pragma unroll
         for (int c0 = 0; c0 < HC; c0 += 32) {
           uint32_t r[32];
           tmem_ld_32x32(tmem + ((uint32_t)(q * 32) << 16) + a * BN + half * HC + c0, r);
-          const float s0 = sx * __shfl_sync(0xffffffffu, wv[c0 / 16], k & 31), s1 = sx * __shfl_sync(0xffffffffu, wv[c0 / 16 + 1], k & 31);
+          const float2 sw = swp[c0 / 32];
+          const float s0 = sx * sw.x, s1 = sx * sw.y;
           tmem_ld_wait();
           if (c0 + 32 == HC) {
             tc_fence_before();
@@ -209,10 +233,11 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
           }
         }
         if (++a == ACC) { a = 0; aph ^= 1; }
+        if (++ring == S::RING) ring = 0;
       }
       if (!ok) break;
 
-      // ---- the tile: 32 sums at a time to 32 or 16 outputs, collected until a row has 128 bytes
+      // ---- the tile: 32 sums at a time to 32 or 16 outputs, collected until a row has 64 bytes
       const float rs = p.row_scale && mine < at.rows ? p.row_scale[at.row0 + mine] : 1.f;
       const float* bias = p.bias ? p.bias + (size_t)at.e * p.N : nullptr;
       int fill = 0, out0 = gated ? col0 >> 1 : col0;
@@ -232,39 +257,41 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
         } else if (p.act) {
           act_unary_run<false>(p.act, v, p.act_alpha, p.act_limit);
         }
-        const int n = gated ? 16 : 32;
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] *= rs;
-        uint8_t* row = stage + lane * 128;
-        if (p.out_f32) {
 #pragma unroll
-          for (int j = 0; j < 32; j += 4)
-            if (j < n) *reinterpret_cast<float4*>(row + (((fill / 16 + j / 4) ^ (lane & 7)) << 4)) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-        } else {
+        for (int h = 0; h < 32; h += 16) {                 // 16 outputs: 32 or 64 bytes
+          if (h && gated) break;
+          auto chunk = [&](int c) { return stage + lane * 64 + (((c + (lane >> 1)) & 3) << 4); };      // (eight rows' chunks lie in different banks)
+          if (p.out_f32) {
 #pragma unroll
-          for (int j = 0; j < 32; j += 8)
-            if (j < n)
-              *reinterpret_cast<uint4*>(row + (((fill / 16 + j / 8) ^ (lane & 7)) << 4)) =
-                  make_uint4(pack_bf16(v[j], v[j + 1]), pack_bf16(v[j + 2], v[j + 3]), pack_bf16(v[j + 4], v[j + 5]), pack_bf16(v[j + 6], v[j + 7]));
-        }
-        fill += n * esz;
-        if (fill == 128 || g + 1 == HC / 32) {
-          __syncwarp();
-          const int n_el = fill / esz;
-          uint8_t* const c = (uint8_t*)p.C + ((size_t)(at.row0 + q * 32) * p.ldc + out0) * esz;
-          const int live = at.rows - q * 32;
-          if (wide && out0 + n_el <= on) {
-            const int per_row = fill / 16, step = 32 / per_row;
-            const int ch = lane % per_row;
-            for (int r = lane / per_row; r < 32; r += step)
-              if (r < live) *reinterpret_cast<uint4*>(c + (size_t)r * p.ldc * esz + ch * 16) = *reinterpret_cast<const uint4*>(stage + r * 128 + ((ch ^ (r & 7)) << 4));
+            for (int j = 0; j < 16; j += 4) *reinterpret_cast<float4*>(chunk(j / 4)) = make_float4(v[h + j], v[h + j + 1], v[h + j + 2], v[h + j + 3]);
           } else {
-            for (int r = 0; r < min(32, live); ++r)
-              for (int j = lane; j < n_el && out0 + j < on; j += 32) {
-                const uint8_t* src = stage + r * 128 + (((j * esz / 16) ^ (r & 7)) << 4) + (j * esz) % 16;
-                if (p.out_f32) reinterpret_cast<float*>(c)[(size_t)r * p.ldc + j] = *reinterpret_cast<const float*>(src);
-                else reinterpret_cast<uint16_t*>(c)[(size_t)r * p.ldc + j] = *reinterpret_cast<const uint16_t*>(src);
+#pragma unroll
+            for (int j = 0; j < 16; j += 8)
+              *reinterpret_cast<uint4*>(chunk(fill / 16 + j / 8)) = make_uint4(pack_bf16(v[h + j], v[h + j + 1]), pack_bf16(v[h + j + 2], v[h + j + 3]),
+                                                                              pack_bf16(v[h + j + 4], v[h + j + 5]), pack_bf16(v[h + j + 6], v[h + j + 7]));
+          }
+          fill += 16 * esz;
+          if (fill < 64) continue;                         // (a thread's columns make whole runs)
+          __syncwarp();
+          const int n_el = 64 / esz, live = at.rows - q * 32;
+          uint8_t* const c = (uint8_t*)p.C + ((size_t)(at.row0 + q * 32) * p.ldc + out0) * esz;
+          if (wide && out0 + n_el <= on) {
+            const int ch = lane & 3;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int r = 8 * i + (lane >> 2);
+              if (r < live) *reinterpret_cast<uint4*>(c + (size_t)r * p.ldc * esz + ch * 16) = *reinterpret_cast<const uint4*>(stage + r * 64 + (((ch + (r >> 1)) & 3) << 4));
+            }
+          } else if (out0 < on) {
+            for (int r = 0; r < min(32, live); ++r) {
+              const uint8_t* src = stage + r * 64 + ((((lane * esz) >> 4) + (r >> 1) & 3) << 4) + (lane * esz & 15);
+              if (lane < n_el && out0 + lane < on) {
+                if (p.out_f32) reinterpret_cast<float*>(c)[(size_t)r * p.ldc + lane] = *reinterpret_cast<const float*>(src);
+                else reinterpret_cast<uint16_t*>(c)[(size_t)r * p.ldc + lane] = *reinterpret_cast<const uint16_t*>(src);
               }
+            }
           }
           __syncwarp();
           out0 += n_el;
@@ -310,21 +337,11 @@ MX_HOST_API int mx_fp8_gemm(const void* x, const float* sx, int x_rows, const vo
   const long long tiles = ((M + FG_BM - 1) / FG_BM + (counts ? (E < M ? E : M) : 0)) * (long long)((N + bn - 1) / bn);
   if (tiles >= 1ll << 31) return -106;
   Fp8Params p{};
-  p.sx = sx; p.x_rows = x_rows; p.sw = sw; p.C = c; p.ldc = ldc; p.out_f32 = out_f32; p.M = M; p.N = N; p.K = K; p.kb = kb; p.E = E; p.bias = bias; p.row_scale = row_scale;
+  p.sx = sx; p.x_rows = x_rows; p.sw = sw; p.C = c; p.ldc = ldc; p.out_f32 = out_f32; p.M = M; p.N = N; p.kb = kb; p.E = E; p.bias = bias; p.row_scale = row_scale;
   p.act = act; p.act_alpha = act_alpha; p.act_limit = act_limit; p.counts = counts; p.seg = seg; p.x_div = 1; p.status = status_word();
   CUtensorMap tx, tw;
-  const uint64_t row = (uint64_t)kb * FP8_BLOCK;               // codes travel as two-byte elements: the tile is bytes either way
-  {
-    uint64_t dims[2] = {row / 2, (uint64_t)x_rows}, strides[1] = {row};
-    uint32_t box[2] = {FP8_BLOCK / 2, FG_BM};
-    int r = make_tmap_bf16(&tx, x, 2, dims, strides, box, 1);
-    if (r) return r;
-  }
-  {
-    uint64_t dims[3] = {row / 2, (uint64_t)N, (uint64_t)E}, strides[2] = {row, row * (uint64_t)N};
-    uint32_t box[3] = {FP8_BLOCK / 2, (uint32_t)bn, 1};
-    int r = make_tmap_bf16(&tw, w, 3, dims, strides, box, 1);
-    if (r) return r;
-  }
+  int r = fp8_tmap(&tx, x, kb, x_rows, 0, FG_BM);
+  if (!r) r = fp8_tmap(&tw, w, kb, N, E, bn);
+  if (r) return r;
   return bn == 256 ? launch_gemm<256>(tx, tw, p, tiles, st) : launch_gemm<128>(tx, tw, p, tiles, st);
 }

@@ -4,11 +4,9 @@
 // The weights are the M side of tcgen05.mma (128 weight rows x 128 bytes: one block of K, one TMA box) and the rows its N side, padded to NT = 16 to 128
 // columns; the tensor cores need a small part of the time that the box takes to arrive, whatever NT.  Every block has scales of its own, so its sums go from
 // TMEM to registers, where a thread owns a weight row and adds s_x s_w times them to NT sums in fp32.
-//   warp 0      TMA: weight boxes (and boxes of codes, where the rows have been rounded before) into a ring of NST stages
+//   warp 0      TMA boxes of weights and of rows into a ring of NST stages, and asynchronous copies of their scales into a ring of their own
 //   warp 1      tcgen05.mma from one thread into a ring of ACC accumulators
 //   warps 2-5   32 weight rows each: scale and add, epilogue
-//   warps 6-    the rows' side of a stage: bf16 rows are read ahead into registers, rounded to e4m3 and put into the swizzled tile with their scales, so that a
-//               decode step needs no launch for it; rows that have been rounded: their scales
 // The work is the list of (group of rows, 128 weight rows, block of K) laid end to end, of which every CTA takes an equal run.  A tile that is cut leaves fp32
 // partials (at most two per CTA); the warp that arrives last adds them in the order of the CTAs, so results do not depend on timing.
 // Every mbarrier wait is bounded.
@@ -24,21 +22,19 @@ constexpr int FS_W = FS_TILE * FP8_BLOCK;
 constexpr int FS_MAX_E = 1024;
 constexpr int FS_MAX_GRID = CUT_TICKETS / 4;
 
-template <int NT, bool ROUND> struct Fp8StreamShape {
+template <int NT> struct Fp8StreamShape {
   static constexpr int X = NT * FP8_BLOCK;
   static constexpr int STAGE = FS_W + X;
-  // up to 64 columns the next launch's CTA fits beside this one's and fetches its first weights while this one drains
-  static constexpr int LIMIT = (NT <= 64 ? 108 : 200) * 1024;
-  static constexpr int NST = LIMIT / STAGE < 8 ? LIMIT / STAGE : 8;
+  static constexpr int CTAS = NT <= 64 ? 2 : 1;        // per SM; 128 sums a thread want all the registers
+  static constexpr int NST = (CTAS == 2 ? 104 : 200) * 1024 / STAGE;
   static constexpr int SMEM = NST * STAGE + 1024;
-  static constexpr int ACC = NT <= 32 ? 4 : NT == 64 ? 4 : 2;
-  static constexpr int TMEM = NT * ACC;  // 64, 128, 256, 256 columns
-  // warps of the rows' side.  Registers are shared out by the warps of a quarter of the SM, so eight warps leave an epilogue thread 255 of them (twice eight: 128),
-  // and ten only 168
-  static constexpr int RW = !ROUND ? 1 : NT <= 32 ? 2 : 4;
-  static constexpr int THREADS = 192 + 32 * RW;
-  static constexpr int AHEAD = NT <= 16 ? 4 : NT <= 32 ? 2 : 1;      // units whose bf16 rows are in registers ahead of their use
+  static constexpr int ACC = NT <= 64 ? 4 : 2;
+  static constexpr int TMEM = NT * ACC;                // 64, 128, 256, 256 columns: two CTAs have 512
+  // Scales of a unit: NT of the rows, 8 of the weights.  A slot is free again when the products of the unit NST before are done, since they waited for the sums
+  // of the unit ACC before them.
+  static constexpr int RING = NST + ACC, SC = NT + 8;
 };
+constexpr int FS_THREADS = 192;
 
 // A run of `per` units for every CTA; shorter runs would cost more in partial sums than they gain.
 __host__ __device__ inline int fp8_run(int total, int grid) {
@@ -46,38 +42,28 @@ __host__ __device__ inline int fp8_run(int total, int grid) {
   return per < 2 ? 2 : per;
 }
 
-template <int NT, bool ROUND>
-__global__ void __launch_bounds__(Fp8StreamShape<NT, ROUND>::THREADS, NT <= 32 ? 2 : 1)
+template <int NT>
+__global__ void __launch_bounds__(FS_THREADS, Fp8StreamShape<NT>::CTAS)
 fp8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const Fp8Params p) {
-  using S = Fp8StreamShape<NT, ROUND>;
-  constexpr int NST = S::NST, ACC = S::ACC, RW = S::RW, FS_THREADS = S::THREADS;
+  using S = Fp8StreamShape<NT>;
+  constexpr int NST = S::NST, ACC = S::ACC;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t s_bar[2 * NST + 2 * ACC];
-  __shared__ __align__(16) float s_sx[NST][NT];
+  __shared__ __align__(16) float s_scale[S::RING][S::SC];
   __shared__ uint16_t s_pre[FS_MAX_E + 1];
   __shared__ int s_sum[FS_THREADS / 32];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  uint8_t* const smem = smem_raw + (base - smem_u32(smem_raw));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t bar_full = smem_u32(s_bar), bar_empty = bar_full + 8 * NST, bar_tfull = bar_empty + 8 * NST, bar_tempty = bar_tfull + 8 * ACC;
   volatile int* abort_flag = &s_abort;
   if (tid == 0) {
-    for (int s = 0; s < NST; ++s) {
-      mbar_init(bar_full + 8 * s, 1 + RW);             // the TMA thread, the row warps
-      mbar_init(bar_empty + 8 * s, 1 + 4);             // the products, four epilogue warps (they read the scales)
-    }
-    for (int a = 0; a < ACC; ++a) { mbar_init(bar_tfull + 8 * a, 1); mbar_init(bar_tempty + 8 * a, 4); }
+    for (int s = 0; s < NST; ++s) { mbar_init(bar_full + 8 * s, 1 + 32); mbar_init(bar_empty + 8 * s, 1); }      // (the boxes, and every lane's copies)
+    for (int a = 0; a < ACC; ++a) { mbar_init(bar_tfull + 8 * a, 2); mbar_init(bar_tempty + 8 * a, 4); }
     s_abort = 0;
     fence_mbar_init();
   }
-  if (ROUND) {                                         // rows that no group fills stay zero
-    for (int i = tid; i < NST * S::X / 16; i += FS_THREADS)
-      *reinterpret_cast<uint4*>(smem + (i / (S::X / 16)) * S::STAGE + FS_W + (i % (S::X / 16)) * 16) = make_uint4(0, 0, 0, 0);
-    fence_proxy_async();
-  }
-  for (int i = tid; i < NST * NT; i += FS_THREADS) (&s_sx[0][0])[i] = 0.f;
 
   // ---- the list of work
   const bool banked = p.counts != nullptr;
@@ -151,34 +137,47 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
     }
   };
   const bool early = !banked && !p.slot;               // which weights are read does not depend on the launch before
+  const int sw_groups = (p.N + FP8_ROWS - 1) / FP8_ROWS;
 
   if (warp == 0) {
-    // ------------------------------------------------ TMA
-    if (lane == 0 && my0 < my1) {
-      prefetch_tmap(&tm_w);
-      if (!ROUND) prefetch_tmap(&tm_x);
+    // ------------------------------------------------ TMA, scales
+    if (my0 < my1) {
+      if (lane == 0) { prefetch_tmap(&tm_w); prefetch_tmap(&tm_x); }
       if (!early && !banked) pdl_wait();
       auto load_w = [&](int s, const Place& at) {
-        mbar_expect_tx(bar_full + 8 * s, ROUND ? FS_W : S::STAGE);
+        mbar_expect_tx(bar_full + 8 * s, S::STAGE);
         tma_load_3d(base + s * S::STAGE, &tm_w, bar_full + 8 * s, at.k * (FP8_BLOCK / 2), at.nt * FS_TILE, min(max(at.e, 0), p.E - 1));
       };
-      Place at = place(my0), w = at;
-      int ahead = 0, pos = my0;
       auto next = [&](Place& r, int i) {
         if (++r.k == p.kb) next_tile(r, i + 1 < my1);
       };
+      Place at = place(my0), w = at;
+      int ahead = 0;
       if (early) {
-        for (; ahead < NST && my0 + ahead < my1; ++ahead) { load_w(ahead, w); next(w, my0 + ahead); }
+        for (; ahead < NST && my0 + ahead < my1; ++ahead) {
+          if (lane == 0) load_w(ahead, w);
+          next(w, my0 + ahead);
+        }
         pdl_wait();
       }
-      uint32_t s = 0, ph = 1;
-      for (; pos < my1; ++pos) {
+      uint32_t s = 0, ph = 1, r = 0;
+      for (int pos = my0; pos < my1; ++pos) {
         if (pos - my0 >= ahead) {
           if (!mbar_wait(bar_empty + 8 * s, ph, p.status, ERR_MBAR_TIMEOUT_PRODUCER, abort_flag)) break;
-          load_w(s, at);
+          if (lane == 0) load_w(s, at);
         }
-        if (!ROUND) tma_load_2d(base + s * S::STAGE + FS_W, &tm_x, bar_full + 8 * s, at.k * (FP8_BLOCK / 2), p.slot ? at.row0 / p.x_div : at.row0);
+        const int row = p.slot ? at.row0 / p.x_div : at.row0;
+        if (lane == 0) tma_load_2d(base + s * S::STAGE + FS_W, &tm_x, bar_full + 8 * s, at.k * (FP8_BLOCK / 2), row);
+        const uint32_t to = smem_u32(s_scale[r]) + 4 * lane;
+        const float* from = p.sx + (size_t)at.k * p.x_rows + row + lane;
+#pragma unroll
+        for (int c = 0; c < NT; c += 32)
+          if (c + lane < at.rows) copy4(to + 4 * c, from + c);
+        if (lane < 8)
+          copy4(to + 4 * NT, p.sw + ((size_t)min(max(at.e, 0), p.E - 1) * sw_groups + min(at.nt * (FS_TILE / FP8_ROWS) + lane, sw_groups - 1)) * p.kb + at.k);
+        arrive_copies(bar_full + 8 * s);
         if (++s == NST) { s = 0; ph ^= 1; }
+        if (++r == S::RING) r = 0;
         next(at, pos);
       }
     }
@@ -205,19 +204,20 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
 #pragma unroll
         for (int kk = 0; kk < FP8_BLOCK / 32; ++kk) umma_e4m3(tmem + a * NT, dw + 2 * kk, dx + 2 * kk, idesc, kk != 0);
         umma_commit(bar_empty + 8 * s);
+        mbar_arrive(bar_tfull + 8 * a);                // (what this thread has seen arrive, the scales among it, is seen by who waits here)
         umma_commit(bar_tfull + 8 * a);
         if (++s == NST) { s = 0; ph ^= 1; }
         if (++a == ACC) { a = 0; aph ^= 1; }
       }
     }
-  } else if (warp < 6) {
+  } else {
     // ------------------------------------------------ scales, sums, epilogue: a thread owns weight row `n`
-    const int q = warp & 3, sw_groups = (p.N + FP8_ROWS - 1) / FP8_ROWS;
+    const int q = warp & 3;
     asm volatile("bar.sync 1, 160;" ::: "memory");
     tc_fence_after();
     const uint32_t tmem = s_tmem;
     if (!banked) pdl_wait();
-    uint32_t s = 0, ph = 0, a = 0, aph = 0;
+    uint32_t a = 0, aph = 0, ring = 0;
     bool ok = true;
     Place at;
     if (my0 < my1) at = place(my0);
@@ -225,24 +225,14 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
       const int first = at.k, n_units = min(my1 - pos, p.kb - at.k);
       const int n = at.nt * FS_TILE + q * 32 + lane;
       const int e = min(max(at.e, 0), p.E - 1);
-      // scales of 16 blocks at a time, one per lane of the half-warp that shares a group of rows
-      const float* swp = p.sw + ((size_t)e * sw_groups + min(n / FP8_ROWS, sw_groups - 1)) * p.kb;
-      auto fetch = [&](int k) { return __ldg(swp + min(k + (lane & 15), p.kb - 1)); };
-      float wv = fetch(first), wn = first + 16 < p.kb ? fetch(first + 16) : 0.f;
       float2 acc[NT / 2];
 #pragma unroll
       for (int j = 0; j < NT / 2; ++j) acc[j] = make_float2(0.f, 0.f);
       for (int i = 0; i < n_units; ++i) {
-        if (i && (i & 15) == 0) {
-          wv = wn;
-          if (i + 16 < n_units) wn = fetch(first + i + 16);
-        }
-        const float sw = __shfl_sync(0xffffffffu, wv, (lane & 16) | (i & 15));
-        // the scales of the rows: written by the row warps before they arrived at the stage's barrier
-        if (!(ok = mbar_wait(bar_full + 8 * s, ph, p.status, ERR_MBAR_TIMEOUT_EPILOGUE, abort_flag))) break;
         if (!(ok = mbar_wait(bar_tfull + 8 * a, aph, p.status, ERR_MBAR_TIMEOUT_EPILOGUE, abort_flag))) break;
         tc_fence_after();
-        const float4* sx = reinterpret_cast<const float4*>(s_sx[s]);
+        const float4* sx = reinterpret_cast<const float4*>(s_scale[ring]);
+        const float sw = s_scale[ring][NT + 2 * q + (lane >> 4)];
         constexpr int C = NT < 32 ? NT : 32;
 #pragma unroll
         for (int c0 = 0; c0 < NT; c0 += C) {
@@ -260,8 +250,8 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) { mbar_arrive(bar_tempty + 8 * a); mbar_arrive(bar_empty + 8 * s); }
-        if (++s == NST) { s = 0; ph ^= 1; }
+        if (lane == 0) mbar_arrive(bar_tempty + 8 * a);
+        if (++ring == S::RING) ring = 0;
         if (++a == ACC) { a = 0; aph ^= 1; }
       }
       if (!ok) break;
@@ -324,106 +314,6 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
       pos += n_units;
       next_tile(at, pos < my1);
     }
-  } else {
-    // ------------------------------------------------ the rows' side of the stages
-    const int rw = warp - 6;
-    if (!banked) pdl_wait();
-    if (my0 < my1) {
-      uint32_t s = 0, ph = 1;
-      if constexpr (ROUND) {
-        constexpr int R = NT / RW, D = S::AHEAD;         // rows of a warp: rw, rw + RW, ..
-        const bool vec = p.ldx % 4 == 0 && ((uintptr_t)p.xb & 7) == 0;
-        uint2 raw[D][R];
-        auto row_of = [&](const Place& r, int j) { return p.slot ? r.row0 / p.x_div : p.x_index ? p.x_index[r.row0 + j] : r.row0 + j; };
-        const int skip = 4 * lane;
-        auto load = [&](uint2 (&v)[R], const Place& r) {
-#pragma unroll
-          for (int j = 0; j < R; ++j) {
-            v[j] = make_uint2(0, 0);
-            if (rw + RW * j >= r.rows) continue;
-            const int src = row_of(r, rw + RW * j);
-            if (src < 0) continue;
-            if (src >= p.x_rows) { v[j] = make_uint2(0x7fc07fc0u, 0x7fc07fc0u); continue; }       // no such row: NaN
-            const __nv_bfloat16* at = p.xb + src * p.ldx + r.k * FP8_BLOCK + skip;
-            const int left = p.K - r.k * FP8_BLOCK - skip;
-            if (vec && left >= 4) {
-              v[j] = __ldg(reinterpret_cast<const uint2*>(at));
-            } else {
-              const uint16_t* h = reinterpret_cast<const uint16_t*>(at);
-              const uint32_t a = left > 0 ? h[0] : 0, b = left > 1 ? h[1] : 0, c = left > 2 ? h[2] : 0, d = left > 3 ? h[3] : 0;
-              v[j] = make_uint2(a | b << 16, c | d << 16);
-            }
-          }
-        };
-        Place at = place(my0), pf = at;
-        int pf_pos = my0;
-        auto advance = [&](Place& r, int pos) { if (++r.k == p.kb) next_tile(r, pos + 1 < my1); };
-#pragma unroll
-        for (int d = 0; d < D; ++d)
-          if (pf_pos < my1) { load(raw[d], pf); advance(pf, pf_pos); ++pf_pos; }
-        bool ok = true;
-        for (int pos = my0; ok && pos < my1;) {
-#pragma unroll
-          for (int d = 0; d < D; ++d) {
-            if (!ok || pos >= my1) continue;
-            if (!(ok = mbar_wait(bar_empty + 8 * s, ph, p.status, ERR_MBAR_TIMEOUT_DEQUANT, abort_flag))) continue;
-            uint8_t* tile = smem + s * S::STAGE + FS_W;
-#pragma unroll
-            for (int j = 0; j < R; ++j) {
-              const int r = rw + RW * j;
-              if (r >= at.rows) continue;
-              const float v0 = bf16_lo(raw[d][j].x), v1 = bf16_hi(raw[d][j].x), v2 = bf16_lo(raw[d][j].y), v3 = bf16_hi(raw[d][j].y);
-              const uint32_t m = __reduce_max_sync(0xffffffffu, max(max(fp8_mag(v0), fp8_mag(v1)), max(fp8_mag(v2), fp8_mag(v3))));
-              float inv;
-              const float sc = fp8_scale(__uint_as_float(m), &inv);
-              const uint32_t word = m >= 0x7f800000u ? 0u : fp8_pack4(v0 * inv, v1 * inv, v2 * inv, v3 * inv);
-              *reinterpret_cast<uint32_t*>(tile + sw128_offset(r, lane >> 2) + (lane & 3) * 4) = word;
-              if (lane == 0) s_sx[s][r] = sc;
-            }
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar_full + 8 * s);
-            if (++s == NST) { s = 0; ph ^= 1; }
-            advance(at, pos);
-            ++pos;
-            if (pf_pos < my1) { load(raw[d], pf); advance(pf, pf_pos); ++pf_pos; }
-          }
-        }
-      } else {
-        // scales of the rows: columns lane, lane + 32, .. of the stage
-        constexpr int D = 4, C = (NT + 31) / 32;
-        Place at = place(my0), pf = at;
-        int pf_pos = my0;
-        float v[D][C];
-        auto advance = [&](Place& r, int pos) { if (++r.k == p.kb) next_tile(r, pos + 1 < my1); };
-        auto load = [&](float (&t)[C], const Place& r) {
-#pragma unroll
-          for (int c = 0; c < C; ++c) {
-            const int j = c * 32 + lane;
-            t[c] = j < r.rows ? __ldg(p.sx + (size_t)r.k * p.x_rows + (p.slot ? r.row0 / p.x_div : r.row0 + j)) : 0.f;
-          }
-        };
-#pragma unroll
-        for (int d = 0; d < D; ++d)
-          if (pf_pos < my1) { load(v[d], pf); advance(pf, pf_pos); ++pf_pos; }
-        bool ok = true;
-        for (int pos = my0; ok && pos < my1;) {
-#pragma unroll
-          for (int d = 0; d < D; ++d) {
-            if (!ok || pos >= my1) continue;
-            if (!(ok = mbar_wait(bar_empty + 8 * s, ph, p.status, ERR_MBAR_TIMEOUT_DEQUANT, abort_flag))) continue;
-#pragma unroll
-            for (int c = 0; c < C; ++c)
-              if (c * 32 + lane < NT) s_sx[s][c * 32 + lane] = v[d][c];
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar_full + 8 * s);
-            if (++s == NST) { s = 0; ph ^= 1; }
-            ++pos;
-            if (pf_pos < my1) { load(v[d], pf); advance(pf, pf_pos); ++pf_pos; }
-          }
-        }
-      }
-    }
   }
   if (*abort_flag)                                         // a wait ran out: copies still in flight land before shared memory is released
     for (int i = 0; i < 200; ++i) __nanosleep(1000);
@@ -432,17 +322,17 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
   if (warp == 1) { tc_fence_after(); tmem_dealloc(s_tmem, S::TMEM); }
 }
 
-template <int NT, bool ROUND> static int launch_stream(const CUtensorMap& tw, const CUtensorMap& tx, const Fp8Params& p, cudaStream_t st) {
-  using S = Fp8StreamShape<NT, ROUND>;
-  auto kern = fp8_stream_kernel<NT, ROUND>;
+template <int NT> static int launch_stream(const CUtensorMap& tw, const CUtensorMap& tx, const Fp8Params& p, cudaStream_t st) {
+  using S = Fp8StreamShape<NT>;
+  auto kern = fp8_stream_kernel<NT>;
   static DeviceOnce configured;
   if (configured.pending()) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
     if (e != cudaSuccess) return (int)e;
     configured.mark();
   }
-  const int grid = sm_count() < FS_MAX_GRID ? sm_count() : FS_MAX_GRID;
-  launch_pdl(kern, dim3(grid), dim3(S::THREADS), S::SMEM, st, tw, tx, p);
+  const int grid = S::CTAS * sm_count() < FS_MAX_GRID ? S::CTAS * sm_count() : FS_MAX_GRID;
+  launch_pdl(kern, dim3(grid), dim3(FS_THREADS), S::SMEM, st, tw, tx, p);
   return (int)cudaGetLastError();
 }
 
@@ -458,37 +348,28 @@ MX_HOST_API int mx_fp8_stream_takes(long long groups, int N, int kb, int E) {
   return E <= FS_MAX_E && groups < 65536 && groups * ((N + FS_TILE - 1) / FS_TILE) * kb < (1ll << 30);
 }
 
-// Dense (M <= nt), experts (counts / seg: from the bank's first expert on) or slots (slot).  nt 16, 32, 64 or 128: rows of a group, padded.  xb: bf16 rows, rounded on the
-// way (nt <= 64); null: codes x and scales sx of x_rows rows.  tickets: see host_util.h.
-MX_HOST_API int mx_fp8_stream(const void* x, const float* sx, const void* xb, long long ldx, const int* x_index, int x_rows, const void* w, const float* sw, int E, void* c,
-                              long long ldc, int out_f32, const float* bias, const float* row_scale, int act, float act_alpha, float act_limit, int M, int N, int K,
-                              const int* counts, const int* seg, const int* slot, int x_div, int e_lo, int nt, float* scratch, int* tickets, cudaStream_t st) {
+// Codes x and scales sx of x_rows rows against w.  Dense (M <= nt), experts (counts / seg: from the bank's first expert on) or slots (slot).  nt 16, 32, 64 or 128: rows of a
+// group, padded.  tickets: see host_util.h.
+MX_HOST_API int mx_fp8_stream(const void* x, const float* sx, int x_rows, const void* w, const float* sw, int E, void* c, long long ldc, int out_f32, const float* bias,
+                              const float* row_scale, int act, float act_alpha, float act_limit, int M, int N, int K, const int* counts, const int* seg, const int* slot,
+                              int x_div, int e_lo, int nt, float* scratch, int* tickets, cudaStream_t st) {
   if (M <= 0 || N <= 0) return 0;
   const int kb = (K + FP8_BLOCK - 1) / FP8_BLOCK;
   if (K < 1 || x_div < 1 || E < 1 || x_rows < 1) return -101;
   if (act_gated(act) && N % 32) return -104;
   const long long groups = slot ? M : counts ? (long long)M / nt + (E < M ? E : M) + 1 : 1;
-  if (!mx_fp8_stream_takes(groups, N, kb, E) || (!slot && !counts && M > nt) || (xb && nt > 64)) return -106;
+  if (!mx_fp8_stream_takes(groups, N, kb, E) || (!slot && !counts && M > nt)) return -106;
   if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)scratch) & 15) return -114;
-  Fp8Params p{(const __nv_bfloat16*)xb, ldx, x_index, sx, x_rows, sw, c, ldc, out_f32, M, N, K, kb, E, bias, row_scale, act, act_alpha, act_limit, counts, seg, slot, x_div,
-              e_lo, scratch, tickets, status_word()};
+  Fp8Params p{sx, x_rows, sw, c, ldc, out_f32, M, N, kb, E, bias, row_scale, act, act_alpha, act_limit, counts, seg, slot, x_div, e_lo, scratch, tickets, status_word()};
   CUtensorMap tw, tx;
-  const uint64_t row = (uint64_t)kb * FP8_BLOCK;               // codes travel as two-byte elements: the tile is bytes either way
-  {
-    uint64_t dims[3] = {row / 2, (uint64_t)N, (uint64_t)E}, strides[2] = {row, row * (uint64_t)N};
-    uint32_t box[3] = {FP8_BLOCK / 2, FS_TILE, 1};
-    int r = make_tmap_bf16(&tw, w, 3, dims, strides, box, 1);
-    if (r) return r;
+  int r = fp8_tmap(&tw, w, kb, N, E, FS_TILE);
+  if (!r) r = fp8_tmap(&tx, x, kb, x_rows, 0, nt);
+  if (r) return r;
+  switch (nt) {
+    case 16: return launch_stream<16>(tw, tx, p, st);
+    case 32: return launch_stream<32>(tw, tx, p, st);
+    case 64: return launch_stream<64>(tw, tx, p, st);
+    case 128: return launch_stream<128>(tw, tx, p, st);
+    default: return -106;
   }
-  tx = tw;
-  if (!xb) {
-    uint64_t dims[2] = {row / 2, (uint64_t)x_rows}, strides[1] = {row};
-    uint32_t box[2] = {FP8_BLOCK / 2, (uint32_t)nt};
-    int r = make_tmap_bf16(&tx, x, 2, dims, strides, box, 1);
-    if (r) return r;
-  }
-#define MX_FS(NT_) if (nt == NT_) return xb ? launch_stream<NT_, NT_ <= 64>(tw, tx, p, st) : launch_stream<NT_, false>(tw, tx, p, st)
-  MX_FS(16); MX_FS(32); MX_FS(64); MX_FS(128);
-#undef MX_FS
-  return -106;
 }

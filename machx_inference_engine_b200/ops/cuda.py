@@ -909,22 +909,17 @@ def fp8_rows(x, index=None) -> FP8Rows:
 
 
 FP8_STREAM_ROWS = (16, 32, 64, 128)      # rows of a group in the weight-streaming kernel
-FP8_ROUND_ROWS = 64                      # bf16 rows are rounded inside it up to groups of this many
 
 
 def _fp8_stream(x, w: QuantWeight, out, bias, row_scale, act, act_alpha, act_limit, nt, counts=None, seg=None, slot=None, x_div=1, e_lo=0, index=None):
     """The weight-streaming kernel (csrc/cuda/fp8_stream.cu) with groups of up to ``nt`` rows."""
     lib = _lib.cuda()
-    if not isinstance(x, FP8Rows) and nt > FP8_ROUND_ROWS:
-        x, index = fp8_rows(x, index), None
-    rounded = isinstance(x, FP8Rows)
+    q = x if isinstance(x, FP8Rows) else fp8_rows(x, index)
     scratch = torch.empty(lib.mx_fp8_stream_scratch(nt), dtype=torch.float32, device=out.device)
     tickets = _tickets(out.device)
-    null = _vp(0)
-    _check(lib.mx_fp8_stream(_p(x.codes) if rounded else null, _p(x.scale) if rounded else null, null if rounded else _p(x), C.c_longlong(0 if rounded else x.stride(0)),
-                             _p(index), x.shape[0], _p(w.p0), _p(w.p1), w.E, _p(out), C.c_longlong(out.stride(0)), int(out.dtype == torch.float32), _p(bias), _p(row_scale),
-                             act, C.c_float(act_alpha), C.c_float(act_limit), out.shape[0], w.N, w.K, _p(counts), _p(seg), _p(slot), int(x_div), int(e_lo), nt, _p(scratch),
-                             tickets[1], tickets[2]), "fp8_stream")
+    _check(lib.mx_fp8_stream(_p(q.codes), _p(q.scale), q.codes.shape[0], _p(w.p0), _p(w.p1), w.E, _p(out), C.c_longlong(out.stride(0)), int(out.dtype == torch.float32),
+                             _p(bias), _p(row_scale), act, C.c_float(act_alpha), C.c_float(act_limit), out.shape[0], w.N, w.K, _p(counts), _p(seg), _p(slot), int(x_div),
+                             int(e_lo), nt, _p(scratch), tickets[1], tickets[2]), "fp8_stream")
     _count()
     return out
 
