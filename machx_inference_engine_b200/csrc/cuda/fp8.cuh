@@ -30,14 +30,22 @@ __device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d
   return (uint32_t)lo | ((uint32_t)hi << 16);
 }
 
-// D[tmem] (+)= A[smem] * B[smem], e4m3 inputs (K = 32 a step), fp32 accumulate; issued by one thread.
-__device__ __forceinline__ void umma_e4m3(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+// D[tmem] (+)= A[smem] * B[smem], e4m3 inputs (K = 32 a step), fp32 accumulate.  A whole warp comes here and `leader` (elect_one) issues: in a branch of one
+// thread the descriptors would have to be moved to uniform registers before every instruction (four products and two commits 470 -> see the kernels).
+__device__ __forceinline__ void umma_e4m3(uint32_t leader, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n"
-      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(leader)
       : "memory");
+}
+__device__ __forceinline__ void umma_commit_if(uint32_t leader, uint32_t bar) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n"
+               ::"r"(bar), "r"(leader) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_if(uint32_t leader, uint32_t bar) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t@q mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}\n" ::"r"(bar), "r"(leader) : "memory");
 }
 // kind::f8f6f4 instruction descriptor: e4m3 x e4m3 -> fp32, M x N tile, both operands K-major.
 __host__ __device__ constexpr uint32_t umma_idesc_e4m3(int M, int N) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }

@@ -146,7 +146,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
           if (++s == NST) { s = 0; ph ^= 1; }
         }
       }
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1) {
+      const uint32_t leader = elect_one();
       constexpr uint32_t idesc = umma_idesc_e4m3(FG_BM, BN);
       uint32_t s = 0, ph = 0, a = 0, aph = 1;
       bool ok = true;
@@ -154,13 +155,14 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
         for (int k = 0; k < p.kb; ++k) {
           if (!(ok = mbar_wait(bar_tempty + 8 * a, aph, p.status, ERR_MBAR_TIMEOUT_MMA, abort_flag))) break;
           if (!(ok = mbar_wait(bar_full + 8 * s, ph, p.status, ERR_MBAR_TIMEOUT_MMA, abort_flag))) break;
+          __syncwarp();                                    // (no lane may miss a phase)
           tc_fence_after();
           const uint64_t dx = umma_desc_k_sw128(base + s * S::STAGE), dw = umma_desc_k_sw128(base + s * S::STAGE + S::A);
 #pragma unroll
-          for (int kk = 0; kk < FP8_BLOCK / 32; ++kk) umma_e4m3(tmem + a * BN, dx + 2 * kk, dw + 2 * kk, idesc, kk != 0);
-          umma_commit(bar_empty + 8 * s);
-          mbar_arrive(bar_tfull + 8 * a);                  // (what this thread has seen arrive, the scales among it, is seen by who waits here)
-          umma_commit(bar_tfull + 8 * a);
+          for (int kk = 0; kk < FP8_BLOCK / 32; ++kk) umma_e4m3(leader, tmem + a * BN, dx + 2 * kk, dw + 2 * kk, idesc, kk != 0);
+          umma_commit_if(leader, bar_empty + 8 * s);
+          mbar_arrive_if(leader, bar_tfull + 8 * a);                  // (what this thread has seen arrive, the scales among it, is seen by who waits here)
+          umma_commit_if(leader, bar_tfull + 8 * a);
           if (++s == NST) { s = 0; ph ^= 1; }
           if (++a == ACC) { a = 0; aph ^= 1; }
         }
@@ -252,8 +254,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
           for (int j = 0; j < 32; ++j) v[j] += __ldg(bias + min(c + j, p.N - 1));
         }
         if (gated) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] = glu_apply(p.act, v[j], v[16 + j], p.act_alpha, p.act_limit);
+          glu_run<16>(p.act, v, p.act_alpha, p.act_limit);
         } else if (p.act) {
           act_unary_run<false>(p.act, v, p.act_alpha, p.act_limit);
         }

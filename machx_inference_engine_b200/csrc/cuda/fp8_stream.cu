@@ -193,19 +193,21 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
     asm volatile("bar.sync 1, 160;" ::: "memory");
     tc_fence_after();
     const uint32_t tmem = s_tmem;
-    if (lane == 0) {
+    {
+      const uint32_t leader = elect_one();
       constexpr uint32_t idesc = umma_idesc_e4m3(FS_TILE, NT);
       uint32_t s = 0, ph = 0, a = 0, aph = 1;
       for (int pos = my0; pos < my1; ++pos) {
         if (!mbar_wait(bar_tempty + 8 * a, aph, p.status, ERR_MBAR_TIMEOUT_MMA, abort_flag)) break;
         if (!mbar_wait(bar_full + 8 * s, ph, p.status, ERR_MBAR_TIMEOUT_MMA, abort_flag)) break;
+        __syncwarp();                                  // (no lane may miss a phase)
         tc_fence_after();
         const uint64_t dw = umma_desc_k_sw128(base + s * S::STAGE), dx = umma_desc_k_sw128(base + s * S::STAGE + FS_W);
 #pragma unroll
-        for (int kk = 0; kk < FP8_BLOCK / 32; ++kk) umma_e4m3(tmem + a * NT, dw + 2 * kk, dx + 2 * kk, idesc, kk != 0);
-        umma_commit(bar_empty + 8 * s);
-        mbar_arrive(bar_tfull + 8 * a);                // (what this thread has seen arrive, the scales among it, is seen by who waits here)
-        umma_commit(bar_tfull + 8 * a);
+        for (int kk = 0; kk < FP8_BLOCK / 32; ++kk) umma_e4m3(leader, tmem + a * NT, dw + 2 * kk, dx + 2 * kk, idesc, kk != 0);
+        umma_commit_if(leader, bar_empty + 8 * s);
+        mbar_arrive_if(leader, bar_tfull + 8 * a);                // (what this thread has seen arrive, the scales among it, is seen by who waits here)
+        umma_commit_if(leader, bar_tfull + 8 * a);
         if (++s == NST) { s = 0; ph ^= 1; }
         if (++a == ACC) { a = 0; aph ^= 1; }
       }
