@@ -23,8 +23,9 @@ constexpr int FG_GROUP = 8;                                // m-tiles that are w
 
 template <int BN> struct Fp8GemmShape {
   static constexpr int A = FG_BM * FP8_BLOCK, B = BN * FP8_BLOCK, STAGE = A + B;
-  static constexpr int OUT = 8 * 2048;                     // 32 rows x 64 bytes for each warp
-  static constexpr int NST = 192 * 1024 / STAGE;
+  static constexpr int ROW = BN;                           // bytes of a staged row of a warp's outputs
+  static constexpr int OUT = 8 * 32 * ROW;
+  static constexpr int NST = BN == 256 ? 3 : 5;
   static constexpr int ACC = 512 / BN;
   // A slot of scales is free again when the products of the block NST before are done, since they waited for the sums of the block ACC before them.
   static constexpr int RING = NST + ACC, SC = FG_BM + BN / FP8_ROWS;
@@ -40,7 +41,8 @@ template <int BN> struct Fp8GemmShape {
   static_assert(SMEM <= 227 * 1024, "shared memory of a block");
 };
 
-template <int BN>
+// KIND: 0 no activation, 1 gated, 2 element-wise.  The tile's end runs once per tile and is bound by fetching its instructions, so each instance has what it needs only.
+template <int BN, int KIND, bool F32>
 __global__ void __launch_bounds__(FG_THREADS, 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, const Fp8Params p) {
   using S = Fp8GemmShape<BN>;
@@ -199,10 +201,12 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     constexpr int HC = BN / 2, G = HC / FP8_ROWS;          // columns of a thread, and the scales that they have
     const int q = warp & 3, half = (warp - 4) >> 2;
-    uint8_t* const stage = smem_raw + NST * S::STAGE + (warp - 4) * 2048;
-    const bool gated = act_gated(p.act);
-    const int on = gated ? p.N >> 1 : p.N, esz = p.out_f32 ? 4 : 2;
-    const bool wide = (((uintptr_t)p.C) & 15) == 0 && (p.ldc * esz) % 16 == 0;
+    constexpr int ESZ = F32 ? 4 : 2, PIECE = KIND == 1 ? 8 : 16;        // outputs of 16 sums
+    constexpr int ROW_BYTES = HC * PIECE / 16 * ESZ;       // of a thread's outputs
+    constexpr int PASSES = ROW_BYTES > S::ROW ? ROW_BYTES / S::ROW : 1, RB = ROW_BYTES / PASSES, CPR = RB / 16;
+    uint8_t* const stage = smem_raw + NST * S::STAGE + (warp - 4) * (32 * S::ROW);
+    const int on = KIND == 1 ? p.N >> 1 : p.N;
+    const bool wide = (((uintptr_t)p.C) & 15) == 0 && (p.ldc * ESZ) % 16 == 0;
     uint32_t a = 0, aph = 0, ring = 0;
     bool ok = true;
     for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
@@ -215,89 +219,77 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
         if (!(ok = mbar_wait(bar_tfull + 8 * a, aph, p.status, ERR_MBAR_TIMEOUT_EPILOGUE, abort_flag))) break;
         tc_fence_after();
         const float sx = small.scale[ring][mine];
-        const float2* swp = reinterpret_cast<const float2*>(&small.scale[ring][FG_BM + half * G]);
+        const float* swp = &small.scale[ring][FG_BM + half * G];
+        const uint32_t from = tmem + ((uint32_t)(q * 32) << 16) + a * BN + half * HC;
+        uint32_t r[2][16];                                 // a load is under way while the one before is added
+        tmem_ld_cols<16>(from, r[0]);
 #pragma unroll
-        for (int c0 = 0; c0 < HC; c0 += 32) {
-          uint32_t r[32];
-          tmem_ld_32x32(tmem + ((uint32_t)(q * 32) << 16) + a * BN + half * HC + c0, r);
-          const float2 sw = swp[c0 / 32];
-          const float s0 = sx * sw.x, s1 = sx * sw.y;
-          tmem_ld_wait();
-          if (c0 + 32 == HC) {
+        for (int g = 0; g < G; ++g) {
+          tmem_wait_for(r[g & 1]);
+          if (g + 1 < G) {
+            tmem_ld_cols<16>(from + 16 * (g + 1), r[(g + 1) & 1]);
+          } else {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar_tempty + 8 * a);
           }
+          const float sc = sx * swp[g];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float sc = j < 8 ? s0 : s1;
-            acc[c0 / 2 + j] = fma2(make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), make_float2(sc, sc), acc[c0 / 2 + j]);
-          }
+          for (int j = 0; j < 8; ++j)
+            acc[8 * g + j] = fma2(make_float2(__uint_as_float(r[g & 1][2 * j]), __uint_as_float(r[g & 1][2 * j + 1])), make_float2(sc, sc), acc[8 * g + j]);
         }
         if (++a == ACC) { a = 0; aph ^= 1; }
         if (++ring == S::RING) ring = 0;
       }
       if (!ok) break;
 
-      // ---- the tile: 32 sums at a time to 32 or 16 outputs, collected until a row has 64 bytes
+      // ---- the tile: bias, activation, scale; a row's outputs meet in shared memory and are written as lines
       const float rs = p.row_scale && mine < at.rows ? p.row_scale[at.row0 + mine] : 1.f;
       const float* bias = p.bias ? p.bias + (size_t)at.e * p.N : nullptr;
-      int fill = 0, out0 = gated ? col0 >> 1 : col0;
+      const int live = min(32, at.rows - q * 32);
 #pragma unroll
-      for (int g = 0; g < HC / 32; ++g) {
-        float v[32];
+      for (int pass = 0; pass < PASSES; ++pass) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) { v[2 * j] = acc[16 * g + j].x; v[2 * j + 1] = acc[16 * g + j].y; }
-        if (bias) {
-          const int c = col0 + 32 * g;
+        for (int g = 0; g < HC / 32 / PASSES; ++g) {
+          const int c0 = (pass * (HC / 32 / PASSES) + g) * 32;
+          float v[32];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] += __ldg(bias + min(c + j, p.N - 1));
+          for (int j = 0; j < 16; ++j) { v[2 * j] = acc[c0 / 2 + j].x; v[2 * j + 1] = acc[c0 / 2 + j].y; }
+          if (bias) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] += __ldg(bias + min(col0 + c0 + j, p.N - 1));
+          }
+          if constexpr (KIND == 1) glu_run<16>(p.act, v, p.act_alpha, p.act_limit);
+          if constexpr (KIND == 2) act_unary_run<false>(p.act, v, p.act_alpha, p.act_limit);
+          constexpr int n = 2 * PIECE;
+#pragma unroll
+          for (int j = 0; j < n; j += 16 / ESZ) {
+            uint8_t* to = stage + lane * S::ROW + ((((g * n + j) * ESZ / 16) ^ (lane & 7)) << 4);
+            if constexpr (F32) *reinterpret_cast<float4*>(to) = make_float4(v[j] * rs, v[j + 1] * rs, v[j + 2] * rs, v[j + 3] * rs);
+            else *reinterpret_cast<uint4*>(to) = make_uint4(pack_bf16(v[j] * rs, v[j + 1] * rs), pack_bf16(v[j + 2] * rs, v[j + 3] * rs),
+                                                            pack_bf16(v[j + 4] * rs, v[j + 5] * rs), pack_bf16(v[j + 6] * rs, v[j + 7] * rs));
+          }
         }
-        if (gated) {
-          glu_run<16>(p.act, v, p.act_alpha, p.act_limit);
-        } else if (p.act) {
-          act_unary_run<false>(p.act, v, p.act_alpha, p.act_limit);
-        }
-#pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] *= rs;
-#pragma unroll
-        for (int h = 0; h < 32; h += 16) {                 // 16 outputs: 32 or 64 bytes
-          if (h && gated) break;
-          auto chunk = [&](int c) { return stage + lane * 64 + (((c + (lane >> 1)) & 3) << 4); };      // (eight rows' chunks lie in different banks)
-          if (p.out_f32) {
-#pragma unroll
-            for (int j = 0; j < 16; j += 4) *reinterpret_cast<float4*>(chunk(j / 4)) = make_float4(v[h + j], v[h + j + 1], v[h + j + 2], v[h + j + 3]);
+        __syncwarp();
+        const int ch = lane % CPR, out0 = (KIND == 1 ? col0 >> 1 : col0) + pass * (RB / ESZ) + ch * (16 / ESZ), inside = min(16 / ESZ, on - out0);
+        uint8_t* to = (uint8_t*)p.C + ((size_t)(at.row0 + q * 32 + lane / CPR) * p.ldc + out0) * ESZ;
+        const size_t step = (size_t)(32 / CPR) * p.ldc * ESZ;
+#pragma unroll 4
+        for (int r = lane / CPR; r < live; r += 32 / CPR, to += step) {
+          const uint4 x = *reinterpret_cast<const uint4*>(stage + r * S::ROW + ((ch ^ (r & 7)) << 4));
+          if (wide && inside == 16 / ESZ) {
+            *reinterpret_cast<uint4*>(to) = x;
           } else {
+            const uint32_t word[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-            for (int j = 0; j < 16; j += 8)
-              *reinterpret_cast<uint4*>(chunk(fill / 16 + j / 8)) = make_uint4(pack_bf16(v[h + j], v[h + j + 1]), pack_bf16(v[h + j + 2], v[h + j + 3]),
-                                                                              pack_bf16(v[h + j + 4], v[h + j + 5]), pack_bf16(v[h + j + 6], v[h + j + 7]));
-          }
-          fill += 16 * esz;
-          if (fill < 64) continue;                         // (a thread's columns make whole runs)
-          __syncwarp();
-          const int n_el = 64 / esz, live = at.rows - q * 32;
-          uint8_t* const c = (uint8_t*)p.C + ((size_t)(at.row0 + q * 32) * p.ldc + out0) * esz;
-          if (wide && out0 + n_el <= on) {
-            const int ch = lane & 3;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int r = 8 * i + (lane >> 2);
-              if (r < live) *reinterpret_cast<uint4*>(c + (size_t)r * p.ldc * esz + ch * 16) = *reinterpret_cast<const uint4*>(stage + r * 64 + (((ch + (r >> 1)) & 3) << 4));
-            }
-          } else if (out0 < on) {
-            for (int r = 0; r < min(32, live); ++r) {
-              const uint8_t* src = stage + r * 64 + ((((lane * esz) >> 4) + (r >> 1) & 3) << 4) + (lane * esz & 15);
-              if (lane < n_el && out0 + lane < on) {
-                if (p.out_f32) reinterpret_cast<float*>(c)[(size_t)r * p.ldc + lane] = *reinterpret_cast<const float*>(src);
-                else reinterpret_cast<uint16_t*>(c)[(size_t)r * p.ldc + lane] = *reinterpret_cast<const uint16_t*>(src);
+            for (int j = 0; j < 16 / ESZ; ++j)
+              if (j < inside) {
+                if constexpr (F32) reinterpret_cast<uint32_t*>(to)[j] = word[j];
+                else reinterpret_cast<uint16_t*>(to)[j] = (uint16_t)(word[j / 2] >> (16 * (j & 1)));
               }
-            }
           }
-          __syncwarp();
-          out0 += n_el;
-          fill = 0;
         }
+        __syncwarp();
       }
     }
   }
@@ -308,9 +300,9 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
   if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem, 512); }
 }
 
-template <int BN> static int launch_gemm(const CUtensorMap& tx, const CUtensorMap& tw, const Fp8Params& p, long long tiles, cudaStream_t st) {
+template <int BN, int KIND, bool F32> static int launch_gemm(const CUtensorMap& tx, const CUtensorMap& tw, const Fp8Params& p, long long tiles, cudaStream_t st) {
   using S = Fp8GemmShape<BN>;
-  auto kern = fp8_gemm_kernel<BN>;
+  auto kern = fp8_gemm_kernel<BN, KIND, F32>;
   static DeviceOnce configured;
   if (configured.pending()) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
@@ -344,5 +336,10 @@ MX_HOST_API int mx_fp8_gemm(const void* x, const float* sx, int x_rows, const vo
   int r = fp8_tmap(&tx, x, kb, x_rows, 0, FG_BM);
   if (!r) r = fp8_tmap(&tw, w, kb, N, E, bn);
   if (r) return r;
-  return bn == 256 ? launch_gemm<256>(tx, tw, p, tiles, st) : launch_gemm<128>(tx, tw, p, tiles, st);
+  const int kind = act == 0 ? 0 : act_gated(act) ? 1 : 2;
+#define MX_FG(BN_, KIND_) if (bn == BN_ && kind == KIND_) return out_f32 ? launch_gemm<BN_, KIND_, true>(tx, tw, p, tiles, st) : launch_gemm<BN_, KIND_, false>(tx, tw, p, tiles, st)
+  MX_FG(256, 0); MX_FG(256, 1); MX_FG(256, 2);
+  MX_FG(128, 0); MX_FG(128, 1); MX_FG(128, 2);
+#undef MX_FG
+  return -106;
 }
