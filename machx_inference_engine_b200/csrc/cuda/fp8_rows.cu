@@ -1,6 +1,7 @@
 // Rows of activations as e4m3 codes with a power-of-two scale per 128 elements: codes [rows][KB * 128] (zeros past K), scales [KB][rows].
 //
-// Bound: memory.  A warp takes a block of a row, a lane four elements of it; the largest magnitude is a maximum of bit patterns over the warp.
+// Bound: memory.  Sixteen lanes take a block, eight elements each: 16-byte loads, a maximum of bit patterns over the half-warp, 8-byte stores.  A warp has IT
+// such pairs of blocks of a row under way.  The warps of eight neighbouring rows lie side by side, so that their scales, four bytes each, share a sector.
 #include "act.cuh"
 #include "common.cuh"
 #include "fp8.cuh"
@@ -8,30 +9,106 @@
 
 namespace mx {
 
-template <typename T>
-__global__ void __launch_bounds__(256) fp8_rows_kernel(const T* __restrict__ x, long long ldx, const int* __restrict__ index, int x_rows, int rows, int K, int kb,
-                                                       uint8_t* __restrict__ codes, float* __restrict__ scale) {
-  pdl_prologue();
-  const int lane = threadIdx.x & 31;
-  const long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (unit >= (long long)rows * kb) return;
-  const int r = (int)(unit / kb), b = (int)(unit - (long long)r * kb);
-  const int src = index ? index[r] : r;
-  float v[4] = {0.f, 0.f, 0.f, 0.f};
-  if (src >= 0 && src < x_rows) {
-    const T* p = x + src * ldx + b * FP8_BLOCK;
+struct Fp8RowsParams {
+  const void* x;
+  long long ldx;
+  const int* index;
+  int x_rows, rows, K, kb, chunks;       // chunks: runs of 2 IT blocks in a row
+  uint8_t* codes;
+  float* scale;
+};
+
+template <typename T> struct Row8;       // eight elements as they were loaded
+template <> struct Row8<__nv_bfloat16> {
+  uint4 v;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = __ldg(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (b * FP8_BLOCK + 4 * lane + i < K) v[i] = to_f32<T>(p[4 * lane + i]);
+    for (int i = 0; i < 4; ++i) { f[2 * i] = bf16_lo(w[i]); f[2 * i + 1] = bf16_hi(w[i]); }
   }
-  uint32_t m = max(max(fp8_mag(v[0]), fp8_mag(v[1])), max(fp8_mag(v[2]), fp8_mag(v[3])));
-  m = __reduce_max_sync(0xffffffffu, m);
-  if (src >= x_rows) m = 0x7fc00000u;
-  float inv;
-  const float s = fp8_scale(__uint_as_float(m), &inv);
-  const uint32_t word = m >= 0x7f800000u ? 0u : fp8_pack4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
-  *reinterpret_cast<uint32_t*>(codes + ((size_t)r * kb + b) * FP8_BLOCK + 4 * lane) = word;
-  if (lane == 0) scale[(size_t)b * rows + r] = s;
+};
+template <> struct Row8<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p) { a = __ldg(reinterpret_cast<const float4*>(p)); b = __ldg(reinterpret_cast<const float4*>(p) + 1); }
+  __device__ __forceinline__ void get(float (&f)[8]) const { f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w; }
+};
+
+// VEC: rows start on 16 bytes
+template <typename T, int IT, bool VEC>
+__global__ void __launch_bounds__(256) fp8_rows_kernel(const Fp8RowsParams p) {
+  pdl_prologue();
+  const int lane = threadIdx.x & 31, half = lane >> 4, sub = lane & 15;
+  const int unit = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int g = unit / (8 * p.chunks), i = unit - g * 8 * p.chunks, n = min(8, p.rows - g * 8);
+  if (n <= 0) return;
+  const int chunk = i / n, r = g * 8 + i - chunk * n;
+  if (chunk >= p.chunks) return;
+  const int src = p.index ? p.index[r] : r;
+  const bool some = src >= 0 && src < p.x_rows;
+  const T* row = (const T*)p.x + (some ? src : 0) * p.ldx;
+  const int b0 = chunk * 2 * IT + half;
+  float v[IT][8];
+  if constexpr (VEC) {
+    Row8<T> raw[IT];
+#pragma unroll
+    for (int t = 0; t < IT; ++t) {
+      const int at = (b0 + 2 * t) * FP8_BLOCK + 8 * sub;
+      raw[t].load(row + (at + 8 <= p.K ? at : 0));         // (the row's first elements where the lane's are not whole; K is 8 at least)
+    }
+#pragma unroll
+    for (int t = 0; t < IT; ++t) {
+      const int at = (b0 + 2 * t) * FP8_BLOCK + 8 * sub;
+      raw[t].get(v[t]);
+      if (!some || at + 8 > p.K) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[t][j] = some && at + j < p.K ? to_f32<T>(row[at + j]) : 0.f;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int t = 0; t < IT; ++t)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int at = (b0 + 2 * t) * FP8_BLOCK + 8 * sub + j;
+        v[t][j] = some && at < p.K ? to_f32<T>(row[at]) : 0.f;
+      }
+  }
+#pragma unroll
+  for (int t = 0; t < IT; ++t) {
+    const int b = b0 + 2 * t;
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, fp8_mag(v[t][j]));
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (src >= p.x_rows) m = 0x7fc00000u;                  // no such row: NaN
+    float inv;
+    const float s = fp8_scale(__uint_as_float(m), &inv);
+    uint2 w = make_uint2(0, 0);
+    if (m < 0x7f800000u) {
+      w.x = fp8_pack4(v[t][0] * inv, v[t][1] * inv, v[t][2] * inv, v[t][3] * inv);
+      w.y = fp8_pack4(v[t][4] * inv, v[t][5] * inv, v[t][6] * inv, v[t][7] * inv);
+    }
+    if (b < p.kb) {
+      *reinterpret_cast<uint2*>(p.codes + ((size_t)r * p.kb + b) * FP8_BLOCK + 8 * sub) = w;
+      if (sub == 0) p.scale[(size_t)b * p.rows + r] = s;
+    }
+  }
+}
+
+template <typename T> static int launch_rows(Fp8RowsParams p, cudaStream_t st) {
+  const bool vec = p.K >= 8 && p.ldx * (long long)sizeof(T) % 16 == 0 && ((uintptr_t)p.x & 15) == 0;
+  // pairs of blocks per warp: four where that leaves the SMs eight warps each, one for the few rows of a decode step
+  const bool many = (long long)p.rows * p.kb >= 8ll * 8 * sm_count();
+  const int per = many ? 8 : 2;
+  p.chunks = (p.kb + per - 1) / per;
+  const long long ctas = ((long long)p.rows * p.chunks + 7) / 8;
+  if (ctas >= 1ll << 28) return -106;
+  const dim3 grid((unsigned)ctas);
+  if (many) { if (vec) launch_pdl(fp8_rows_kernel<T, 4, true>, grid, dim3(256), 0, st, p); else launch_pdl(fp8_rows_kernel<T, 4, false>, grid, dim3(256), 0, st, p); }
+  else { if (vec) launch_pdl(fp8_rows_kernel<T, 1, true>, grid, dim3(256), 0, st, p); else launch_pdl(fp8_rows_kernel<T, 1, false>, grid, dim3(256), 0, st, p); }
+  return (int)cudaGetLastError();
 }
 
 }  // namespace mx
@@ -43,10 +120,6 @@ MX_HOST_API int mx_fp8_rows(const void* x, int f32, long long ldx, const int* in
   if (rows <= 0) return 0;
   if (K < 1 || x_rows < 0) return -101;
   if (((uintptr_t)codes) & 15) return -114;
-  const int kb = (K + FP8_BLOCK - 1) / FP8_BLOCK;
-  const long long ctas = ((long long)rows * kb + 7) / 8;
-  if (ctas > 0x7fffffffll) return -106;
-  if (f32) launch_pdl(fp8_rows_kernel<float>, dim3((unsigned)ctas), dim3(256), 0, st, (const float*)x, ldx, index, x_rows, rows, K, kb, (uint8_t*)codes, scale);
-  else launch_pdl(fp8_rows_kernel<__nv_bfloat16>, dim3((unsigned)ctas), dim3(256), 0, st, (const __nv_bfloat16*)x, ldx, index, x_rows, rows, K, kb, (uint8_t*)codes, scale);
-  return (int)cudaGetLastError();
+  Fp8RowsParams p{x, ldx, index, x_rows, rows, K, (K + FP8_BLOCK - 1) / FP8_BLOCK, 0, (uint8_t*)codes, scale};
+  return f32 ? launch_rows<float>(p, st) : launch_rows<__nv_bfloat16>(p, st);
 }
