@@ -111,6 +111,40 @@ struct Fp8Params {
   int* status;
 };
 
+// A product as the caller describes it (ops/cuda.py packs the fields in this order).
+struct Fp8Call {
+  const void* xb;            // bf16 rows, rounded into codes and scale first; null: these hold the rounded rows
+  long long ldx;
+  const int* index;          // row of xb that rounded row r is; null: r
+  void* codes;               // [rows][kb * 128]
+  float* scale;              // [kb][rows]
+  const void* w;
+  const float* sw;
+  void* c;
+  long long ldc;
+  const float* bias;         // the rest as in Fp8Params
+  const float* row_scale;
+  const int* counts;
+  const int* seg;
+  const int* slot;
+  float* scratch;            // streaming kernel: partial sums, and the counters of cut work (host_util.h)
+  int* tickets;
+  int xb_rows, rows;         // rows of xb, and rounded rows
+  int M, N, K, E, out_f32, act, x_div, e_lo;
+  int nt, bn;                // rows of a group of the streaming kernel, or 0 and the columns of a tile of the tiled one
+  float act_alpha, act_limit;
+};
+int fp8_rows_launch(const void* x, int f32, long long ldx, const int* index, int x_rows, int rows, int K, void* codes, float* scale, cudaStream_t st);
+int fp8_stream_launch(const Fp8Call& c, cudaStream_t st);
+int fp8_gemm_launch(const Fp8Call& c, cudaStream_t st);
+inline Fp8Params fp8_params(const Fp8Call& c) {
+  Fp8Params p{};
+  p.sx = c.scale; p.x_rows = c.rows; p.sw = c.sw; p.C = c.c; p.ldc = c.ldc; p.out_f32 = c.out_f32; p.M = c.M; p.N = c.N; p.kb = (c.K + FP8_BLOCK - 1) / FP8_BLOCK; p.E = c.E;
+  p.bias = c.bias; p.row_scale = c.row_scale; p.act = c.act; p.act_alpha = c.act_alpha; p.act_limit = c.act_limit; p.counts = c.counts; p.seg = c.seg; p.slot = c.slot;
+  p.x_div = c.x_div; p.e_lo = c.e_lo; p.part = c.scratch; p.tickets = c.tickets; p.status = status_word();
+  return p;
+}
+
 // Boxes of `rows` rows by one block of codes [E][n][kb * 128] (E = 0: [n][kb * 128]).  Codes travel as two-byte elements: the tile is bytes either way.
 inline int fp8_tmap(CUtensorMap* out, const void* codes, int kb, int n, int E, int rows) {
   const uint64_t row = (uint64_t)kb * FP8_BLOCK;

@@ -313,33 +313,41 @@ template <int BN, int KIND, bool F32> static int launch_gemm(const CUtensorMap& 
   return (int)cudaGetLastError();
 }
 
-}  // namespace mx
-
-using namespace mx;
-
-// Dense (M rows) or experts (counts / seg: from the bank's first expert on; M rows of the packing).  bn: 128 or 256 columns a tile.
-MX_HOST_API int mx_fp8_gemm(const void* x, const float* sx, int x_rows, const void* w, const float* sw, int E, void* c, long long ldc, int out_f32, const float* bias,
-                            const float* row_scale, int act, float act_alpha, float act_limit, int M, int N, int K, const int* counts, const int* seg, int bn,
-                            cudaStream_t st) {
-  if (M <= 0 || N <= 0) return 0;
-  const int kb = (K + FP8_BLOCK - 1) / FP8_BLOCK;
-  if (K < 1 || E < 1 || E > FG_MAX_E || x_rows < 1 || (bn != 128 && bn != 256)) return -101;
-  if (act_gated(act) && N % 32) return -104;
-  if (((uintptr_t)x | (uintptr_t)w) & 15) return -114;
-  if (counts && (M + FG_BM - 1) / FG_BM + E > 65535) return -106;
-  const long long tiles = ((M + FG_BM - 1) / FG_BM + (counts ? (E < M ? E : M) : 0)) * (long long)((N + bn - 1) / bn);
+// Dense (M rows) or experts (counts / seg: from the bank's first expert on; M rows of the packing), tiles of bn = 128 or 256 columns.
+int fp8_gemm_launch(const Fp8Call& c, cudaStream_t st) {
+  const Fp8Params p = fp8_params(c);
+  const int bn = c.bn;
+  if (c.E > FG_MAX_E || c.slot || (bn != 128 && bn != 256) || (c.counts && (c.M + FG_BM - 1) / FG_BM + c.E > 65535)) return -106;
+  if (((uintptr_t)c.codes | (uintptr_t)c.w) & 15) return -114;
+  const long long tiles = ((c.M + FG_BM - 1) / FG_BM + (c.counts ? (c.E < c.M ? c.E : c.M) : 0)) * (long long)((c.N + bn - 1) / bn);
   if (tiles >= 1ll << 31) return -106;
-  Fp8Params p{};
-  p.sx = sx; p.x_rows = x_rows; p.sw = sw; p.C = c; p.ldc = ldc; p.out_f32 = out_f32; p.M = M; p.N = N; p.kb = kb; p.E = E; p.bias = bias; p.row_scale = row_scale;
-  p.act = act; p.act_alpha = act_alpha; p.act_limit = act_limit; p.counts = counts; p.seg = seg; p.x_div = 1; p.status = status_word();
   CUtensorMap tx, tw;
-  int r = fp8_tmap(&tx, x, kb, x_rows, 0, FG_BM);
-  if (!r) r = fp8_tmap(&tw, w, kb, N, E, bn);
+  int r = fp8_tmap(&tx, c.codes, p.kb, c.rows, 0, FG_BM);
+  if (!r) r = fp8_tmap(&tw, c.w, p.kb, p.N, c.E, bn);
   if (r) return r;
-  const int kind = act == 0 ? 0 : act_gated(act) ? 1 : 2;
-#define MX_FG(BN_, KIND_) if (bn == BN_ && kind == KIND_) return out_f32 ? launch_gemm<BN_, KIND_, true>(tx, tw, p, tiles, st) : launch_gemm<BN_, KIND_, false>(tx, tw, p, tiles, st)
+  const int kind = p.act == 0 ? 0 : act_gated(p.act) ? 1 : 2;
+#define MX_FG(BN_, KIND_) if (bn == BN_ && kind == KIND_) return p.out_f32 ? launch_gemm<BN_, KIND_, true>(tx, tw, p, tiles, st) : launch_gemm<BN_, KIND_, false>(tx, tw, p, tiles, st)
   MX_FG(256, 0); MX_FG(256, 1); MX_FG(256, 2);
   MX_FG(128, 0); MX_FG(128, 1); MX_FG(128, 2);
 #undef MX_FG
   return -106;
+}
+
+}  // namespace mx
+
+using namespace mx;
+
+MX_HOST_API int mx_fp8_call_bytes() { return (int)sizeof(Fp8Call); }
+
+// A product (see Fp8Call): the rows are rounded where they are bf16 still, then the streaming kernel (nt) or the tiled one (bn) runs.
+MX_HOST_API int mx_fp8_product(const Fp8Call* call, cudaStream_t st) {
+  const Fp8Call& c = *call;
+  if (c.M <= 0 || c.N <= 0) return 0;
+  if (c.K < 1 || c.x_div < 1 || c.E < 1 || c.rows < 1) return -101;
+  if (act_gated(c.act) && c.N % 32) return -104;
+  if (c.xb) {
+    const int r = fp8_rows_launch(c.xb, 0, c.ldx, c.index, c.xb_rows, c.rows, c.K, c.codes, c.scale, st);
+    if (r) return r;
+  }
+  return c.nt ? fp8_stream_launch(c, st) : fp8_gemm_launch(c, st);
 }

@@ -1,7 +1,7 @@
 // Rows of activations as e4m3 codes with a power-of-two scale per 128 elements: codes [rows][KB * 128] (zeros past K), scales [KB][rows].
 //
 // Bound: memory.  Sixteen lanes take a block, eight elements each: 16-byte loads, a maximum of bit patterns over the half-warp, 8-byte stores.  A warp has IT
-// such pairs of blocks of a row under way.  The warps of eight neighbouring rows lie side by side, so that their scales, four bytes each, share a sector.
+// such pairs of blocks of a row under way, and eight CTAs share an SM.  The warps of eight neighbouring rows lie side by side, so that their scales, four bytes each, share a sector.
 #include "act.cuh"
 #include "common.cuh"
 #include "fp8.cuh"
@@ -18,25 +18,69 @@ struct Fp8RowsParams {
   float* scale;
 };
 
-template <typename T> struct Row8;       // eight elements as they were loaded
+// Eight elements as they were loaded, and the bits of their largest magnitude: 16 for bf16, which are the high half of an fp32's.
+template <typename T> struct Row8;
 template <> struct Row8<__nv_bfloat16> {
-  uint4 v;
-  __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = __ldg(reinterpret_cast<const uint4*>(p)); }
-  __device__ __forceinline__ void get(float (&f)[8]) const {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { f[2 * i] = bf16_lo(w[i]); f[2 * i + 1] = bf16_hi(w[i]); }
+  uint32_t w[4];
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) {
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+  }
+  __device__ __forceinline__ void zero() { w[0] = w[1] = w[2] = w[3] = 0; }
+  __device__ __forceinline__ void put(int j, __nv_bfloat16 v) { w[j >> 1] |= (uint32_t)__bfloat16_as_ushort(v) << (16 * (j & 1)); }
+  __device__ __forceinline__ uint32_t top() const {
+    const uint32_t k = 0x7fff7fffu, m = __vmaxu2(__vmaxu2(w[0] & k, w[1] & k), __vmaxu2(w[2] & k, w[3] & k));
+    return max(m & 0xffffu, m >> 16);
+  }
+  __device__ __forceinline__ uint2 codes(float inv) const {
+    return make_uint2(fp8_pack4(bf16_lo(w[0]) * inv, bf16_hi(w[0]) * inv, bf16_lo(w[1]) * inv, bf16_hi(w[1]) * inv),
+                      fp8_pack4(bf16_lo(w[2]) * inv, bf16_hi(w[2]) * inv, bf16_lo(w[3]) * inv, bf16_hi(w[3]) * inv));
   }
 };
 template <> struct Row8<float> {
-  float4 a, b;
-  __device__ __forceinline__ void load(const float* p) { a = __ldg(reinterpret_cast<const float4*>(p)); b = __ldg(reinterpret_cast<const float4*>(p) + 1); }
-  __device__ __forceinline__ void get(float (&f)[8]) const { f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w; }
+  float f[8];
+  __device__ __forceinline__ void load(const float* p) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = 0.f;
+  }
+  __device__ __forceinline__ void put(int j, float v) { f[j] = v; }
+  __device__ __forceinline__ uint32_t top() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, fp8_mag(f[j]));
+    return m;
+  }
+  __device__ __forceinline__ uint2 codes(float inv) const {
+    return make_uint2(fp8_pack4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv), fp8_pack4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
+  }
 };
+// the largest over the sixteen lanes of a block, for IT blocks: bf16 magnitudes of two blocks share a register on the way
+template <int IT> __device__ __forceinline__ void half_warp_max(uint32_t (&m)[IT], __nv_bfloat16) {
+  constexpr int W = (IT + 1) / 2;
+  uint32_t w[W];
+#pragma unroll
+  for (int t = 0; t < W; ++t) w[t] = m[2 * t] | (2 * t + 1 < IT ? m[2 * t + 1 < IT ? 2 * t + 1 : 0] << 16 : 0u);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+    for (int t = 0; t < W; ++t) w[t] = __vmaxu2(w[t], __shfl_xor_sync(0xffffffffu, w[t], o));
+#pragma unroll
+  for (int t = 0; t < IT; ++t) m[t] = t & 1 ? w[t / 2] & 0xffff0000u : w[t / 2] << 16;
+}
+template <int IT> __device__ __forceinline__ void half_warp_max(uint32_t (&m)[IT], float) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+    for (int t = 0; t < IT; ++t) m[t] = max(m[t], __shfl_xor_sync(0xffffffffu, m[t], o));
+}
 
 // VEC: rows start on 16 bytes
 template <typename T, int IT, bool VEC>
-__global__ void __launch_bounds__(256) fp8_rows_kernel(const Fp8RowsParams p) {
+__global__ void __launch_bounds__(256, VEC && sizeof(T) == 2 ? 8 : 4) fp8_rows_kernel(const Fp8RowsParams p) {
   pdl_prologue();
   const int lane = threadIdx.x & 31, half = lane >> 4, sub = lane & 15;
   const int unit = blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -47,49 +91,34 @@ __global__ void __launch_bounds__(256) fp8_rows_kernel(const Fp8RowsParams p) {
   const int src = p.index ? p.index[r] : r;
   const bool some = src >= 0 && src < p.x_rows;
   const T* row = (const T*)p.x + (some ? src : 0) * p.ldx;
-  const int b0 = chunk * 2 * IT + half;
-  float v[IT][8];
-  if constexpr (VEC) {
-    Row8<T> raw[IT];
+  const int b0 = chunk * 2 * IT + half, at0 = b0 * FP8_BLOCK + 8 * sub;
+  Row8<T> v[IT];
+  if (VEC) {
 #pragma unroll
-    for (int t = 0; t < IT; ++t) {
-      const int at = (b0 + 2 * t) * FP8_BLOCK + 8 * sub;
-      raw[t].load(row + (at + 8 <= p.K ? at : 0));         // (the row's first elements where the lane's are not whole; K is 8 at least)
-    }
-#pragma unroll
-    for (int t = 0; t < IT; ++t) {
-      const int at = (b0 + 2 * t) * FP8_BLOCK + 8 * sub;
-      raw[t].get(v[t]);
-      if (!some || at + 8 > p.K) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[t][j] = some && at + j < p.K ? to_f32<T>(row[at + j]) : 0.f;
-      }
-    }
-  } else {
-#pragma unroll
-    for (int t = 0; t < IT; ++t)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int at = (b0 + 2 * t) * FP8_BLOCK + 8 * sub + j;
-        v[t][j] = some && at < p.K ? to_f32<T>(row[at]) : 0.f;
-      }
+    for (int t = 0; t < IT; ++t) v[t].load(row + (at0 + t * 2 * FP8_BLOCK + 8 <= p.K ? at0 + t * 2 * FP8_BLOCK : 0));      // (K is 8 at least)
   }
+  if (!VEC || !some || (chunk + 1) * 2 * IT * FP8_BLOCK > p.K) {                // the row's last run, or no row
+#pragma unroll
+    for (int t = 0; t < IT; ++t) {
+      const int at = at0 + t * 2 * FP8_BLOCK;
+      if (VEC && some && at + 8 <= p.K) continue;
+      v[t].zero();
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (some && at + j < p.K) v[t].put(j, row[at + j]);
+    }
+  }
+  uint32_t m[IT];
+#pragma unroll
+  for (int t = 0; t < IT; ++t) m[t] = v[t].top();
+  half_warp_max<IT>(m, T());
 #pragma unroll
   for (int t = 0; t < IT; ++t) {
     const int b = b0 + 2 * t;
-    uint32_t m = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) m = max(m, fp8_mag(v[t][j]));
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (src >= p.x_rows) m = 0x7fc00000u;                  // no such row: NaN
+    if (src >= p.x_rows) m[t] = 0x7fc00000u;               // no such row: NaN
     float inv;
-    const float s = fp8_scale(__uint_as_float(m), &inv);
-    uint2 w = make_uint2(0, 0);
-    if (m < 0x7f800000u) {
-      w.x = fp8_pack4(v[t][0] * inv, v[t][1] * inv, v[t][2] * inv, v[t][3] * inv);
-      w.y = fp8_pack4(v[t][4] * inv, v[t][5] * inv, v[t][6] * inv, v[t][7] * inv);
-    }
+    const float s = fp8_scale(__uint_as_float(m[t]), &inv);
+    const uint2 w = m[t] < 0x7f800000u ? v[t].codes(inv) : make_uint2(0, 0);
     if (b < p.kb) {
       *reinterpret_cast<uint2*>(p.codes + ((size_t)r * p.kb + b) * FP8_BLOCK + 8 * sub) = w;
       if (sub == 0) p.scale[(size_t)b * p.rows + r] = s;
@@ -111,15 +140,17 @@ template <typename T> static int launch_rows(Fp8RowsParams p, cudaStream_t st) {
   return (int)cudaGetLastError();
 }
 
-}  // namespace mx
-
-using namespace mx;
-
 // x: bf16 (f32 = 0) or fp32 rows, `ldx` elements apart, K of them used; index: row r of the result is row index[r] of x (negative: zeros; past the end: NaN).
-MX_HOST_API int mx_fp8_rows(const void* x, int f32, long long ldx, const int* index, int x_rows, int rows, int K, void* codes, float* scale, cudaStream_t st) {
+int fp8_rows_launch(const void* x, int f32, long long ldx, const int* index, int x_rows, int rows, int K, void* codes, float* scale, cudaStream_t st) {
   if (rows <= 0) return 0;
   if (K < 1 || x_rows < 0) return -101;
   if (((uintptr_t)codes) & 15) return -114;
   Fp8RowsParams p{x, ldx, index, x_rows, rows, K, (K + FP8_BLOCK - 1) / FP8_BLOCK, 0, (uint8_t*)codes, scale};
   return f32 ? launch_rows<float>(p, st) : launch_rows<__nv_bfloat16>(p, st);
+}
+
+}  // namespace mx
+
+MX_HOST_API int mx_fp8_rows(const void* x, int f32, long long ldx, const int* index, int x_rows, int rows, int K, void* codes, float* scale, cudaStream_t st) {
+  return mx::fp8_rows_launch(x, f32, ldx, index, x_rows, rows, K, codes, scale, st);
 }

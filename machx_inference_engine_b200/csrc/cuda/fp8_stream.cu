@@ -338,34 +338,16 @@ template <int NT> static int launch_stream(const CUtensorMap& tw, const CUtensor
   return (int)cudaGetLastError();
 }
 
-}  // namespace mx
-
-using namespace mx;
-
-// Floats of scratch (16-byte aligned) that mx_fp8_stream wants for groups of up to `nt` rows.
-MX_HOST_API int mx_fp8_stream_scratch(int nt) { return FS_MAX_GRID * 2 * FS_TILE * nt; }
-
-// Whether the units of a launch can be counted: `groups` is the most there can be.
-MX_HOST_API int mx_fp8_stream_takes(long long groups, int N, int kb, int E) {
-  return E <= FS_MAX_E && groups < 65536 && groups * ((N + FS_TILE - 1) / FS_TILE) * kb < (1ll << 30);
-}
-
-// Codes x and scales sx of x_rows rows against w.  Dense (M <= nt), experts (counts / seg: from the bank's first expert on) or slots (slot).  nt 16, 32, 64 or 128: rows of a
-// group, padded.  tickets: see host_util.h.
-MX_HOST_API int mx_fp8_stream(const void* x, const float* sx, int x_rows, const void* w, const float* sw, int E, void* c, long long ldc, int out_f32, const float* bias,
-                              const float* row_scale, int act, float act_alpha, float act_limit, int M, int N, int K, const int* counts, const int* seg, const int* slot,
-                              int x_div, int e_lo, int nt, float* scratch, int* tickets, cudaStream_t st) {
-  if (M <= 0 || N <= 0) return 0;
-  const int kb = (K + FP8_BLOCK - 1) / FP8_BLOCK;
-  if (K < 1 || x_div < 1 || E < 1 || x_rows < 1) return -101;
-  if (act_gated(act) && N % 32) return -104;
-  const long long groups = slot ? M : counts ? (long long)M / nt + (E < M ? E : M) + 1 : 1;
-  if (!mx_fp8_stream_takes(groups, N, kb, E) || (!slot && !counts && M > nt)) return -106;
-  if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)scratch) & 15) return -114;
-  Fp8Params p{sx, x_rows, sw, c, ldc, out_f32, M, N, kb, E, bias, row_scale, act, act_alpha, act_limit, counts, seg, slot, x_div, e_lo, scratch, tickets, status_word()};
+// Dense (M <= nt), experts (counts / seg) or slots (slot), in groups of nt = 16, 32, 64 or 128 rows.
+int fp8_stream_launch(const Fp8Call& c, cudaStream_t st) {
+  const Fp8Params p = fp8_params(c);
+  const int nt = c.nt;
+  const long long groups = c.slot ? c.M : c.counts ? (long long)c.M / nt + (c.E < c.M ? c.E : c.M) + 1 : 1;
+  if (c.E > FS_MAX_E || groups >= 65536 || groups * ((p.N + FS_TILE - 1) / FS_TILE) * p.kb >= 1ll << 30 || (!c.slot && !c.counts && c.M > nt)) return -106;      // (units are counted in 32 bits)
+  if (((uintptr_t)c.codes | (uintptr_t)c.w | (uintptr_t)c.scratch) & 15) return -114;
   CUtensorMap tw, tx;
-  int r = fp8_tmap(&tw, w, kb, N, E, FS_TILE);
-  if (!r) r = fp8_tmap(&tx, x, kb, x_rows, 0, nt);
+  int r = fp8_tmap(&tw, c.w, p.kb, p.N, c.E, FS_TILE);
+  if (!r) r = fp8_tmap(&tx, c.codes, p.kb, c.rows, 0, nt);
   if (r) return r;
   switch (nt) {
     case 16: return launch_stream<16>(tw, tx, p, st);
@@ -375,3 +357,8 @@ MX_HOST_API int mx_fp8_stream(const void* x, const float* sx, int x_rows, const 
     default: return -106;
   }
 }
+
+}  // namespace mx
+
+// Bytes of scratch (16-byte aligned) that a launch with groups of up to `nt` rows wants.
+MX_HOST_API long long mx_fp8_stream_scratch(int nt) { return 4ll * mx::FS_MAX_GRID * 2 * mx::FS_TILE * nt; }

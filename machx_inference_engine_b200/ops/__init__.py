@@ -8,6 +8,8 @@ from __future__ import annotations
 
 import functools
 
+import torch
+
 from . import ref
 from .ref import ACT_GEGLU, ACT_GELU_TANH, ACT_NONE, ACT_RELU2, ACT_SWIGLU, ACT_SWIGLU_OAI, ACT_TANH, ACT_XIELU, MOE_TILE, BranchMean, ExpertSum, MoePacking, PoolPages, act_gated, moe_max_rows
 from .fp8 import FP8Rows
@@ -41,7 +43,8 @@ def backend() -> str:
 
 
 def _first_tensor(args, kwargs):
-    import torch
+    if args and isinstance(args[0], torch.Tensor):
+        return args[0]
     for a in list(args) + list(kwargs.values()):
         if isinstance(a, torch.Tensor):
             return a

@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 import threading
 from typing import Optional
 
@@ -865,13 +866,10 @@ def grouped_linear(xp, w: QuantWeight, tile_expert, num_tiles, bias=None, act=AC
 def expert_gemv(x, w: QuantWeight, slot_expert, x_div=1, bias=None, act=ACT_NONE, act_alpha=1.702, act_limit=7.0, slot_scale=None, out_f32=False,
                 e_lo=0):
     """``w`` holds experts [e_lo, e_lo + w.E); slots routed to other experts produce zero rows (expert parallelism)."""
+    if w.fmt == WFormat.FP8:
+        return _expert_gemv_fp8(x, w, slot_expert, x_div, bias, act, act_alpha, act_limit, slot_scale, out_f32, e_lo)
     S = slot_expert.numel()
     n_out = w.N // 2 if act_gated(act) else w.N
-    if w.fmt == WFormat.FP8:
-        _fp8.check_slots(x, w, slot_expert, x_div, bias, act_gated(act), slot_scale)
-        with _on(x.device):
-            out = torch.empty(S, n_out, dtype=torch.float32 if out_f32 else torch.bfloat16, device=x.device)
-            return _fp8_product(x, w, out, bias, slot_scale, act, act_alpha, act_limit, slot=slot_expert, x_div=x_div, e_lo=e_lo)
     out = torch.empty(S, n_out, dtype=torch.float32 if out_f32 else torch.bfloat16, device=x.device)
     fmt, p0, p1, p2, p3 = _planes(w)
     _check(_lib.cuda().mx_gemv_experts(fmt, p0, p1, p2, p3, _p(x), _p(out), _p(bias), w.N, w.K, int(out_f32), act, C.c_float(act_alpha),
@@ -882,54 +880,71 @@ def expert_gemv(x, w: QuantWeight, slot_expert, x_div=1, bias=None, act=ACT_NONE
 
 
 # ------------------------------------------------------------------ 8-bit floating point (see ops/fp8.py)
-class _Nothing:
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return False
+FP8_STREAM_ROWS = (16, 32, 64, 128)      # rows of a group in the weight-streaming kernel
+_FP8_CALL = struct.Struct("<16q12i2f")   # csrc/cuda/fp8.cuh: Fp8Call
+_fp8_lib = None
 
 
-def _on(device):
-    """Launches and allocations go to ``device``, whichever is current."""
-    return _Nothing() if device.index is None or device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def _fp8_entry():
+    """The library with the signatures of the entries below: plain integers for pointers, which a decode step is too short to wrap one by one."""
+    global _fp8_lib
+    lib = _lib.cuda()
+    if lib is not _fp8_lib:
+        lib.mx_fp8_rows.argtypes = [_vp, C.c_int, C.c_longlong, _vp, C.c_int, C.c_int, C.c_int, _vp, _vp, _vp]
+        lib.mx_fp8_product.argtypes = [C.c_char_p, _vp]
+        lib.mx_fp8_stream_scratch.restype = C.c_longlong
+        if lib.mx_fp8_call_bytes() != _FP8_CALL.size:
+            raise KernelError("the kernel library's description of an FP8 product is another one: rebuild it")
+        _fp8_lib = lib
+    return lib
+
+
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
 
 
 def fp8_rows(x, index=None) -> FP8Rows:
     _fp8.check_rows(x, index)
-    with _on(x.device):
-        rows, K = x.shape[0] if index is None else index.numel(), x.shape[1]
-        kb = -(-K // _fp8.FP8_BLOCK)
-        q = FP8Rows(torch.empty(rows, kb * _fp8.FP8_BLOCK, dtype=torch.float8_e4m3fn, device=x.device), torch.empty(kb, rows, dtype=torch.float32, device=x.device), K)
-        if rows:
-            _check(_lib.cuda().mx_fp8_rows(_p(x), int(x.dtype == torch.float32), C.c_longlong(x.stride(0)), _p(index), x.shape[0], rows, K, _p(q.codes), _p(q.scale),
-                                           _stream()), "fp8_rows")
-            _count()
-    return q
+    dev = x.device
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return fp8_rows(x, index)
+    rows, K = x.shape if index is None else (index.numel(), x.shape[1])
+    kb = -(-K // _fp8.FP8_BLOCK)
+    codes = torch.empty((rows, kb * _fp8.FP8_BLOCK), dtype=torch.float8_e4m3fn, device=dev)
+    scale = torch.empty((kb, rows), dtype=torch.float32, device=dev)
+    if rows:
+        _check(_fp8_entry().mx_fp8_rows(x.data_ptr(), x.dtype == torch.float32, x.stride(0), _ptr(index), x.shape[0], rows, K, codes.data_ptr(), scale.data_ptr(),
+                                        torch._C._cuda_getCurrentRawStream(dev.index)), "fp8_rows")
+        _count()
+    return FP8Rows(codes, scale, K)
 
 
-FP8_STREAM_ROWS = (16, 32, 64, 128)      # rows of a group in the weight-streaming kernel
-
-
-def _fp8_stream(x, w: QuantWeight, out, bias, row_scale, act, act_alpha, act_limit, nt, counts=None, seg=None, slot=None, x_div=1, e_lo=0, index=None):
-    """The weight-streaming kernel (csrc/cuda/fp8_stream.cu) with groups of up to ``nt`` rows."""
-    lib = _lib.cuda()
-    q = x if isinstance(x, FP8Rows) else fp8_rows(x, index)
-    scratch = torch.empty(lib.mx_fp8_stream_scratch(nt), dtype=torch.float32, device=out.device)
-    tickets = _tickets(out.device)
-    _check(lib.mx_fp8_stream(_p(q.codes), _p(q.scale), q.codes.shape[0], _p(w.p0), _p(w.p1), w.E, _p(out), C.c_longlong(out.stride(0)), int(out.dtype == torch.float32),
-                             _p(bias), _p(row_scale), act, C.c_float(act_alpha), C.c_float(act_limit), out.shape[0], w.N, w.K, _p(counts), _p(seg), _p(slot), int(x_div),
-                             int(e_lo), nt, _p(scratch), tickets[1], tickets[2]), "fp8_stream")
-    _count()
-    return out
-
-
-def _fp8_tiles(x, w: QuantWeight, out, bias, row_scale, act, act_alpha, act_limit, bn, counts=None, seg=None, index=None):
-    """The tiled kernel (csrc/cuda/fp8_gemm.cu) with ``bn`` columns a tile."""
-    q = x if isinstance(x, FP8Rows) else fp8_rows(x, index)
-    _check(_lib.cuda().mx_fp8_gemm(_p(q.codes), _p(q.scale), q.codes.shape[0], _p(w.p0), _p(w.p1), w.E, _p(out), C.c_longlong(out.stride(0)), int(out.dtype == torch.float32),
-                                   _p(bias), _p(row_scale), act, C.c_float(act_alpha), C.c_float(act_limit), out.shape[0], w.N, w.K, _p(counts), _p(seg), bn, _stream()),
-           "fp8_gemm")
+def _fp8_call(x, w: QuantWeight, out, bias, row_scale, act, act_alpha, act_limit, nt=0, bn=0, counts=None, seg=None, slot=None, x_div=1, e_lo=0, index=None):
+    """One product on the current device: ``nt`` rows of a group (csrc/cuda/fp8_stream.cu) or ``bn`` columns of a tile (csrc/cuda/fp8_gemm.cu).  bf16 rows are rounded into a
+    scratch buffer first, by the same call.  The scratch is an ordinary allocation: stream-ordered, of the graph's own pool under capture."""
+    lib = _fp8_entry()
+    dev = out.device
+    K, kb = w.K, -(-w.K // _fp8.FP8_BLOCK)
+    work = lib.mx_fp8_stream_scratch(nt) if nt else 0
+    if isinstance(x, FP8Rows):
+        rows = x.codes.shape[0]
+        xb, ldx, xb_rows = 0, 0, 0
+        scratch = torch.empty(work, dtype=torch.uint8, device=dev) if work else None
+        at = _ptr(scratch)
+        codes, scale = x.codes.data_ptr(), x.scale.data_ptr()
+    else:
+        xb, ldx, xb_rows = x.data_ptr(), x.stride(0), x.shape[0]
+        rows = xb_rows if index is None else index.numel()
+        n = rows * kb
+        scratch = torch.empty(work + n * (_fp8.FP8_BLOCK + 4), dtype=torch.uint8, device=dev)
+        at = scratch.data_ptr()
+        codes, scale = at + work, at + work + n * _fp8.FP8_BLOCK
+    tickets = _tickets(dev) if nt else None
+    call = _FP8_CALL.pack(xb, ldx, _ptr(index), codes, scale, w.p0.data_ptr(), w.p1.data_ptr(), out.data_ptr(), out.stride(0), _ptr(bias), _ptr(row_scale), _ptr(counts), _ptr(seg),
+                          _ptr(slot), at, tickets[0].data_ptr() if nt else 0, xb_rows, rows, out.shape[0], w.N, K, w.E, out.dtype == torch.float32, act, x_div, e_lo, nt, bn,
+                          act_alpha, act_limit)
+    _check(lib.mx_fp8_product(call, torch._C._cuda_getCurrentRawStream(dev.index)), "fp8 product")
     _count()
     return out
 
@@ -940,36 +955,48 @@ def _fp8_bn(M: int, N: int) -> int:
     return 256 if 1.9 * waves(256) < waves(128) else 128
 
 
-def _fp8_product(x, w: QuantWeight, out, bias, row_scale, act, act_alpha, act_limit, counts=None, seg=None, slot=None, x_div=1, e_lo=0, index=None):
-    M = out.shape[0]
+def _fp8_product(x, w: QuantWeight, shape, dtype, out, bias, row_scale, act, act_alpha, act_limit, **kw):
+    """Checked arguments -> the result, on the rows' device, whichever is current."""
+    dev = x.device
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return _fp8_product(x, w, shape, dtype, out, bias, row_scale, act, act_alpha, act_limit, **kw)
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=dev)
+    M = shape[0]
     if M == 0:
         return out
-    if slot is not None:
-        return _fp8_stream(x, w, out, bias, row_scale, act, act_alpha, act_limit, 16, slot=slot, x_div=x_div, e_lo=e_lo)
-    rows = M if counts is None else 2 * M / w.E
-    nt = next((n for n in FP8_STREAM_ROWS if rows <= n), 0)
-    if nt:
-        return _fp8_stream(x, w, out, bias, row_scale, act, act_alpha, act_limit, nt, counts=counts, seg=seg, index=index)
-    return _fp8_tiles(x, w, out, bias, row_scale, act, act_alpha, act_limit, _fp8_bn(M, w.N), counts=counts, seg=seg, index=index)
+    if kw.get("slot") is not None:
+        nt = 16
+    else:
+        rows = M if kw.get("counts") is None else 2 * M / w.E
+        nt = 16 if rows <= 16 else 32 if rows <= 32 else 64 if rows <= 64 else 128 if rows <= 128 else 0
+    return _fp8_call(x, w, out, bias, row_scale, act, act_alpha, act_limit, nt, 0 if nt else _fp8_bn(M, w.N), **kw)
 
 
 def _linear_fp8(x, w: QuantWeight, bias, act, act_alpha, act_limit, out_f32, row_scale, out):
-    M, n_out, odt = x.shape[0], w.N // 2 if act_gated(act) else w.N, torch.float32 if out_f32 else torch.bfloat16
-    _fp8.check_product(x, w, False, M, bias, act_gated(act), "linear")
-    _fp8.check_out(out, row_scale, M, n_out, odt, x.device)
-    with _on(x.device):
-        if out is None:
-            out = torch.empty(M, n_out, dtype=odt, device=x.device)
-        return _fp8_product(x, w, out, bias, row_scale, act, act_alpha, act_limit)
+    gated = act_gated(act)
+    shape, dtype = (x.shape[0], w.N // 2 if gated else w.N), torch.float32 if out_f32 else torch.bfloat16
+    _fp8.check_product(x, w, False, shape[0], bias, gated, "linear")
+    if out is not None or row_scale is not None:
+        _fp8.check_out(out, row_scale, *shape, dtype, x.device)
+    return _fp8_product(x, w, shape, dtype, out, bias, row_scale, act, act_alpha, act_limit)
+
+
+def _expert_gemv_fp8(x, w: QuantWeight, slot_expert, x_div, bias, act, act_alpha, act_limit, slot_scale, out_f32, e_lo):
+    gated = act_gated(act)
+    _fp8.check_slots(x, w, slot_expert, x_div, bias, gated, slot_scale)
+    return _fp8_product(x, w, (slot_expert.numel(), w.N // 2 if gated else w.N), torch.float32 if out_f32 else torch.bfloat16, None, bias, slot_scale, act, act_alpha, act_limit,
+                        slot=slot_expert, x_div=int(x_div), e_lo=int(e_lo))
 
 
 def expert_linear(x, w: QuantWeight, pk: MoePacking, x_index=None, bias=None, act=ACT_NONE, act_alpha=1.702, act_limit=7.0, out_f32=False, e_lo=0):
-    P, n_out = pk.max_rows, w.N // 2 if act_gated(act) else w.N
-    _fp8.check_product(x, w, True, P, bias, act_gated(act), "expert_linear")
+    gated = act_gated(act)
+    P = pk.max_rows
+    _fp8.check_product(x, w, True, P, bias, gated, "expert_linear")
     _fp8.check_packing(pk, w, x, x_index, e_lo)
-    with _on(x.device):
-        out = torch.empty(P, n_out, dtype=torch.float32 if out_f32 else torch.bfloat16, device=x.device)
-        return _fp8_product(x, w, out, bias, None, act, act_alpha, act_limit, counts=pk.counts[e_lo:], seg=pk.seg_start[e_lo:], index=None if x_index is None else x_index[:P])
+    return _fp8_product(x, w, (P, w.N // 2 if gated else w.N), torch.float32 if out_f32 else torch.bfloat16, None, bias, None, act, act_alpha, act_limit,
+                        counts=pk.counts[e_lo:] if e_lo else pk.counts, seg=pk.seg_start[e_lo:] if e_lo else pk.seg_start, index=None if x_index is None else x_index[:P])
 
 
 # ------------------------------------------------------------------ attention

@@ -122,12 +122,12 @@ def test_each_kernel_at_every_tile_size(M, N, K):
     for rows in (x, q):
         for nt in (n for n in K_().FP8_STREAM_ROWS if n >= M):
             out = torch.empty(M, N, device=DEV)
-            assert O.rel(K_()._fp8_stream(rows, w, out, None, None, 0, 0.0, 0.0, nt), want) < tolerance(K), nt
-            assert O.rel(K_()._fp8_stream(rows, w, out, bias, rs, 0, 0.0, 0.0, nt), full) < tolerance(K), nt
+            assert O.rel(K_()._fp8_call(rows, w, out, None, None, 0, 0.0, 0.0, nt), want) < tolerance(K), nt
+            assert O.rel(K_()._fp8_call(rows, w, out, bias, rs, 0, 0.0, 0.0, nt), full) < tolerance(K), nt
         for bn in (128, 256):
             out = torch.empty(M, N, device=DEV)
-            assert O.rel(K_()._fp8_tiles(rows, w, out, None, None, 0, 0.0, 0.0, bn), want) < tolerance(K), bn
-            assert O.rel(K_()._fp8_tiles(rows, w, out, bias, rs, 0, 0.0, 0.0, bn), full) < tolerance(K), bn
+            assert O.rel(K_()._fp8_call(rows, w, out, None, None, 0, 0.0, 0.0, 0, bn), want) < tolerance(K), bn
+            assert O.rel(K_()._fp8_call(rows, w, out, bias, rs, 0, 0.0, 0.0, 0, bn), full) < tolerance(K), bn
 
 
 @pytest.mark.parametrize("act", ["none", "geglu"])
@@ -142,10 +142,10 @@ def test_each_kernel_over_experts(T, E, k, act):
     n = F // 2 if act != "none" else F
     for rows, index in ((x, pk.packed_token), (ops.fp8_rows(x, index=pk.packed_token), None)):
         for nt in K_().FP8_STREAM_ROWS:
-            got = K_()._fp8_stream(rows, w, torch.empty(T * k, n, device=DEV), None, None, ACTS[act], 1.702, 7.0, nt, index=index, **kw)
+            got = K_()._fp8_call(rows, w, torch.empty(T * k, n, device=DEV), None, None, ACTS[act], 1.702, 7.0, nt, index=index, **kw)
             assert O.rel(got[pk.pair_to_packed.long()], want) < tolerance(H, act), nt
         for bn in (128, 256):
-            got = K_()._fp8_tiles(rows, w, torch.empty(T * k, n, device=DEV), None, None, ACTS[act], 1.702, 7.0, bn, index=index, **kw)
+            got = K_()._fp8_call(rows, w, torch.empty(T * k, n, device=DEV), None, None, ACTS[act], 1.702, 7.0, 0, bn, index=index, **kw)
             assert O.rel(got[pk.pair_to_packed.long()], want) < tolerance(H, act), bn
 
 
