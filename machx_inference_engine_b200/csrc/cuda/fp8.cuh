@@ -30,6 +30,66 @@ __device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d
   return (uint32_t)lo | ((uint32_t)hi << 16);
 }
 
+// Eight elements as they were loaded, and the bits of their largest magnitude: 16 for bf16, which are the high half of an fp32's.
+template <typename T> struct Row8;
+template <> struct Row8<__nv_bfloat16> {
+  uint32_t w[4];
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) {
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+  }
+  __device__ __forceinline__ void zero() { w[0] = w[1] = w[2] = w[3] = 0; }
+  __device__ __forceinline__ void put(int j, __nv_bfloat16 v) { w[j >> 1] |= (uint32_t)__bfloat16_as_ushort(v) << (16 * (j & 1)); }
+  __device__ __forceinline__ uint32_t top() const {
+    const uint32_t k = 0x7fff7fffu, m = __vmaxu2(__vmaxu2(w[0] & k, w[1] & k), __vmaxu2(w[2] & k, w[3] & k));
+    return max(m & 0xffffu, m >> 16);
+  }
+  __device__ __forceinline__ uint2 codes(float inv) const {
+    return make_uint2(fp8_pack4(bf16_lo(w[0]) * inv, bf16_hi(w[0]) * inv, bf16_lo(w[1]) * inv, bf16_hi(w[1]) * inv),
+                      fp8_pack4(bf16_lo(w[2]) * inv, bf16_hi(w[2]) * inv, bf16_lo(w[3]) * inv, bf16_hi(w[3]) * inv));
+  }
+};
+template <> struct Row8<float> {
+  float f[8];
+  __device__ __forceinline__ void load(const float* p) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = 0.f;
+  }
+  __device__ __forceinline__ void put(int j, float v) { f[j] = v; }
+  __device__ __forceinline__ uint32_t top() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, fp8_mag(f[j]));
+    return m;
+  }
+  __device__ __forceinline__ uint2 codes(float inv) const {
+    return make_uint2(fp8_pack4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv), fp8_pack4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
+  }
+};
+// the largest over the sixteen lanes of a block, for IT blocks: bf16 magnitudes of two blocks share a register on the way
+template <int IT> __device__ __forceinline__ void half_warp_max(uint32_t (&m)[IT], __nv_bfloat16) {
+  constexpr int W = (IT + 1) / 2;
+  uint32_t w[W];
+#pragma unroll
+  for (int t = 0; t < W; ++t) w[t] = m[2 * t] | (2 * t + 1 < IT ? m[2 * t + 1 < IT ? 2 * t + 1 : 0] << 16 : 0u);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+    for (int t = 0; t < W; ++t) w[t] = __vmaxu2(w[t], __shfl_xor_sync(0xffffffffu, w[t], o));
+#pragma unroll
+  for (int t = 0; t < IT; ++t) m[t] = t & 1 ? w[t / 2] & 0xffff0000u : w[t / 2] << 16;
+}
+template <int IT> __device__ __forceinline__ void half_warp_max(uint32_t (&m)[IT], float) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+    for (int t = 0; t < IT; ++t) m[t] = max(m[t], __shfl_xor_sync(0xffffffffu, m[t], o));
+}
+
 // D[tmem] (+)= A[smem] * B[smem], e4m3 inputs (K = 32 a step), fp32 accumulate.  A whole warp comes here and `leader` (elect_one) issues: in a branch of one
 // thread the descriptors would have to be moved to uniform registers before every instruction (four products and two commits 470 -> see the kernels).
 __device__ __forceinline__ void umma_e4m3(uint32_t leader, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
@@ -92,6 +152,9 @@ __device__ __forceinline__ void arrive_copies(uint32_t bar) { asm volatile("cp.a
 
 // What a product multiplies and writes.
 struct Fp8Params {
+  const __nv_bfloat16* xb;   // rows that the streaming kernel rounds itself, `ldx` elements apart, of K
+  long long ldx;
+  int K;
   const float* sx;           // [kb][x_rows]
   int x_rows;
   const float* sw;           // [E][ceil(N / 16)][kb]
@@ -135,11 +198,12 @@ struct Fp8Call {
   float act_alpha, act_limit;
 };
 int fp8_rows_launch(const void* x, int f32, long long ldx, const int* index, int x_rows, int rows, int K, void* codes, float* scale, cudaStream_t st);
-int fp8_stream_launch(const Fp8Call& c, cudaStream_t st);
+bool fp8_stream_rounds(const Fp8Call& c);
+int fp8_stream_launch(const Fp8Call& c, bool round, cudaStream_t st);
 int fp8_gemm_launch(const Fp8Call& c, cudaStream_t st);
 inline Fp8Params fp8_params(const Fp8Call& c) {
   Fp8Params p{};
-  p.sx = c.scale; p.x_rows = c.rows; p.sw = c.sw; p.C = c.c; p.ldc = c.ldc; p.out_f32 = c.out_f32; p.M = c.M; p.N = c.N; p.kb = (c.K + FP8_BLOCK - 1) / FP8_BLOCK; p.E = c.E;
+  p.sx = c.scale; p.x_rows = c.rows; p.sw = c.sw; p.C = c.c; p.ldc = c.ldc; p.out_f32 = c.out_f32; p.M = c.M; p.N = c.N; p.K = c.K; p.kb = (c.K + FP8_BLOCK - 1) / FP8_BLOCK; p.E = c.E;
   p.bias = c.bias; p.row_scale = c.row_scale; p.act = c.act; p.act_alpha = c.act_alpha; p.act_limit = c.act_limit; p.counts = c.counts; p.seg = c.seg; p.slot = c.slot;
   p.x_div = c.x_div; p.e_lo = c.e_lo; p.part = c.scratch; p.tickets = c.tickets; p.status = status_word();
   return p;

@@ -339,15 +339,16 @@ using namespace mx;
 
 MX_HOST_API int mx_fp8_call_bytes() { return (int)sizeof(Fp8Call); }
 
-// A product (see Fp8Call): the rows are rounded where they are bf16 still, then the streaming kernel (nt) or the tiled one (bn) runs.
+// A product (see Fp8Call): rows that are bf16 still are rounded, then the streaming kernel (nt) or the tiled one (bn) runs.
 MX_HOST_API int mx_fp8_product(const Fp8Call* call, cudaStream_t st) {
   const Fp8Call& c = *call;
   if (c.M <= 0 || c.N <= 0) return 0;
   if (c.K < 1 || c.x_div < 1 || c.E < 1 || c.rows < 1) return -101;
   if (act_gated(c.act) && c.N % 32) return -104;
-  if (c.xb) {
+  const bool round = fp8_stream_rounds(c);
+  if (c.xb && !round) {
     const int r = fp8_rows_launch(c.xb, 0, c.ldx, c.index, c.xb_rows, c.rows, c.K, c.codes, c.scale, st);
     if (r) return r;
   }
-  return c.nt ? fp8_stream_launch(c, st) : fp8_gemm_launch(c, st);
+  return c.nt ? fp8_stream_launch(c, round, st) : fp8_gemm_launch(c, st);
 }

@@ -18,66 +18,6 @@ struct Fp8RowsParams {
   float* scale;
 };
 
-// Eight elements as they were loaded, and the bits of their largest magnitude: 16 for bf16, which are the high half of an fp32's.
-template <typename T> struct Row8;
-template <> struct Row8<__nv_bfloat16> {
-  uint32_t w[4];
-  __device__ __forceinline__ void load(const __nv_bfloat16* p) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
-    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-  }
-  __device__ __forceinline__ void zero() { w[0] = w[1] = w[2] = w[3] = 0; }
-  __device__ __forceinline__ void put(int j, __nv_bfloat16 v) { w[j >> 1] |= (uint32_t)__bfloat16_as_ushort(v) << (16 * (j & 1)); }
-  __device__ __forceinline__ uint32_t top() const {
-    const uint32_t k = 0x7fff7fffu, m = __vmaxu2(__vmaxu2(w[0] & k, w[1] & k), __vmaxu2(w[2] & k, w[3] & k));
-    return max(m & 0xffffu, m >> 16);
-  }
-  __device__ __forceinline__ uint2 codes(float inv) const {
-    return make_uint2(fp8_pack4(bf16_lo(w[0]) * inv, bf16_hi(w[0]) * inv, bf16_lo(w[1]) * inv, bf16_hi(w[1]) * inv),
-                      fp8_pack4(bf16_lo(w[2]) * inv, bf16_hi(w[2]) * inv, bf16_lo(w[3]) * inv, bf16_hi(w[3]) * inv));
-  }
-};
-template <> struct Row8<float> {
-  float f[8];
-  __device__ __forceinline__ void load(const float* p) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-  }
-  __device__ __forceinline__ void zero() {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = 0.f;
-  }
-  __device__ __forceinline__ void put(int j, float v) { f[j] = v; }
-  __device__ __forceinline__ uint32_t top() const {
-    uint32_t m = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) m = max(m, fp8_mag(f[j]));
-    return m;
-  }
-  __device__ __forceinline__ uint2 codes(float inv) const {
-    return make_uint2(fp8_pack4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv), fp8_pack4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
-  }
-};
-// the largest over the sixteen lanes of a block, for IT blocks: bf16 magnitudes of two blocks share a register on the way
-template <int IT> __device__ __forceinline__ void half_warp_max(uint32_t (&m)[IT], __nv_bfloat16) {
-  constexpr int W = (IT + 1) / 2;
-  uint32_t w[W];
-#pragma unroll
-  for (int t = 0; t < W; ++t) w[t] = m[2 * t] | (2 * t + 1 < IT ? m[2 * t + 1 < IT ? 2 * t + 1 : 0] << 16 : 0u);
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1)
-#pragma unroll
-    for (int t = 0; t < W; ++t) w[t] = __vmaxu2(w[t], __shfl_xor_sync(0xffffffffu, w[t], o));
-#pragma unroll
-  for (int t = 0; t < IT; ++t) m[t] = t & 1 ? w[t / 2] & 0xffff0000u : w[t / 2] << 16;
-}
-template <int IT> __device__ __forceinline__ void half_warp_max(uint32_t (&m)[IT], float) {
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1)
-#pragma unroll
-    for (int t = 0; t < IT; ++t) m[t] = max(m[t], __shfl_xor_sync(0xffffffffu, m[t], o));
-}
-
 // VEC: rows start on 16 bytes
 template <typename T, int IT, bool VEC>
 __global__ void __launch_bounds__(256, VEC && sizeof(T) == 2 ? 8 : 4) fp8_rows_kernel(const Fp8RowsParams p) {

@@ -7,6 +7,8 @@
 //   warp 0      TMA boxes of weights and of rows into a ring of NST stages, and asynchronous copies of their scales into a ring of their own
 //   warp 1      tcgen05.mma from one thread into a ring of ACC accumulators
 //   warps 2-5   32 weight rows each: scale and add, epilogue
+//   warps 6, 7  (ROUND) bf16 rows to codes: for up to 16 rows every CTA rounds the blocks that it needs itself, once, into shared memory, so that a decode step is
+//               one launch.  linear 1 x 6144 x 4096: see below
 // The work is the list of (group of rows, 128 weight rows, block of K) laid end to end, of which every CTA takes an equal run.  A tile that is cut leaves fp32
 // partials (at most two per CTA); the warp that arrives last adds them in the order of the CTAs, so results do not depend on timing.
 // Every mbarrier wait is bounded.
@@ -22,19 +24,22 @@ constexpr int FS_W = FS_TILE * FP8_BLOCK;
 constexpr int FS_MAX_E = 1024;
 constexpr int FS_MAX_GRID = CUT_TICKETS / 4;
 
-template <int NT> struct Fp8StreamShape {
+template <int NT, bool ROUND> struct Fp8StreamShape {
+  static_assert(!ROUND || NT == 16, "rows that are rounded here");
   static constexpr int X = NT * FP8_BLOCK;
-  static constexpr int STAGE = FS_W + X;
+  static constexpr int STAGE = FS_W + (ROUND ? 0 : X);
+  static constexpr int BLOCKS = ROUND ? 26 : 0;        // blocks of rounded rows that a CTA keeps
   static constexpr int CTAS = NT <= 64 ? 2 : 1;        // per SM; 128 sums a thread want all the registers
-  static constexpr int NST = (CTAS == 2 ? 104 : 200) * 1024 / STAGE;
-  static constexpr int SMEM = NST * STAGE + 1024;
+  static constexpr int OUT = 4 * 8 * 32 * 4;           // eight columns of a warp's sums, on their way out
+  static constexpr int NST = ((CTAS == 2 ? 104 : 200) * 1024 - BLOCKS * X - OUT) / STAGE;
+  static constexpr int SMEM = NST * STAGE + BLOCKS * X + OUT + 1024;
   static constexpr int ACC = NT <= 64 ? 4 : 2;
   static constexpr int TMEM = NT * ACC;                // 64, 128, 256, 256 columns: two CTAs have 512
-  // Scales of a unit: NT of the rows, 8 of the weights.  A slot is free again when the products of the unit NST before are done, since they waited for the sums
+  // Scales of a unit: 8 of the weights, NT of the rows.  A slot is free again when the products of the unit NST before are done, since they waited for the sums
   // of the unit ACC before them.
-  static constexpr int RING = NST + ACC, SC = NT + 8;
+  static constexpr int RING = NST + ACC, SC = 8 + (ROUND ? 0 : NT);
+  static constexpr int THREADS = ROUND ? 256 : 192;
 };
-constexpr int FS_THREADS = 192;
 
 // A run of `per` units for every CTA; shorter runs would cost more in partial sums than they gain.
 __host__ __device__ inline int fp8_run(int total, int grid) {
@@ -42,25 +47,27 @@ __host__ __device__ inline int fp8_run(int total, int grid) {
   return per < 2 ? 2 : per;
 }
 
-template <int NT>
-__global__ void __launch_bounds__(FS_THREADS, Fp8StreamShape<NT>::CTAS)
+template <int NT, bool ROUND>
+__global__ void __launch_bounds__(Fp8StreamShape<NT, ROUND>::THREADS, Fp8StreamShape<NT, ROUND>::CTAS)
 fp8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const Fp8Params p) {
-  using S = Fp8StreamShape<NT>;
-  constexpr int NST = S::NST, ACC = S::ACC;
+  using S = Fp8StreamShape<NT, ROUND>;
+  constexpr int NST = S::NST, ACC = S::ACC, FS_THREADS = S::THREADS;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t s_bar[2 * NST + 2 * ACC];
+  __shared__ __align__(8) uint64_t s_bar[2 * NST + 2 * ACC + S::BLOCKS];
   __shared__ __align__(16) float s_scale[S::RING][S::SC];
+  __shared__ __align__(16) float s_rows[ROUND ? S::BLOCKS : 1][NT];
   __shared__ uint16_t s_pre[FS_MAX_E + 1];
   __shared__ int s_sum[FS_THREADS / 32];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const uint32_t bar_full = smem_u32(s_bar), bar_empty = bar_full + 8 * NST, bar_tfull = bar_empty + 8 * NST, bar_tempty = bar_tfull + 8 * ACC;
+  const uint32_t bar_full = smem_u32(s_bar), bar_empty = bar_full + 8 * NST, bar_tfull = bar_empty + 8 * NST, bar_tempty = bar_tfull + 8 * ACC, bar_x = bar_tempty + 8 * ACC;
   volatile int* abort_flag = &s_abort;
   if (tid == 0) {
     for (int s = 0; s < NST; ++s) { mbar_init(bar_full + 8 * s, 1 + 32); mbar_init(bar_empty + 8 * s, 1); }      // (the boxes, and every lane's copies)
     for (int a = 0; a < ACC; ++a) { mbar_init(bar_tfull + 8 * a, 2); mbar_init(bar_tempty + 8 * a, 4); }
+    for (int b = 0; b < S::BLOCKS; ++b) mbar_init(bar_x + 8 * b, p.slot ? 1 : p.M);
     s_abort = 0;
     fence_mbar_init();
   }
@@ -136,13 +143,14 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
       if (any) group(r);
     }
   };
+  const int blocks = p.slot ? per : min(p.kb, per);    // (ROUND) that a run needs; a dense layer's come again in every tile
   const bool early = !banked && !p.slot;               // which weights are read does not depend on the launch before
   const int sw_groups = (p.N + FP8_ROWS - 1) / FP8_ROWS;
 
   if (warp == 0) {
     // ------------------------------------------------ TMA, scales
     if (my0 < my1) {
-      if (lane == 0) { prefetch_tmap(&tm_w); prefetch_tmap(&tm_x); }
+      if (lane == 0) { prefetch_tmap(&tm_w); if (!ROUND) prefetch_tmap(&tm_x); }
       if (!early && !banked) pdl_wait();
       auto load_w = [&](int s, const Place& at) {
         mbar_expect_tx(bar_full + 8 * s, S::STAGE);
@@ -166,15 +174,16 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
           if (!mbar_wait(bar_empty + 8 * s, ph, p.status, ERR_MBAR_TIMEOUT_PRODUCER, abort_flag)) break;
           if (lane == 0) load_w(s, at);
         }
-        const int row = p.slot ? at.row0 / p.x_div : at.row0;
-        if (lane == 0) tma_load_2d(base + s * S::STAGE + FS_W, &tm_x, bar_full + 8 * s, at.k * (FP8_BLOCK / 2), row);
         const uint32_t to = smem_u32(s_scale[r]) + 4 * lane;
-        const float* from = p.sx + (size_t)at.k * p.x_rows + row + lane;
+        if (lane < 8) copy4(to, p.sw + ((size_t)min(max(at.e, 0), p.E - 1) * sw_groups + min(at.nt * (FS_TILE / FP8_ROWS) + lane, sw_groups - 1)) * p.kb + at.k);
+        if constexpr (!ROUND) {
+          const int row = p.slot ? at.row0 / p.x_div : at.row0;
+          if (lane == 0) tma_load_2d(base + s * S::STAGE + FS_W, &tm_x, bar_full + 8 * s, at.k * (FP8_BLOCK / 2), row);
+          const float* from = p.sx + (size_t)at.k * p.x_rows + row + lane;
 #pragma unroll
-        for (int c = 0; c < NT; c += 32)
-          if (c + lane < at.rows) copy4(to + 4 * c, from + c);
-        if (lane < 8)
-          copy4(to + 4 * NT, p.sw + ((size_t)min(max(at.e, 0), p.E - 1) * sw_groups + min(at.nt * (FS_TILE / FP8_ROWS) + lane, sw_groups - 1)) * p.kb + at.k);
+          for (int c = 0; c < NT; c += 32)
+            if (c + lane < at.rows) copy4(to + 32 + 4 * c, from + c);
+        }
         arrive_copies(bar_full + 8 * s);
         if (++s == NST) { s = 0; ph ^= 1; }
         if (++r == S::RING) r = 0;
@@ -197,12 +206,15 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
       const uint32_t leader = elect_one();
       constexpr uint32_t idesc = umma_idesc_e4m3(FS_TILE, NT);
       uint32_t s = 0, ph = 0, a = 0, aph = 1;
+      int x = 0;                                       // block of rounded rows
       for (int pos = my0; pos < my1; ++pos) {
         if (!mbar_wait(bar_tempty + 8 * a, aph, p.status, ERR_MBAR_TIMEOUT_MMA, abort_flag)) break;
         if (!mbar_wait(bar_full + 8 * s, ph, p.status, ERR_MBAR_TIMEOUT_MMA, abort_flag)) break;
+        if (ROUND && !mbar_wait(bar_x + 8 * x, 0, p.status, ERR_MBAR_TIMEOUT_DEQUANT, abort_flag)) break;
         __syncwarp();                                  // (no lane may miss a phase)
         tc_fence_after();
-        const uint64_t dw = umma_desc_k_sw128(base + s * S::STAGE), dx = umma_desc_k_sw128(base + s * S::STAGE + FS_W);
+        const uint64_t dw = umma_desc_k_sw128(base + s * S::STAGE);
+        const uint64_t dx = umma_desc_k_sw128(ROUND ? base + NST * S::STAGE + x * S::X : base + s * S::STAGE + FS_W);
 #pragma unroll
         for (int kk = 0; kk < FP8_BLOCK / 32; ++kk) umma_e4m3(leader, tmem + a * NT, dw + 2 * kk, dx + 2 * kk, idesc, kk != 0);
         umma_commit_if(leader, bar_empty + 8 * s);
@@ -210,9 +222,10 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
         umma_commit_if(leader, bar_tfull + 8 * a);
         if (++s == NST) { s = 0; ph ^= 1; }
         if (++a == ACC) { a = 0; aph ^= 1; }
+        if (ROUND && ++x == blocks) x = 0;
       }
     }
-  } else {
+  } else if (warp < 6) {
     // ------------------------------------------------ scales, sums, epilogue: a thread owns weight row `n`
     const int q = warp & 3;
     asm volatile("bar.sync 1, 160;" ::: "memory");
@@ -220,6 +233,7 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
     const uint32_t tmem = s_tmem;
     if (!banked) pdl_wait();
     uint32_t a = 0, aph = 0, ring = 0;
+    int x = 0;
     bool ok = true;
     Place at;
     if (my0 < my1) at = place(my0);
@@ -233,8 +247,8 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
       for (int i = 0; i < n_units; ++i) {
         if (!(ok = mbar_wait(bar_tfull + 8 * a, aph, p.status, ERR_MBAR_TIMEOUT_EPILOGUE, abort_flag))) break;
         tc_fence_after();
-        const float4* sx = reinterpret_cast<const float4*>(s_scale[ring]);
-        const float sw = s_scale[ring][NT + 2 * q + (lane >> 4)];
+        const float4* sx = reinterpret_cast<const float4*>(ROUND ? s_rows[x] : s_scale[ring] + 8);
+        const float sw = s_scale[ring][2 * q + (lane >> 4)];
         constexpr int C = NT < 32 ? NT : 32;
 #pragma unroll
         for (int c0 = 0; c0 < NT; c0 += C) {
@@ -254,6 +268,7 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_tempty + 8 * a);
         if (++ring == S::RING) ring = 0;
+        if (ROUND && ++x == blocks) x = 0;
         if (++a == ACC) { a = 0; aph ^= 1; }
       }
       if (!ok) break;
@@ -281,30 +296,59 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
           __threadfence();
 #pragma unroll
           for (int j = 0; j < NT / 2; ++j) acc[j] = make_float2(0.f, 0.f);
-          for (int c = c0; c <= c1; ++c) {
-            const float4* src = slab(c);
+          // four parts of sixteen columns at a time are under way; they are added in order
+          constexpr int J = NT / 4 < 4 ? NT / 4 : 4;
 #pragma unroll
-            for (int j = 0; j < NT / 4; ++j)
-              if (4 * j < at.rows) {
-                const float4 v = __ldcg(src + j * 32);
-                acc[2 * j].x += v.x; acc[2 * j].y += v.y; acc[2 * j + 1].x += v.z; acc[2 * j + 1].y += v.w;
+          for (int j0 = 0; j0 < NT / 4; j0 += J) {
+            if (4 * j0 < at.rows) {
+              for (int c = c0; c <= c1; c += 4) {
+                float4 v[4][J];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                  for (int j = 0; j < J; ++j)
+                    v[i][j] = c + i <= c1 && 4 * (j0 + j) < at.rows ? __ldcg(slab(c + i) + (j0 + j) * 32) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                  for (int j = 0; j < J; ++j) {
+                    float2& u = acc[2 * (j0 + j)];
+                    float2& w = acc[2 * (j0 + j) + 1];
+                    u.x += v[i][j].x; u.y += v[i][j].y; w.x += v[i][j].z; w.y += v[i][j].w;
+                  }
               }
+            }
           }
         }
       }
       if (mine_to_finish) {
-        // ---- epilogue: gate rows are lanes 0-15, their up rows lanes 16-31
+        // ---- epilogue: gate rows are lanes 0-15, their up rows lanes 16-31.  Eight columns at a time go through shared memory, so that the code that follows exists
+        // once: unrolled over the columns it is fetched from L2 instruction by instruction (20 rows: 14000 cycles)
         const bool gated = act_gated(p.act), owned = at.e >= 0 && at.e < p.E;
         const float bias = p.bias && n < p.N ? p.bias[(size_t)e * p.N + n] : 0.f;
         const int on = gated ? p.N >> 1 : p.N, o = gated ? at.nt * (FS_TILE / 2) + q * 16 + (lane & 15) : n;
         const bool write = o < on && (!gated || lane < 16);
+        float* const col = reinterpret_cast<float*>(smem_raw + (base - smem_u32(smem_raw)) + NST * S::STAGE + S::BLOCKS * S::X) + q * 256 + lane;
+#pragma unroll 1
+        for (int j0 = 0; j0 < at.rows; j0 += 8) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
-          if (j < at.rows) {
-            float v = (j & 1 ? acc[j / 2].y : acc[j / 2].x) + bias;
-            if (gated) v = glu_apply(p.act, v, __shfl_down_sync(0xffffffffu, v, 16), p.act_alpha, p.act_limit);
-            else if (p.act) v = act_unary<false>(p.act, v, p.act_alpha, p.act_limit);
-            const int row = at.row0 + j;
+          for (int g = 0; g < NT / 8; ++g)
+            if (8 * g == j0) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) { col[64 * j] = acc[4 * g + j].x; col[64 * j + 32] = acc[4 * g + j].y; }
+            }
+          const int live = min(8, at.rows - j0);
+#pragma unroll 2
+          for (int j = 0; j < live; ++j) {
+            float v = col[32 * j] + bias;                // (a lane reads what it has written)
+            const int row = at.row0 + j0 + j;
+            if (gated) {
+              float pair[2] = {v, __shfl_down_sync(0xffffffffu, v, 16)};
+              glu_run<1>(p.act, pair, p.act_alpha, p.act_limit);
+              v = pair[0];
+            } else if (p.act) {
+              v = act_unary<false>(p.act, v, p.act_alpha, p.act_limit);
+            }
             if (p.row_scale) v *= p.row_scale[row];
             if (!owned) v = 0.f;
             if (write) {
@@ -312,9 +356,54 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
               else ((__nv_bfloat16*)p.C)[row * p.ldc + o] = __float2bfloat16(v);
             }
           }
+        }
       }
       pos += n_units;
       next_tile(at, pos < my1);
+    }
+  } else if constexpr (ROUND) {
+    // ------------------------------------------------ rows to codes: half a warp a block of a row, four pairs of blocks at a time; the blocks in the order of their use
+    pdl_wait();
+    const int half = lane >> 4, sub = lane & 15, rows = p.slot ? 1 : p.M, need = min(blocks, my1 - my0), items = (need + 1) / 2 * rows;
+    uint8_t* const xs = smem_raw + (base - smem_u32(smem_raw)) + NST * S::STAGE;
+    for (int i0 = (warp - 6) * 4; i0 < items; i0 += 8) {
+      Row8<__nv_bfloat16> v[4];
+      int b[4], r[4];
+      uint32_t m[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int i = min(i0 + t, items - 1), pair = i / rows;
+        r[t] = i - pair * rows;
+        b[t] = 2 * pair + half;
+        const int unit = my0 + min(b[t], need - 1), tile = unit / p.kb, at = (unit - tile * p.kb) * FP8_BLOCK + 8 * sub;
+        const __nv_bfloat16* row = p.xb + (long long)(p.slot ? tile / n_tiles / p.x_div : r[t]) * p.ldx;
+        v[t].load(row + (at + 8 <= p.K ? at : 0));             // (K is 8 at least)
+        if (at + 8 > p.K) {
+          v[t].zero();
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (at + j < p.K) v[t].put(j, row[at + j]);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) m[t] = v[t].top();
+      half_warp_max<4>(m, __nv_bfloat16());
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        if (i0 + t >= items || b[t] >= need) continue;
+        float inv;
+        const float sc = fp8_scale(__uint_as_float(m[t]), &inv);
+        const uint2 w = m[t] < 0x7f800000u ? v[t].codes(inv) : make_uint2(0, 0);
+        *reinterpret_cast<uint2*>(xs + b[t] * S::X + sw128_offset(r[t], sub >> 1) + (sub & 1) * 8) = w;
+        if (sub == 0) s_rows[b[t]][r[t]] = sc;
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (sub == 0) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          if (i0 + t < items && b[t] < need) mbar_arrive(bar_x + 8 * b[t]);
+      }
     }
   }
   if (*abort_flag)                                         // a wait ran out: copies still in flight land before shared memory is released
@@ -324,36 +413,54 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
   if (warp == 1) { tc_fence_after(); tmem_dealloc(s_tmem, S::TMEM); }
 }
 
-template <int NT> static int launch_stream(const CUtensorMap& tw, const CUtensorMap& tx, const Fp8Params& p, cudaStream_t st) {
-  using S = Fp8StreamShape<NT>;
-  auto kern = fp8_stream_kernel<NT>;
+static int stream_grid(int ctas) { return ctas * sm_count() < FS_MAX_GRID ? ctas * sm_count() : FS_MAX_GRID; }
+
+template <int NT, bool ROUND> static int launch_stream(const CUtensorMap& tw, const CUtensorMap& tx, const Fp8Params& p, cudaStream_t st) {
+  using S = Fp8StreamShape<NT, ROUND>;
+  auto kern = fp8_stream_kernel<NT, ROUND>;
   static DeviceOnce configured;
   if (configured.pending()) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
     if (e != cudaSuccess) return (int)e;
     configured.mark();
   }
-  const int grid = S::CTAS * sm_count() < FS_MAX_GRID ? S::CTAS * sm_count() : FS_MAX_GRID;
-  launch_pdl(kern, dim3(grid), dim3(FS_THREADS), S::SMEM, st, tw, tx, p);
+  launch_pdl(kern, dim3(stream_grid(S::CTAS)), dim3(S::THREADS), S::SMEM, st, tw, tx, p);
   return (int)cudaGetLastError();
 }
 
+// Whether the streaming kernel rounds a launch's rows itself: up to 16, of which a CTA's share of the blocks fits its shared memory.
+bool fp8_stream_rounds(const Fp8Call& c) {
+  using S = Fp8StreamShape<16, true>;
+  if (!c.xb || c.nt != 16 || c.counts || c.K < 8 || c.ldx % 8 || ((uintptr_t)c.xb & 15)) return false;
+  const int kb = (c.K + FP8_BLOCK - 1) / FP8_BLOCK, n_tiles = (c.N + FS_TILE - 1) / FS_TILE;
+  const long long total = (c.slot ? (long long)c.M : 1) * n_tiles * kb;
+  if (total >= 1ll << 30) return false;
+  const int per = fp8_run((int)total, stream_grid(S::CTAS));
+  return (c.slot ? per : per < kb ? per : kb) <= S::BLOCKS;
+}
+
 // Dense (M <= nt), experts (counts / seg) or slots (slot), in groups of nt = 16, 32, 64 or 128 rows.
-int fp8_stream_launch(const Fp8Call& c, cudaStream_t st) {
-  const Fp8Params p = fp8_params(c);
+int fp8_stream_launch(const Fp8Call& c, bool round, cudaStream_t st) {
+  Fp8Params p = fp8_params(c);
   const int nt = c.nt;
   const long long groups = c.slot ? c.M : c.counts ? (long long)c.M / nt + (c.E < c.M ? c.E : c.M) + 1 : 1;
   if (c.E > FS_MAX_E || groups >= 65536 || groups * ((p.N + FS_TILE - 1) / FS_TILE) * p.kb >= 1ll << 30 || (!c.slot && !c.counts && c.M > nt)) return -106;      // (units are counted in 32 bits)
   if (((uintptr_t)c.codes | (uintptr_t)c.w | (uintptr_t)c.scratch) & 15) return -114;
   CUtensorMap tw, tx;
   int r = fp8_tmap(&tw, c.w, p.kb, p.N, c.E, FS_TILE);
-  if (!r) r = fp8_tmap(&tx, c.codes, p.kb, c.rows, 0, nt);
+  if (r) return r;
+  if (round) {
+    p.xb = (const __nv_bfloat16*)c.xb;
+    p.ldx = c.ldx;
+    return launch_stream<16, true>(tw, tw, p, st);
+  }
+  r = fp8_tmap(&tx, c.codes, p.kb, c.rows, 0, nt);
   if (r) return r;
   switch (nt) {
-    case 16: return launch_stream<16>(tw, tx, p, st);
-    case 32: return launch_stream<32>(tw, tx, p, st);
-    case 64: return launch_stream<64>(tw, tx, p, st);
-    case 128: return launch_stream<128>(tw, tx, p, st);
+    case 16: return launch_stream<16, false>(tw, tx, p, st);
+    case 32: return launch_stream<32, false>(tw, tx, p, st);
+    case 64: return launch_stream<64, false>(tw, tx, p, st);
+    case 128: return launch_stream<128, false>(tw, tx, p, st);
     default: return -106;
   }
 }
