@@ -340,6 +340,7 @@ using namespace mx;
 MX_HOST_API int mx_fp8_call_bytes() { return (int)sizeof(Fp8Call); }
 
 // A product (see Fp8Call): rows that are bf16 still are rounded, then the streaming kernel (nt) or the tiled one (bn) runs.
+// -130: bf16 rows that have to be rounded first, and no room for codes; nothing was launched.
 MX_HOST_API int mx_fp8_product(const Fp8Call* call, cudaStream_t st) {
   const Fp8Call& c = *call;
   if (c.M <= 0 || c.N <= 0) return 0;
@@ -347,6 +348,7 @@ MX_HOST_API int mx_fp8_product(const Fp8Call* call, cudaStream_t st) {
   if (act_gated(c.act) && c.N % 32) return -104;
   const bool round = fp8_stream_rounds(c);
   if (c.xb && !round) {
+    if (!c.codes) return -130;
     const int r = fp8_rows_launch(c.xb, 0, c.ldx, c.index, c.xb_rows, c.rows, c.K, c.codes, c.scale, st);
     if (r) return r;
   }

@@ -31,8 +31,9 @@ template <int NT, bool ROUND> struct Fp8StreamShape {
   static constexpr int BLOCKS = ROUND ? 26 : 0;        // blocks of rounded rows that a CTA keeps
   static constexpr int CTAS = NT <= 64 ? 2 : 1;        // per SM; 128 sums a thread want all the registers
   static constexpr int OUT = 4 * 8 * 32 * 4;           // eight columns of a warp's sums, on their way out
-  static constexpr int NST = ((CTAS == 2 ? 104 : 200) * 1024 - BLOCKS * X - OUT) / STAGE;
-  static constexpr int SMEM = NST * STAGE + BLOCKS * X + OUT + 1024;
+  static constexpr int ROOM = (CTAS == 2 ? 104 : 200) * 1024 - OUT;      // for stages and rounded rows
+  static constexpr int SMEM = ROOM + OUT + 1024;
+  static constexpr int NST = ROUND ? 5 : ROOM / STAGE; // at most; fewer where a run needs more rounded rows
   static constexpr int ACC = NT <= 64 ? 4 : 2;
   static constexpr int TMEM = NT * ACC;                // 64, 128, 256, 256 columns: two CTAs have 512
   // Scales of a unit: 8 of the weights, NT of the rows.  A slot is free again when the products of the unit NST before are done, since they waited for the sums
@@ -51,9 +52,9 @@ template <int NT, bool ROUND>
 __global__ void __launch_bounds__(Fp8StreamShape<NT, ROUND>::THREADS, Fp8StreamShape<NT, ROUND>::CTAS)
 fp8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const Fp8Params p) {
   using S = Fp8StreamShape<NT, ROUND>;
-  constexpr int NST = S::NST, ACC = S::ACC, FS_THREADS = S::THREADS;
+  constexpr int MST = S::NST, ACC = S::ACC, FS_THREADS = S::THREADS;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t s_bar[2 * NST + 2 * ACC + S::BLOCKS];
+  __shared__ __align__(8) uint64_t s_bar[2 * MST + 2 * ACC + S::BLOCKS];
   __shared__ __align__(16) float s_scale[S::RING][S::SC];
   __shared__ __align__(16) float s_rows[ROUND ? S::BLOCKS : 1][NT];
   __shared__ uint16_t s_pre[FS_MAX_E + 1];
@@ -62,10 +63,10 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
   __shared__ int s_abort;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const uint32_t bar_full = smem_u32(s_bar), bar_empty = bar_full + 8 * NST, bar_tfull = bar_empty + 8 * NST, bar_tempty = bar_tfull + 8 * ACC, bar_x = bar_tempty + 8 * ACC;
+  const uint32_t bar_full = smem_u32(s_bar), bar_empty = bar_full + 8 * MST, bar_tfull = bar_empty + 8 * MST, bar_tempty = bar_tfull + 8 * ACC, bar_x = bar_tempty + 8 * ACC;
   volatile int* abort_flag = &s_abort;
   if (tid == 0) {
-    for (int s = 0; s < NST; ++s) { mbar_init(bar_full + 8 * s, 1 + 32); mbar_init(bar_empty + 8 * s, 1); }      // (the boxes, and every lane's copies)
+    for (int s = 0; s < MST; ++s) { mbar_init(bar_full + 8 * s, 1 + 32); mbar_init(bar_empty + 8 * s, 1); }      // (the boxes, and every lane's copies)
     for (int a = 0; a < ACC; ++a) { mbar_init(bar_tfull + 8 * a, 2); mbar_init(bar_tempty + 8 * a, 4); }
     for (int b = 0; b < S::BLOCKS; ++b) mbar_init(bar_x + 8 * b, p.slot ? 1 : p.M);
     s_abort = 0;
@@ -144,6 +145,8 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
     }
   };
   const int blocks = p.slot ? per : min(p.kb, per);    // (ROUND) that a run needs; a dense layer's come again in every tile
+  const int NST = ROUND ? min(MST, (S::ROOM - blocks * S::X) / S::STAGE) : MST;
+  const uint32_t rows_at = base + NST * S::STAGE, out_at = base + S::ROOM;
   const bool early = !banked && !p.slot;               // which weights are read does not depend on the launch before
   const int sw_groups = (p.N + FP8_ROWS - 1) / FP8_ROWS;
 
@@ -214,7 +217,7 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
         __syncwarp();                                  // (no lane may miss a phase)
         tc_fence_after();
         const uint64_t dw = umma_desc_k_sw128(base + s * S::STAGE);
-        const uint64_t dx = umma_desc_k_sw128(ROUND ? base + NST * S::STAGE + x * S::X : base + s * S::STAGE + FS_W);
+        const uint64_t dx = umma_desc_k_sw128(ROUND ? rows_at + x * S::X : base + s * S::STAGE + FS_W);
 #pragma unroll
         for (int kk = 0; kk < FP8_BLOCK / 32; ++kk) umma_e4m3(leader, tmem + a * NT, dw + 2 * kk, dx + 2 * kk, idesc, kk != 0);
         umma_commit_if(leader, bar_empty + 8 * s);
@@ -328,7 +331,7 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
         const float bias = p.bias && n < p.N ? p.bias[(size_t)e * p.N + n] : 0.f;
         const int on = gated ? p.N >> 1 : p.N, o = gated ? at.nt * (FS_TILE / 2) + q * 16 + (lane & 15) : n;
         const bool write = o < on && (!gated || lane < 16);
-        float* const col = reinterpret_cast<float*>(smem_raw + (base - smem_u32(smem_raw)) + NST * S::STAGE + S::BLOCKS * S::X) + q * 256 + lane;
+        float* const col = reinterpret_cast<float*>(smem_raw + (out_at - smem_u32(smem_raw))) + q * 256 + lane;
 #pragma unroll 1
         for (int j0 = 0; j0 < at.rows; j0 += 8) {
 #pragma unroll
@@ -365,7 +368,7 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
     // ------------------------------------------------ rows to codes: half a warp a block of a row, four pairs of blocks at a time; the blocks in the order of their use
     pdl_wait();
     const int half = lane >> 4, sub = lane & 15, rows = p.slot ? 1 : p.M, need = min(blocks, my1 - my0), items = (need + 1) / 2 * rows;
-    uint8_t* const xs = smem_raw + (base - smem_u32(smem_raw)) + NST * S::STAGE;
+    uint8_t* const xs = smem_raw + (rows_at - smem_u32(smem_raw));
     for (int i0 = (warp - 6) * 4; i0 < items; i0 += 8) {
       Row8<__nv_bfloat16> v[4];
       int b[4], r[4];

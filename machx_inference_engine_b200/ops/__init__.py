@@ -42,6 +42,18 @@ def backend() -> str:
     return _BACKEND[0]
 
 
+_cuda = None
+
+
+def _kernels():
+    """:mod:`ops.cuda`, imported when the first op runs on a GPU."""
+    global _cuda
+    if _cuda is None:
+        from . import cuda
+        _cuda = cuda
+    return _cuda
+
+
 def _first_tensor(args, kwargs):
     if args and isinstance(args[0], torch.Tensor):
         return args[0]
@@ -63,7 +75,7 @@ def _make(name):
     @functools.wraps(ref_fn)
     def op(*args, **kwargs):
         if _BACKEND[0] == "auto" and _first_tensor(args, kwargs).is_cuda:
-            from . import cuda
+            cuda = _kernels()
             fn = getattr(cuda, name)
             if _prof.enabled:
                 tag = name

@@ -67,7 +67,8 @@ _capture_tickets: dict = {}         # (device, stream, capture) -> the same
 
 
 def _tickets(device):
-    """(array, its pointer, the stream) for a launch on the current stream of ``device``; the caller keeps the tuple until it has launched."""
+    """(array, its pointer, the stream, what else launches of this stream keep -- None under capture) for a launch on the current stream of ``device``; the caller keeps
+    the tuple until it has launched."""
     s = torch._C._cuda_getCurrentRawStream(device.index)
     key = (device.index, s) if s != 2 else (device.index, s, threading.get_ident())      # (handle 2: every thread's own default stream)
     capturing = torch.cuda.is_current_stream_capturing()
@@ -87,7 +88,7 @@ def _tickets(device):
         t = table.get(key)
         if t is None:
             array = torch.zeros(_lib.cuda().mx_cut_tickets(), dtype=torch.int32, device=device)
-            t = table[key] = (array, _p(array), _vp(s))
+            t = table[key] = (array, _p(array), _vp(s), None if capturing else [])
             if len(_stream_tickets) > STREAM_TICKETS_MAX:
                 del _stream_tickets[next(iter(_stream_tickets))]
         return t
@@ -882,6 +883,8 @@ def expert_gemv(x, w: QuantWeight, slot_expert, x_div=1, bias=None, act=ACT_NONE
 # ------------------------------------------------------------------ 8-bit floating point (see ops/fp8.py)
 FP8_STREAM_ROWS = (16, 32, 64, 128)      # rows of a group in the weight-streaming kernel
 _FP8_CALL = struct.Struct("<16q12i2f")   # csrc/cuda/fp8.cuh: Fp8Call
+_FP8_WANTS_ROOM = -130                   # and the answer to bf16 rows without room for rounded ones, where the kernel does not round them itself
+_FP8_SCRATCH: dict = {}                  # rows of a group -> bytes of partial sums
 _fp8_lib = None
 
 
@@ -911,8 +914,8 @@ def fp8_rows(x, index=None) -> FP8Rows:
             return fp8_rows(x, index)
     rows, K = x.shape if index is None else (index.numel(), x.shape[1])
     kb = -(-K // _fp8.FP8_BLOCK)
-    codes = torch.empty((rows, kb * _fp8.FP8_BLOCK), dtype=torch.float8_e4m3fn, device=dev)
-    scale = torch.empty((kb, rows), dtype=torch.float32, device=dev)
+    codes = x.new_empty((rows, kb * _fp8.FP8_BLOCK), dtype=torch.float8_e4m3fn)
+    scale = x.new_empty((kb, rows), dtype=torch.float32)
     if rows:
         _check(_fp8_entry().mx_fp8_rows(x.data_ptr(), x.dtype == torch.float32, x.stride(0), _ptr(index), x.shape[0], rows, K, codes.data_ptr(), scale.data_ptr(),
                                         torch._C._cuda_getCurrentRawStream(dev.index)), "fp8_rows")
@@ -921,30 +924,40 @@ def fp8_rows(x, index=None) -> FP8Rows:
 
 
 def _fp8_call(x, w: QuantWeight, out, bias, row_scale, act, act_alpha, act_limit, nt=0, bn=0, counts=None, seg=None, slot=None, x_div=1, e_lo=0, index=None):
-    """One product on the current device: ``nt`` rows of a group (csrc/cuda/fp8_stream.cu) or ``bn`` columns of a tile (csrc/cuda/fp8_gemm.cu).  bf16 rows are rounded into a
-    scratch buffer first, by the same call.  The scratch is an ordinary allocation: stream-ordered, of the graph's own pool under capture."""
+    """One product on the current device: ``nt`` rows of a group (csrc/cuda/fp8_stream.cu) or ``bn`` columns of a tile (csrc/cuda/fp8_gemm.cu).  bf16 rows that the kernel does
+    not round itself are rounded into a scratch buffer first, by the same call: an ordinary allocation, stream-ordered and of the graph's own pool under capture.  Partial sums
+    go to memory that a stream's launches share, since they follow one another, and under capture to an allocation as well."""
     lib = _fp8_entry()
     dev = out.device
-    K, kb = w.K, -(-w.K // _fp8.FP8_BLOCK)
-    work = lib.mx_fp8_stream_scratch(nt) if nt else 0
+    part = counters = 0
+    if nt:
+        tickets = _tickets(dev)
+        counters, kept = tickets[0].data_ptr(), tickets[3]
+        work = _FP8_SCRATCH.get(nt) or _FP8_SCRATCH.setdefault(nt, lib.mx_fp8_stream_scratch(nt))
+        if kept is None:
+            scratch = torch.empty(work, dtype=torch.uint8, device=dev)
+        else:
+            if not kept or kept[0].numel() < work:
+                kept[:] = [torch.empty(work, dtype=torch.uint8, device=dev)]
+            scratch = kept[0]
+        part = scratch.data_ptr()
     if isinstance(x, FP8Rows):
-        rows = x.codes.shape[0]
-        xb, ldx, xb_rows = 0, 0, 0
-        scratch = torch.empty(work, dtype=torch.uint8, device=dev) if work else None
-        at = _ptr(scratch)
-        codes, scale = x.codes.data_ptr(), x.scale.data_ptr()
+        rows, xb, ldx, xb_rows, codes, scale = x.codes.shape[0], 0, 0, 0, x.codes.data_ptr(), x.scale.data_ptr()
     else:
-        xb, ldx, xb_rows = x.data_ptr(), x.stride(0), x.shape[0]
+        xb, ldx, xb_rows, codes, scale = x.data_ptr(), x.stride(0), x.shape[0], 0, 0
         rows = xb_rows if index is None else index.numel()
-        n = rows * kb
-        scratch = torch.empty(work + n * (_fp8.FP8_BLOCK + 4), dtype=torch.uint8, device=dev)
-        at = scratch.data_ptr()
-        codes, scale = at + work, at + work + n * _fp8.FP8_BLOCK
-    tickets = _tickets(dev) if nt else None
-    call = _FP8_CALL.pack(xb, ldx, _ptr(index), codes, scale, w.p0.data_ptr(), w.p1.data_ptr(), out.data_ptr(), out.stride(0), _ptr(bias), _ptr(row_scale), _ptr(counts), _ptr(seg),
-                          _ptr(slot), at, tickets[0].data_ptr() if nt else 0, xb_rows, rows, out.shape[0], w.N, K, w.E, out.dtype == torch.float32, act, x_div, e_lo, nt, bn,
-                          act_alpha, act_limit)
-    _check(lib.mx_fp8_product(call, torch._C._cuda_getCurrentRawStream(dev.index)), "fp8 product")
+    rc = _FP8_WANTS_ROOM if xb and (nt != 16 or counts is not None) else None
+    while rc is None or rc == _FP8_WANTS_ROOM:
+        if rc is not None:                   # (no launch has been made)
+            n = rows * -(-w.K // _fp8.FP8_BLOCK)
+            rounded = torch.empty(n * (_fp8.FP8_BLOCK + 4), dtype=torch.uint8, device=dev)
+            codes = rounded.data_ptr()
+            scale = codes + n * _fp8.FP8_BLOCK
+        call = _FP8_CALL.pack(xb, ldx, _ptr(index), codes, scale, w.p0.data_ptr(), w.p1.data_ptr(), out.data_ptr(), out.stride(0), _ptr(bias), _ptr(row_scale), _ptr(counts),
+                              _ptr(seg), _ptr(slot), part, counters, xb_rows, rows, out.shape[0], w.N, w.K, w.E, out.dtype == torch.float32, act, x_div, e_lo, nt, bn, act_alpha,
+                              act_limit)
+        rc = lib.mx_fp8_product(call, torch._C._cuda_getCurrentRawStream(dev.index))
+    _check(rc, "fp8 product")
     _count()
     return out
 
@@ -962,7 +975,7 @@ def _fp8_product(x, w: QuantWeight, shape, dtype, out, bias, row_scale, act, act
         with torch.cuda.device(dev):
             return _fp8_product(x, w, shape, dtype, out, bias, row_scale, act, act_alpha, act_limit, **kw)
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=dev)
+        out = w.p0.new_empty(shape, dtype=dtype)
     M = shape[0]
     if M == 0:
         return out

@@ -62,13 +62,16 @@ def check_product(x, w: QuantWeight, experts: bool, rows: int, bias, act_gated: 
         if x.codes.dtype != torch.float8_e4m3fn or x.codes.shape != (n, kb * FP8_BLOCK) or not x.codes.is_contiguous() or x.scale.dtype != torch.float32 \
                 or x.scale.shape != (kb, n) or not x.scale.is_contiguous() or x.scale.device != x.codes.device:
             raise ValueError(f"{what}: the rounded rows are not as ops.fp8_rows makes them")
+        K, dev = x.K, x.codes.get_device()
     else:
         if x.dtype != torch.bfloat16:
             raise ValueError(f"{what}: FP8 weights take bf16 rows or FP8Rows, not {x.dtype}")
-        check_rows(x)
-    if x.shape[1] != w.K:
-        raise ValueError(f"{what}: rows of {x.shape[1]} elements, a weight of {w.K}")
-    if x.device != w.device:
+        if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
+            raise ValueError(f"{what}: rows [rows, K] with a unit stride along K are wanted, not {list(x.shape)} with strides {x.stride()}")
+        K, dev = x.shape[1], x.get_device()
+    if K != w.K:
+        raise ValueError(f"{what}: rows of {K} elements, a weight of {w.K}")
+    if dev != w.p0.get_device():
         raise ValueError(f"{what}: rows on {x.device}, the weight on {w.device}")
     if act_gated and w.N % 32:
         raise ValueError(f"{what}: a gated activation takes runs of 16 gate and 16 up rows, not {w.N} rows")
