@@ -18,21 +18,21 @@
 
 namespace mx {
 
-constexpr int FG_BM = 128, FG_THREADS = 384, FG_MAX_E = 1024;
+constexpr int FG_BM = 128, FG_SUMS = 16, FG_THREADS = 128 + 32 * FG_SUMS, FG_MAX_E = 1024;      // FG_SUMS: warps that hold sums
 constexpr int FG_GROUP = 8;                                // m-tiles that are walked together: a wave shares bands of x and w in L2
 
-template <int BN> struct Fp8GemmShape {
+template <int BN, bool F32> struct Fp8GemmShape {
   static constexpr int A = FG_BM * FP8_BLOCK, B = BN * FP8_BLOCK, STAGE = A + B;
-  static constexpr int ROW = BN;                           // bytes of a staged row of a warp's outputs
-  static constexpr int OUT = 8 * 32 * ROW;
-  static constexpr int NST = BN == 256 ? 3 : 5;
+  static constexpr int ROW = BN == 128 && !F32 ? 64 : 128; // bytes of a staged row of a warp's outputs
+  static constexpr int OUT = FG_SUMS * 32 * ROW;
+  static constexpr int NST = BN == 256 ? 3 : F32 ? 4 : 5;
   static constexpr int ACC = 512 / BN;
   // A slot of scales is free again when the products of the block NST before are done, since they waited for the sums of the block ACC before them.
   static constexpr int RING = NST + ACC, SC = FG_BM + BN / FP8_ROWS;
   struct Small {                                           // what is not tiles, behind them
     alignas(16) float scale[RING][SC];
     uint64_t bar[2 * NST + 2 * ACC];
-    int sum[12];
+    int sum[FG_THREADS / 32];
     uint32_t tmem;
     int abort;
     uint16_t pre[FG_MAX_E + 1];                            // experts: m-tiles before expert i
@@ -45,7 +45,7 @@ template <int BN> struct Fp8GemmShape {
 template <int BN, int KIND, bool F32>
 __global__ void __launch_bounds__(FG_THREADS, 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, const Fp8Params p) {
-  using S = Fp8GemmShape<BN>;
+  using S = Fp8GemmShape<BN, F32>;
   constexpr int NST = S::NST, ACC = S::ACC;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   auto& small = *reinterpret_cast<typename S::Small*>(smem_raw + NST * S::STAGE + S::OUT);
@@ -64,7 +64,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
   volatile int* abort_flag = &s_abort;
   if (tid == 0) {
     for (int s = 0; s < NST; ++s) { mbar_init(bar_full + 8 * s, 1 + 64); mbar_init(bar_empty + 8 * s, 1); }
-    for (int a = 0; a < ACC; ++a) { mbar_init(bar_tfull + 8 * a, 2); mbar_init(bar_tempty + 8 * a, 8); }
+    for (int a = 0; a < ACC; ++a) { mbar_init(bar_tfull + 8 * a, 2); mbar_init(bar_tempty + 8 * a, FG_SUMS); }
     s_abort = 0;
     fence_mbar_init();
   }
@@ -132,7 +132,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
   };
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp == 0 && lane == 0) {
       prefetch_tmap(&tm_x); prefetch_tmap(&tm_w);
       uint32_t s = 0, ph = 1;
@@ -198,20 +198,24 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
     }
     __syncwarp();
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    constexpr int HC = BN / 2, G = HC / FP8_ROWS;          // columns of a thread, and the scales that they have
-    const int q = warp & 3, half = (warp - 4) >> 2;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    constexpr int HC = BN * 4 / FG_SUMS, G = HC / FP8_ROWS;          // columns of a thread, and the scales that they have
+    const int q = warp & 3, part = (warp - 4) >> 2;
     constexpr int ESZ = F32 ? 4 : 2, PIECE = KIND == 1 ? 8 : 16;        // outputs of 16 sums
     constexpr int ROW_BYTES = HC * PIECE / 16 * ESZ;       // of a thread's outputs
     constexpr int PASSES = ROW_BYTES > S::ROW ? ROW_BYTES / S::ROW : 1, RB = ROW_BYTES / PASSES, CPR = RB / 16;
+    static_assert(HC / 32 >= PASSES, "a pass has whole runs of 32 sums");
     uint8_t* const stage = smem_raw + NST * S::STAGE + (warp - 4) * (32 * S::ROW);
+    // chunks of a staged row are turned so that those of eight rows lie in different banks
+    static_assert(S::ROW == 128 || S::ROW == 64, "staged rows");
+    auto turn = [](int r) { return S::ROW == 128 ? r & 7 : r >> 1 & 3; };
     const int on = KIND == 1 ? p.N >> 1 : p.N;
     const bool wide = (((uintptr_t)p.C) & 15) == 0 && (p.ldc * ESZ) % 16 == 0;
     uint32_t a = 0, aph = 0, ring = 0;
     bool ok = true;
     for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
       const Tile at = tile(t);
-      const int mine = q * 32 + lane, col0 = at.nt * BN + half * HC;
+      const int mine = q * 32 + lane, col0 = at.nt * BN + part * HC;
       float2 acc[HC / 2];
 #pragma unroll
       for (int j = 0; j < HC / 2; ++j) acc[j] = make_float2(0.f, 0.f);
@@ -219,24 +223,22 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
         if (!(ok = mbar_wait(bar_tfull + 8 * a, aph, p.status, ERR_MBAR_TIMEOUT_EPILOGUE, abort_flag))) break;
         tc_fence_after();
         const float sx = small.scale[ring][mine];
-        const float* swp = &small.scale[ring][FG_BM + half * G];
-        const uint32_t from = tmem + ((uint32_t)(q * 32) << 16) + a * BN + half * HC;
-        uint32_t r[2][16];                                 // a load is under way while the one before is added
-        tmem_ld_cols<16>(from, r[0]);
+        const float* swp = &small.scale[ring][FG_BM + part * G];
+        const uint32_t from = tmem + ((uint32_t)(q * 32) << 16) + a * BN + part * HC;
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-          tmem_wait_for(r[g & 1]);
-          if (g + 1 < G) {
-            tmem_ld_cols<16>(from + 16 * (g + 1), r[(g + 1) & 1]);
-          } else {
+          uint32_t r[16];
+          tmem_ld_cols<16>(from + 16 * g, r);
+          const float sc = sx * swp[g];
+          tmem_ld_wait();
+          if (g + 1 == G) {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar_tempty + 8 * a);
           }
-          const float sc = sx * swp[g];
 #pragma unroll
           for (int j = 0; j < 8; ++j)
-            acc[8 * g + j] = fma2(make_float2(__uint_as_float(r[g & 1][2 * j]), __uint_as_float(r[g & 1][2 * j + 1])), make_float2(sc, sc), acc[8 * g + j]);
+            acc[8 * g + j] = fma2(make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), make_float2(sc, sc), acc[8 * g + j]);
         }
         if (++a == ACC) { a = 0; aph ^= 1; }
         if (++ring == S::RING) ring = 0;
@@ -264,7 +266,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
           constexpr int n = 2 * PIECE;
 #pragma unroll
           for (int j = 0; j < n; j += 16 / ESZ) {
-            uint8_t* to = stage + lane * S::ROW + ((((g * n + j) * ESZ / 16) ^ (lane & 7)) << 4);
+            uint8_t* to = stage + lane * S::ROW + ((((g * n + j) * ESZ / 16) ^ turn(lane)) << 4);
             if constexpr (F32) *reinterpret_cast<float4*>(to) = make_float4(v[j] * rs, v[j + 1] * rs, v[j + 2] * rs, v[j + 3] * rs);
             else *reinterpret_cast<uint4*>(to) = make_uint4(pack_bf16(v[j] * rs, v[j + 1] * rs), pack_bf16(v[j + 2] * rs, v[j + 3] * rs),
                                                             pack_bf16(v[j + 4] * rs, v[j + 5] * rs), pack_bf16(v[j + 6] * rs, v[j + 7] * rs));
@@ -276,7 +278,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
         const size_t step = (size_t)(32 / CPR) * p.ldc * ESZ;
 #pragma unroll 4
         for (int r = lane / CPR; r < live; r += 32 / CPR, to += step) {
-          const uint4 x = *reinterpret_cast<const uint4*>(stage + r * S::ROW + ((ch ^ (r & 7)) << 4));
+          const uint4 x = *reinterpret_cast<const uint4*>(stage + r * S::ROW + ((ch ^ turn(r)) << 4));
           if (wide && inside == 16 / ESZ) {
             *reinterpret_cast<uint4*>(to) = x;
           } else {
@@ -301,7 +303,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
 }
 
 template <int BN, int KIND, bool F32> static int launch_gemm(const CUtensorMap& tx, const CUtensorMap& tw, const Fp8Params& p, long long tiles, cudaStream_t st) {
-  using S = Fp8GemmShape<BN>;
+  using S = Fp8GemmShape<BN, F32>;
   auto kern = fp8_gemm_kernel<BN, KIND, F32>;
   static DeviceOnce configured;
   if (configured.pending()) {
