@@ -107,6 +107,12 @@ __device__ __forceinline__ void umma_commit_if(uint32_t leader, uint32_t bar) {
 __device__ __forceinline__ void mbar_arrive_if(uint32_t leader, uint32_t bar) {
   asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t@q mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}\n" ::"r"(bar), "r"(leader) : "memory");
 }
+// whether a phase has completed, without waiting: asked ahead of the work that it is asked before, the answer costs nothing
+__device__ __forceinline__ bool mbar_peek(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok != 0;
+}
 // kind::f8f6f4 instruction descriptor: e4m3 x e4m3 -> fp32, M x N tile, both operands K-major.
 __host__ __device__ constexpr uint32_t umma_idesc_e4m3(int M, int N) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }
 
@@ -168,7 +174,7 @@ struct Fp8Params {
   const int* counts;         // experts: rows of expert i of the bank, and the first of them
   const int* seg;
   const int* slot;           // slots: expert of output row m, whose input is row m / x_div
-  int x_div, e_lo;
+  int x_div, e_lo, cuts;     // cuts: pieces of a tile along K
   float* part;               // partial sums of cut tiles
   int* tickets;
   int* status;
@@ -190,12 +196,13 @@ struct Fp8Call {
   const int* counts;
   const int* seg;
   const int* slot;
-  float* scratch;            // streaming kernel: partial sums, and the counters of cut work (host_util.h)
+  float* scratch;            // partial sums, and the counters of cut work (host_util.h)
   int* tickets;
   int xb_rows, rows;         // rows of xb, and rounded rows
   int M, N, K, E, out_f32, act, x_div, e_lo;
-  int nt, bn;                // rows of a group of the streaming kernel, or 0 and the columns of a tile of the tiled one
+  int nt, bn, cuts;          // rows of a group of the streaming kernel, or 0 and the columns of a tile and its pieces along K of the tiled one
   float act_alpha, act_limit;
+  int unused;
 };
 int fp8_rows_launch(const void* x, int f32, long long ldx, const int* index, int x_rows, int rows, int K, void* codes, float* scale, cudaStream_t st);
 bool fp8_stream_rounds(const Fp8Call& c);

@@ -10,6 +10,7 @@
 //   warps 2, 3  asynchronous copies of the block's scales (128 of the rows, BN / 16 of the weights) into a ring.  Loads into registers would be waited for one block
 //               ahead at most, whatever the distance: they share the counters by which a warp waits
 //   warps 4-11  sums (warp & 3: rows, warp / 8: half of the columns); a finished tile goes through shared memory, so that rows are written in runs of 64 bytes
+// A dense product with fewer tiles than SMs is cut along K: the pieces of a tile leave fp32 sums, and the warp that arrives last adds them in the order of the pieces.
 // Every mbarrier wait is bounded.
 #include "act.cuh"
 #include "common.cuh"
@@ -18,8 +19,10 @@
 
 namespace mx {
 
-constexpr int FG_BM = 128, FG_SUMS = 16, FG_THREADS = 128 + 32 * FG_SUMS, FG_MAX_E = 1024;      // FG_SUMS: warps that hold sums
-constexpr int FG_GROUP = 8;                                // m-tiles that are walked together: a wave shares bands of x and w in L2
+constexpr int FG_BM = 128, FG_SUMS = 16, FG_THREADS = 128 + 32 * FG_SUMS, FG_MAX_E = 1024, FG_MAX_PIECES = 256;      // FG_SUMS: warps that hold sums
+// m-tiles that are walked together under each column of tiles: as many as leave a band of x of 32 MB, which stays in L2 while w streams past it once per band.
+// 4096 x 28672 x 4096 under the power cap: groups of 4, 8, 16 and all 32 m-tiles 643, 595, 586 and 572 us
+__host__ __device__ inline int fg_group(int kb) { return kb >= 256 ? 8 : 2048 / kb; }
 
 template <int BN, bool F32> struct Fp8GemmShape {
   static constexpr int A = FG_BM * FP8_BLOCK, B = BN * FP8_BLOCK, STAGE = A + B;
@@ -72,7 +75,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
   pdl_wait();
   if (warp == 1) { tmem_alloc(smem_u32(&s_tmem), 512); tmem_relinquish(); pdl_launch_dependents(); }
 
-  // ---- tiles: dense in groups of FG_GROUP m-tiles; experts one after the other, their m-tiles under each column of tiles
+  // ---- tiles: dense in bands of m-tiles; experts one after the other, their m-tiles under each column of tiles
   const bool banked = p.counts != nullptr;
   const int n_tiles = (p.N + BN - 1) / BN;
   int m_tiles = (p.M + FG_BM - 1) / FG_BM;
@@ -105,10 +108,14 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
-  const int tiles = m_tiles * n_tiles, sw_groups = (p.N + FP8_ROWS - 1) / FP8_ROWS;
-  struct Tile { int e, row0, rows, nt; };
+  const int cuts = p.cuts, tiles = m_tiles * n_tiles * cuts, sw_groups = (p.N + FP8_ROWS - 1) / FP8_ROWS;
+  struct Tile { int e, row0, rows, nt, k0, k1; };        // and its blocks of K
   auto tile = [&](int t) {
     Tile r;
+    const int piece = cuts > 1 ? t % cuts : 0;
+    if (cuts > 1) t /= cuts;
+    r.k0 = (int)((long long)p.kb * piece / cuts);
+    r.k1 = (int)((long long)p.kb * (piece + 1) / cuts);
     if (banked) {
       int lo = 0, hi = p.E - 1;                            // the expert with s_pre * n_tiles <= t < the next one's
       while (lo < hi) {
@@ -122,24 +129,24 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
       r.row0 = p.seg[lo] + m * FG_BM;
       r.rows = r.row0 < 0 ? 0 : min(min(FG_BM, p.counts[lo] - m * FG_BM), p.M - r.row0);
     } else {
-      const int full = FG_GROUP * n_tiles, g = t / full, i = t - g * full, gm = min(FG_GROUP, m_tiles - g * FG_GROUP);
+      const int band = min(fg_group(p.kb), m_tiles), full = band * n_tiles, g = t / full, i = t - g * full, gm = min(band, m_tiles - g * band);
       r.e = 0;
       r.nt = i / gm;
-      r.row0 = (g * FG_GROUP + i - r.nt * gm) * FG_BM;
+      r.row0 = (g * band + i - r.nt * gm) * FG_BM;
       r.rows = min(FG_BM, p.M - r.row0);
     }
     return r;
   };
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
     if (warp == 0 && lane == 0) {
       prefetch_tmap(&tm_x); prefetch_tmap(&tm_w);
       uint32_t s = 0, ph = 1;
       bool ok = true;
       for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
         const Tile at = tile(t);
-        for (int k = 0; k < p.kb; ++k) {
+        for (int k = at.k0; k < at.k1; ++k) {
           if (!(ok = mbar_wait(bar_empty + 8 * s, ph, p.status, ERR_MBAR_TIMEOUT_PRODUCER, abort_flag))) break;
           const uint32_t dst = base + s * S::STAGE;
           mbar_expect_tx(bar_full + 8 * s, S::STAGE);
@@ -152,22 +159,27 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
       const uint32_t leader = elect_one();
       constexpr uint32_t idesc = umma_idesc_e4m3(FG_BM, BN);
       uint32_t s = 0, ph = 0, a = 0, aph = 1;
-      bool ok = true;
-      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x)
-        for (int k = 0; k < p.kb; ++k) {
-          if (!(ok = mbar_wait(bar_tempty + 8 * a, aph, p.status, ERR_MBAR_TIMEOUT_MMA, abort_flag))) break;
-          if (!(ok = mbar_wait(bar_full + 8 * s, ph, p.status, ERR_MBAR_TIMEOUT_MMA, abort_flag))) break;
+      bool ok = true, data = false, room = false;
+      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        const int piece = cuts > 1 ? t % cuts : 0, n = (int)((long long)p.kb * (piece + 1) / cuts) - (int)((long long)p.kb * piece / cuts);
+        for (int k = 0; k < n; ++k) {
+          if (!room && !(ok = mbar_wait(bar_tempty + 8 * a, aph, p.status, ERR_MBAR_TIMEOUT_MMA, abort_flag))) break;
+          if (!data && !(ok = mbar_wait(bar_full + 8 * s, ph, p.status, ERR_MBAR_TIMEOUT_MMA, abort_flag))) break;
           __syncwarp();                                    // (no lane may miss a phase)
           tc_fence_after();
           const uint64_t dx = umma_desc_k_sw128(base + s * S::STAGE), dw = umma_desc_k_sw128(base + s * S::STAGE + S::A);
-#pragma unroll
-          for (int kk = 0; kk < FP8_BLOCK / 32; ++kk) umma_e4m3(leader, tmem + a * BN, dx + 2 * kk, dw + 2 * kk, idesc, kk != 0);
-          umma_commit_if(leader, bar_empty + 8 * s);
-          mbar_arrive_if(leader, bar_tfull + 8 * a);                  // (what this thread has seen arrive, the scales among it, is seen by who waits here)
-          umma_commit_if(leader, bar_tfull + 8 * a);
+          const uint32_t d = tmem + a * BN, empty = bar_empty + 8 * s, tfull = bar_tfull + 8 * a;
           if (++s == NST) { s = 0; ph ^= 1; }
           if (++a == ACC) { a = 0; aph ^= 1; }
+          data = mbar_peek(bar_full + 8 * s, ph);
+          room = mbar_peek(bar_tempty + 8 * a, aph);
+#pragma unroll
+          for (int kk = 0; kk < FP8_BLOCK / 32; ++kk) umma_e4m3(leader, d, dx + 2 * kk, dw + 2 * kk, idesc, kk != 0);
+          umma_commit_if(leader, empty);
+          mbar_arrive_if(leader, tfull);                   // (what this thread has seen arrive, the scales among it, is seen by who waits here)
+          umma_commit_if(leader, tfull);
         }
+      }
     } else if (warp >= 2) {
       uint32_t s = 0, ph = 1, r = 0;
       bool ok = true;
@@ -181,7 +193,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
         } else {
           from[0] = p.sw + ((size_t)at.e * sw_groups + min(at.nt * (BN / FP8_ROWS) + lane, sw_groups - 1)) * p.kb;
         }
-        for (int k = 0; k < p.kb; ++k) {
+        for (int k = at.k0; k < at.k1; ++k) {
           if (!(ok = mbar_wait(bar_empty + 8 * s, ph, p.status, ERR_MBAR_TIMEOUT_PRODUCER, abort_flag))) break;
           const uint32_t to = smem_u32(small.scale[r]) + 4 * lane;
           if (warp == 2) {
@@ -198,7 +210,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
     }
     __syncwarp();
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
     constexpr int HC = BN * 4 / FG_SUMS, G = HC / FP8_ROWS;          // columns of a thread, and the scales that they have
     const int q = warp & 3, part = (warp - 4) >> 2;
     constexpr int ESZ = F32 ? 4 : 2, PIECE = KIND == 1 ? 8 : 16;        // outputs of 16 sums
@@ -219,31 +231,65 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
       float2 acc[HC / 2];
 #pragma unroll
       for (int j = 0; j < HC / 2; ++j) acc[j] = make_float2(0.f, 0.f);
-      for (int k = 0; k < p.kb; ++k) {
+      for (int k = at.k0; k < at.k1; ++k) {
         if (!(ok = mbar_wait(bar_tfull + 8 * a, aph, p.status, ERR_MBAR_TIMEOUT_EPILOGUE, abort_flag))) break;
         tc_fence_after();
         const float sx = small.scale[ring][mine];
         const float* swp = &small.scale[ring][FG_BM + part * G];
         const uint32_t from = tmem + ((uint32_t)(q * 32) << 16) + a * BN + part * HC;
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-          uint32_t r[16];
-          tmem_ld_cols<16>(from + 16 * g, r);
-          const float sc = sx * swp[g];
+        for (int g = 0; g < G; g += 2) {
+          uint32_t r[32];
+          tmem_ld_cols<32>(from + 16 * g, r);
+          const float2 sw = *reinterpret_cast<const float2*>(swp + g);
+          const float s0 = sx * sw.x, s1 = sx * sw.y;
           tmem_ld_wait();
-          if (g + 1 == G) {
+          if (g + 2 == G) {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar_tempty + 8 * a);
           }
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
+          for (int j = 0; j < 16; ++j) {
+            const float sc = j < 8 ? s0 : s1;
             acc[8 * g + j] = fma2(make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), make_float2(sc, sc), acc[8 * g + j]);
+          }
         }
         if (++a == ACC) { a = 0; aph ^= 1; }
         if (++ring == S::RING) ring = 0;
       }
       if (!ok) break;
+
+      if (cuts > 1) {
+        const int w = warp - 4, own = t / cuts;
+        auto slab = [&](int piece) { return reinterpret_cast<float4*>(p.part) + ((size_t)(own * cuts + piece) * FG_SUMS + w) * (HC / 4 * 32) + lane; };
+        float4* to = slab(t - own * cuts);
+#pragma unroll
+        for (int j = 0; j < HC / 4; ++j) to[j * 32] = make_float4(acc[2 * j].x, acc[2 * j].y, acc[2 * j + 1].x, acc[2 * j + 1].y);
+        __threadfence();
+        __syncwarp();
+        int prev = 0;
+        if (lane == 0) {
+          prev = atomicAdd(p.tickets + own * FG_SUMS + w, 1);
+          if (prev == cuts - 1) p.tickets[own * FG_SUMS + w] = 0;
+        }
+        if (__shfl_sync(0xffffffffu, prev, 0) != cuts - 1) continue;
+        __threadfence();
+        const float4* from = slab(0);
+#pragma unroll
+        for (int j = 0; j < HC / 4; ++j) {
+          const float4 v = __ldcg(from + j * 32);
+          acc[2 * j] = make_float2(v.x, v.y); acc[2 * j + 1] = make_float2(v.z, v.w);
+        }
+        for (int piece = 1; piece < cuts; ++piece) {
+          from = slab(piece);
+#pragma unroll
+          for (int j = 0; j < HC / 4; ++j) {
+            const float4 v = __ldcg(from + j * 32);
+            acc[2 * j].x += v.x; acc[2 * j].y += v.y; acc[2 * j + 1].x += v.z; acc[2 * j + 1].y += v.w;
+          }
+        }
+      }
 
       // ---- the tile: bias, activation, scale; a row's outputs meet in shared memory and are written as lines
       const float rs = p.row_scale && mine < at.rows ? p.row_scale[at.row0 + mine] : 1.f;
@@ -315,20 +361,22 @@ template <int BN, int KIND, bool F32> static int launch_gemm(const CUtensorMap& 
   return (int)cudaGetLastError();
 }
 
-// Dense (M rows) or experts (counts / seg: from the bank's first expert on; M rows of the packing), tiles of bn = 128 or 256 columns.
+// Dense (M rows) or experts (counts / seg: from the bank's first expert on; M rows of the packing), tiles of bn = 128 or 256 columns; dense ones in `cuts` pieces along K.
 int fp8_gemm_launch(const Fp8Call& c, cudaStream_t st) {
-  const Fp8Params p = fp8_params(c);
+  Fp8Params p = fp8_params(c);
+  p.cuts = c.cuts > 1 ? c.cuts : 1;
   const int bn = c.bn;
   if (c.E > FG_MAX_E || c.slot || (bn != 128 && bn != 256) || (c.counts && (c.M + FG_BM - 1) / FG_BM + c.E > 65535)) return -106;
   if (((uintptr_t)c.codes | (uintptr_t)c.w) & 15) return -114;
   const long long tiles = ((c.M + FG_BM - 1) / FG_BM + (c.counts ? (c.E < c.M ? c.E : c.M) : 0)) * (long long)((c.N + bn - 1) / bn);
   if (tiles >= 1ll << 31) return -106;
+  if (p.cuts > 1 && (c.counts || p.cuts > p.kb || tiles * FG_SUMS > CUT_TICKETS || tiles * p.cuts > FG_MAX_PIECES || !c.scratch || !c.tickets || ((uintptr_t)c.scratch & 15))) return -106;
   CUtensorMap tx, tw;
   int r = fp8_tmap(&tx, c.codes, p.kb, c.rows, 0, FG_BM);
   if (!r) r = fp8_tmap(&tw, c.w, p.kb, p.N, c.E, bn);
   if (r) return r;
   const int kind = p.act == 0 ? 0 : act_gated(p.act) ? 1 : 2;
-#define MX_FG(BN_, KIND_) if (bn == BN_ && kind == KIND_) return p.out_f32 ? launch_gemm<BN_, KIND_, true>(tx, tw, p, tiles, st) : launch_gemm<BN_, KIND_, false>(tx, tw, p, tiles, st)
+#define MX_FG(BN_, KIND_) if (bn == BN_ && kind == KIND_) return p.out_f32 ? launch_gemm<BN_, KIND_, true>(tx, tw, p, tiles * p.cuts, st) : launch_gemm<BN_, KIND_, false>(tx, tw, p, tiles * p.cuts, st)
   MX_FG(256, 0); MX_FG(256, 1); MX_FG(256, 2);
   MX_FG(128, 0); MX_FG(128, 1); MX_FG(128, 2);
 #undef MX_FG
@@ -338,6 +386,9 @@ int fp8_gemm_launch(const Fp8Call& c, cudaStream_t st) {
 }  // namespace mx
 
 using namespace mx;
+
+// Bytes of scratch (16-byte aligned) that `pieces` pieces of tiles of bn columns want.
+MX_HOST_API long long mx_fp8_tile_scratch(int pieces, int bn) { return 4ll * pieces * FG_BM * bn; }
 
 MX_HOST_API int mx_fp8_call_bytes() { return (int)sizeof(Fp8Call); }
 

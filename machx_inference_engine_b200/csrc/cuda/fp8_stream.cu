@@ -1,7 +1,7 @@
-// Products of a few e4m3 rows (up to 128 together) with e4m3 weights, bound by reading the weights: a dense layer of a decode batch, an expert's few rows, a slot's one row.
+// Products of a few e4m3 rows (up to 64 together) with e4m3 weights, bound by reading the weights: a dense layer of a decode batch, an expert's few rows, a slot's one row.
 //   y[m, n] = act(sum_b sx[b][m] sw[n / 16][b] sum_{k in b} x8[m][k] w8[n][k] + bias[n])
 //
-// The weights are the M side of tcgen05.mma (128 weight rows x 128 bytes: one block of K, one TMA box) and the rows its N side, padded to NT = 16 to 128
+// The weights are the M side of tcgen05.mma (128 weight rows x 128 bytes: one block of K, one TMA box) and the rows its N side, padded to NT = 16, 32 or 64
 // columns; the tensor cores need a small part of the time that the box takes to arrive, whatever NT.  Every block has scales of its own, so its sums go from
 // TMEM to registers, where a thread owns a weight row and adds s_x s_w times them to NT sums in fp32.
 //   warp 0      TMA boxes of weights and of rows into a ring of NST stages, and asynchronous copies of their scales into a ring of their own
@@ -29,13 +29,13 @@ template <int NT, bool ROUND> struct Fp8StreamShape {
   static constexpr int X = NT * FP8_BLOCK;
   static constexpr int STAGE = FS_W + (ROUND ? 0 : X);
   static constexpr int BLOCKS = ROUND ? 26 : 0;        // blocks of rounded rows that a CTA keeps
-  static constexpr int CTAS = NT <= 64 ? 2 : 1;        // per SM; 128 sums a thread want all the registers
+  static constexpr int CTAS = 2;                       // per SM
   static constexpr int OUT = 4 * 8 * 32 * 4;           // eight columns of a warp's sums, on their way out
-  static constexpr int ROOM = (CTAS == 2 ? 104 : 200) * 1024 - OUT;      // for stages and rounded rows
+  static constexpr int ROOM = 104 * 1024 - OUT;      // for stages and rounded rows
   static constexpr int SMEM = ROOM + OUT + 1024;
   static constexpr int NST = ROUND ? 5 : ROOM / STAGE; // at most; fewer where a run needs more rounded rows
-  static constexpr int ACC = NT <= 64 ? 4 : 2;
-  static constexpr int TMEM = NT * ACC;                // 64, 128, 256, 256 columns: two CTAs have 512
+  static constexpr int ACC = 4;
+  static constexpr int TMEM = NT * ACC;                // 64, 128, 256 columns: two CTAs have 512
   // Scales of a unit: 8 of the weights, NT of the rows.  A slot is free again when the products of the unit NST before are done, since they waited for the sums
   // of the unit ACC before them.
   static constexpr int RING = NST + ACC, SC = 8 + (ROUND ? 0 : NT);
@@ -341,22 +341,37 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
               for (int j = 0; j < 4; ++j) { col[64 * j] = acc[4 * g + j].x; col[64 * j + 32] = acc[4 * g + j].y; }
             }
           const int live = min(8, at.rows - j0);
-#pragma unroll 2
-          for (int j = 0; j < live; ++j) {
-            float v = col[32 * j] + bias;                // (a lane reads what it has written)
-            const int row = at.row0 + j0 + j;
-            if (gated) {
-              float pair[2] = {v, __shfl_down_sync(0xffffffffu, v, 16)};
-              glu_run<1>(p.act, pair, p.act_alpha, p.act_limit);
-              v = pair[0];
-            } else if (p.act) {
-              v = act_unary<false>(p.act, v, p.act_alpha, p.act_limit);
-            }
-            if (p.row_scale) v *= p.row_scale[row];
-            if (!owned) v = 0.f;
-            if (write) {
-              if (p.out_f32) ((float*)p.C)[row * p.ldc + o] = v;
-              else ((__nv_bfloat16*)p.C)[row * p.ldc + o] = __float2bfloat16(v);
+          float v[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = col[32 * j] + bias;             // (a lane reads what it has written; columns past the live ones hold anything)
+          if (gated) {
+            float pair[16];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) { pair[j] = v[j]; pair[8 + j] = __shfl_down_sync(0xffffffffu, v[j], 16); }
+            glu_run<8>(p.act, pair, p.act_alpha, p.act_limit);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = pair[j];
+          } else if (p.act) {
+            act_unary_run<false>(p.act, v, p.act_alpha, p.act_limit);
+          }
+          if (p.row_scale) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] *= p.row_scale[at.row0 + min(j0 + j, at.rows - 1)];
+          }
+          if (!owned) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = 0.f;
+          }
+          const size_t first = (size_t)(at.row0 + j0) * p.ldc + o;
+          if (write) {
+            if (p.out_f32) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (j < live) ((float*)p.C)[first + j * p.ldc] = v[j];
+            } else {
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (j < live) ((__nv_bfloat16*)p.C)[first + j * p.ldc] = __float2bfloat16(v[j]);
             }
           }
         }
@@ -431,10 +446,11 @@ template <int NT, bool ROUND> static int launch_stream(const CUtensorMap& tw, co
   return (int)cudaGetLastError();
 }
 
-// Whether the streaming kernel rounds a launch's rows itself: up to 16, of which a CTA's share of the blocks fits its shared memory.
+// Whether the streaming kernel rounds a launch's rows itself: up to eight (slots: one each), of which a CTA's share of the blocks fits its shared memory.  us, two launches -> one: 4 rows x
+// 6144 x 4096 11.6 -> 10.5, 4096 x 14336 17.6 -> 15.7, 28672 x 4096 28.2 -> 24.9, and a launch less on the host (5 us of 15); 8 rows even; 16 rows 12.3 -> 15.7, 27.7 -> 44.3.
 bool fp8_stream_rounds(const Fp8Call& c) {
   using S = Fp8StreamShape<16, true>;
-  if (!c.xb || c.nt != 16 || c.counts || c.K < 8 || c.ldx % 8 || ((uintptr_t)c.xb & 15)) return false;
+  if (!c.xb || c.nt != 16 || c.counts || (!c.slot && c.M > 8) || c.K < 8 || c.ldx % 8 || ((uintptr_t)c.xb & 15)) return false;
   const int kb = (c.K + FP8_BLOCK - 1) / FP8_BLOCK, n_tiles = (c.N + FS_TILE - 1) / FS_TILE;
   const long long total = (c.slot ? (long long)c.M : 1) * n_tiles * kb;
   if (total >= 1ll << 30) return false;
@@ -442,7 +458,7 @@ bool fp8_stream_rounds(const Fp8Call& c) {
   return (c.slot ? per : per < kb ? per : kb) <= S::BLOCKS;
 }
 
-// Dense (M <= nt), experts (counts / seg) or slots (slot), in groups of nt = 16, 32, 64 or 128 rows.
+// Dense (M <= nt), experts (counts / seg) or slots (slot), in groups of nt = 16, 32 or 64 rows.
 int fp8_stream_launch(const Fp8Call& c, bool round, cudaStream_t st) {
   Fp8Params p = fp8_params(c);
   const int nt = c.nt;
@@ -463,7 +479,6 @@ int fp8_stream_launch(const Fp8Call& c, bool round, cudaStream_t st) {
     case 16: return launch_stream<16, false>(tw, tx, p, st);
     case 32: return launch_stream<32, false>(tw, tx, p, st);
     case 64: return launch_stream<64, false>(tw, tx, p, st);
-    case 128: return launch_stream<128, false>(tw, tx, p, st);
     default: return -106;
   }
 }

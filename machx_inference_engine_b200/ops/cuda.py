@@ -6,6 +6,7 @@ to PyTorch math: a missing or failing kernel raises.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 import struct
 import threading
@@ -881,10 +882,9 @@ def expert_gemv(x, w: QuantWeight, slot_expert, x_div=1, bias=None, act=ACT_NONE
 
 
 # ------------------------------------------------------------------ 8-bit floating point (see ops/fp8.py)
-FP8_STREAM_ROWS = (16, 32, 64, 128)      # rows of a group in the weight-streaming kernel
-_FP8_CALL = struct.Struct("<16q12i2f")   # csrc/cuda/fp8.cuh: Fp8Call
+FP8_STREAM_ROWS = (16, 32, 64)           # rows of a group in the weight-streaming kernel
+_FP8_CALL = struct.Struct("<16q13i2fi")   # csrc/cuda/fp8.cuh: Fp8Call
 _FP8_WANTS_ROOM = -130                   # and the answer to bf16 rows without room for rounded ones, where the kernel does not round them itself
-_FP8_SCRATCH: dict = {}                  # rows of a group -> bytes of partial sums
 _fp8_lib = None
 
 
@@ -895,7 +895,7 @@ def _fp8_entry():
     if lib is not _fp8_lib:
         lib.mx_fp8_rows.argtypes = [_vp, C.c_int, C.c_longlong, _vp, C.c_int, C.c_int, C.c_int, _vp, _vp, _vp]
         lib.mx_fp8_product.argtypes = [C.c_char_p, _vp]
-        lib.mx_fp8_stream_scratch.restype = C.c_longlong
+        lib.mx_fp8_stream_scratch.restype = lib.mx_fp8_tile_scratch.restype = C.c_longlong
         if lib.mx_fp8_call_bytes() != _FP8_CALL.size:
             raise KernelError("the kernel library's description of an FP8 product is another one: rebuild it")
         _fp8_lib = lib
@@ -923,17 +923,22 @@ def fp8_rows(x, index=None) -> FP8Rows:
     return FP8Rows(codes, scale, K)
 
 
-def _fp8_call(x, w: QuantWeight, out, bias, row_scale, act, act_alpha, act_limit, nt=0, bn=0, counts=None, seg=None, slot=None, x_div=1, e_lo=0, index=None):
-    """One product on the current device: ``nt`` rows of a group (csrc/cuda/fp8_stream.cu) or ``bn`` columns of a tile (csrc/cuda/fp8_gemm.cu).  bf16 rows that the kernel does
+@functools.lru_cache(maxsize=None)
+def _fp8_scratch_bytes(nt: int) -> int:
+    return _fp8_entry().mx_fp8_stream_scratch(nt)
+
+
+def _fp8_call(x, w: QuantWeight, out, bias, row_scale, act, act_alpha, act_limit, nt=0, bn=0, cuts=1, counts=None, seg=None, slot=None, x_div=1, e_lo=0, index=None):
+    """One product on the current device: ``nt`` rows of a group (csrc/cuda/fp8_stream.cu) or ``bn`` columns of a tile in ``cuts`` pieces along K (csrc/cuda/fp8_gemm.cu).  bf16 rows that the kernel does
     not round itself are rounded into a scratch buffer first, by the same call: an ordinary allocation, stream-ordered and of the graph's own pool under capture.  Partial sums
     go to memory that a stream's launches share, since they follow one another, and under capture to an allocation as well."""
     lib = _fp8_entry()
     dev = out.device
     part = counters = 0
-    if nt:
+    if nt or cuts > 1:
         tickets = _tickets(dev)
         counters, kept = tickets[0].data_ptr(), tickets[3]
-        work = _FP8_SCRATCH.get(nt) or _FP8_SCRATCH.setdefault(nt, lib.mx_fp8_stream_scratch(nt))
+        work = _fp8_scratch_bytes(nt) if nt else lib.mx_fp8_tile_scratch(-(-out.shape[0] // 128) * -(-w.N // bn) * cuts, bn)
         if kept is None:
             scratch = torch.empty(work, dtype=torch.uint8, device=dev)
         else:
@@ -954,18 +959,48 @@ def _fp8_call(x, w: QuantWeight, out, bias, row_scale, act, act_alpha, act_limit
             codes = rounded.data_ptr()
             scale = codes + n * _fp8.FP8_BLOCK
         call = _FP8_CALL.pack(xb, ldx, _ptr(index), codes, scale, w.p0.data_ptr(), w.p1.data_ptr(), out.data_ptr(), out.stride(0), _ptr(bias), _ptr(row_scale), _ptr(counts),
-                              _ptr(seg), _ptr(slot), part, counters, xb_rows, rows, out.shape[0], w.N, w.K, w.E, out.dtype == torch.float32, act, x_div, e_lo, nt, bn, act_alpha,
-                              act_limit)
+                              _ptr(seg), _ptr(slot), part, counters, xb_rows, rows, out.shape[0], w.N, w.K, w.E, out.dtype == torch.float32, act, x_div, e_lo, nt, bn, cuts, act_alpha,
+                              act_limit, 0)
         rc = lib.mx_fp8_product(call, torch._C._cuda_getCurrentRawStream(dev.index))
     _check(rc, "fp8 product")
     _count()
     return out
 
 
-def _fp8_bn(M: int, N: int) -> int:
-    sms = sm_count()
-    waves = lambda bn: -(-(-(-M // 128) * -(-N // bn)) // sms)
-    return 256 if 1.9 * waves(256) < waves(128) else 128
+@functools.lru_cache(maxsize=4096)
+def _fp8_plan(M: int, N: int, K: int) -> tuple:
+    """(nt, bn, cuts) of a dense product.  Up to 32 rows the weights are streamed past groups of 16 or 32; us, that -> tiles: 17 rows x 6144 x 4096 13.2 -> 15.2, 4096 x 14336 19.1 ->
+    22.2, 2048 x 2048 8.7 -> 10.1; 33 rows (groups of 64) 16.6 -> 15.2, 24.0 -> 22.7, 11.5 -> 10.1.
+
+    Tiles: in us, a wave takes 0.31 a block of K with 128 columns and 0.5 with 256, and 1.2 or 1.8 at its end; where the tiles leave SMs idle they are cut along K,
+    which costs about 4 + 0.5 (6 + 0.6) a piece.  Measured, one piece -> the cut that is taken: 64 x 4096 x 14336 39.5 -> 23.2 (four of 128 columns), 256 x 4096 x
+    14336 42.8 -> 33.1 (two), 384 x 4096 x 14336 45.0 -> 40.7 (three of 256), 128 x 1024 x 8192 25.1 -> 15.5 (six); 64 x 6144 x 4096 stays at 15.6 (two: 15.6), 64 x 2048 x 2048
+    at 10.3 (11.4).  256 columns for 128: 33 x 28672 x 4096 31.3 -> 27.5, 1024 x 4096 x 14336 84 -> 70; not 512 x 4096 x 14336 (45.6, 64.4)."""
+    if M <= 32:
+        return (16 if M <= 16 else 32), 0, 1
+    sms, kb = sm_count(), -(-K // _fp8.FP8_BLOCK)
+    best = None
+    for bn, block, end, cut, piece in ((128, 0.31, 1.2, 4.0, 0.5), (256, 0.5, 1.8, 6.0, 0.6)):
+        tiles = -(-M // 128) * -(-N // bn)
+        for cuts in range(1, max(1, min(sms // tiles, kb // 4, 16)) + 1):
+            cost = -(-tiles * cuts // sms) * (-(-kb // cuts) * block + end) + (cut + piece * cuts if cuts > 1 else 0.0)
+            if best is None or cost < best[0]:
+                best = (cost, bn, cuts)
+    return 0, best[1], best[2]
+
+
+def _fp8_expert_plan(rows: int, experts: int, K: int) -> tuple:
+    """(nt, bn) of a bank's product by the mean rows per expert: the weights streamed past groups of nt rows, or tiles of 128 rows and bn columns.  us with groups of 16, 32,
+    64 and tiles of 256 columns, scores of the experts spread by half a standard deviation: 512 experts of 1024 x 2048, 0.8 rows 79, 79, 78, 82; 3.1 rows 136, 133, 127, 139; 5 rows 161,
+    153, 143, 155; 12.5 rows 255, 207, 188, 186; 40 rows 509, 367, 318, 227.  128 of 1536 x 2048, 1 row 39.3, 40.0, 40.5, 44.0; 10 rows 75, 78, 77, 85; 16 rows 97, 75, 80, 77.  32 of 5760 x
+    2880, 12.5 rows 113, 102, 97, 100; 20 rows 160, 123, 105, 103.  Short rows (128 of 2048 x 768) prefer smaller groups, 10 rows 41, 45, 55, 48; 16 rows 51, 49, 63, 52.  Tiles of 128
+    columns were slower than 256 throughout (40 rows of 1024 x 2048 246, 227)."""
+    mean = rows / experts
+    if mean <= 2:
+        return 16, 0
+    if mean <= 12:
+        return (64 if K >= 1024 else 32), 0
+    return 0, 256
 
 
 def _fp8_product(x, w: QuantWeight, shape, dtype, out, bias, row_scale, act, act_alpha, act_limit, **kw):
@@ -980,11 +1015,12 @@ def _fp8_product(x, w: QuantWeight, shape, dtype, out, bias, row_scale, act, act
     if M == 0:
         return out
     if kw.get("slot") is not None:
-        nt = 16
+        nt, bn, cuts = 16, 0, 1
+    elif kw.get("counts") is not None:
+        (nt, bn), cuts = _fp8_expert_plan(M, w.E, w.K), 1
     else:
-        rows = M if kw.get("counts") is None else 2 * M / w.E
-        nt = 16 if rows <= 16 else 32 if rows <= 32 else 64 if rows <= 64 else 128 if rows <= 128 else 0
-    return _fp8_call(x, w, out, bias, row_scale, act, act_alpha, act_limit, nt, 0 if nt else _fp8_bn(M, w.N), **kw)
+        nt, bn, cuts = _fp8_plan(M, w.N, w.K)
+    return _fp8_call(x, w, out, bias, row_scale, act, act_alpha, act_limit, nt, bn, cuts, **kw)
 
 
 def _linear_fp8(x, w: QuantWeight, bias, act, act_alpha, act_limit, out_f32, row_scale, out):

@@ -124,10 +124,12 @@ def test_each_kernel_at_every_tile_size(M, N, K):
             out = torch.empty(M, N, device=DEV)
             assert O.rel(K_()._fp8_call(rows, w, out, None, None, 0, 0.0, 0.0, nt), want) < tolerance(K), nt
             assert O.rel(K_()._fp8_call(rows, w, out, bias, rs, 0, 0.0, 0.0, nt), full) < tolerance(K), nt
-        for bn in (128, 256):
+        for bn, cuts in ((128, 1), (256, 1), (128, 2), (256, 3), (128, 4), (256, 5)):
+            if cuts > -(-K // 128):
+                continue
             out = torch.empty(M, N, device=DEV)
-            assert O.rel(K_()._fp8_call(rows, w, out, None, None, 0, 0.0, 0.0, 0, bn), want) < tolerance(K), bn
-            assert O.rel(K_()._fp8_call(rows, w, out, bias, rs, 0, 0.0, 0.0, 0, bn), full) < tolerance(K), bn
+            assert O.rel(K_()._fp8_call(rows, w, out, None, None, 0, 0.0, 0.0, 0, bn, cuts), want) < tolerance(K), (bn, cuts)
+            assert O.rel(K_()._fp8_call(rows, w, out, bias, rs, 0, 0.0, 0.0, 0, bn, cuts), full) < tolerance(K), (bn, cuts)
 
 
 @pytest.mark.parametrize("act", ["none", "geglu"])
