@@ -17,6 +17,7 @@ from typing import Optional
 import numpy as np
 
 from .gguf import GGMLType, GGUFReader, GGUFWriter
+from .names import FP8_BLOCK_COLS, FP8_BLOCK_ROWS, FP8_SCALES
 from .quant import quantize
 from .safetensors import SafetensorsModel, awq_dequant, gptq_dequant
 
@@ -41,7 +42,8 @@ class HFMeta:
     rms_eps: float = 1e-6
     tie_word_embeddings: bool = False
     attention_bias: bool = False
-    quant_method: str = ""           # "" | awq | gptq | exl3
+    quant_method: str = ""           # "" | awq | gptq | exl3 | fp8
+    fp8_block: tuple = (128, 128)    # rows and elements of K that share a scale
     bits: int = 4
     group_size: int = 128
     version: str = "gemm"
@@ -80,9 +82,16 @@ def parse_hf_config(text: str) -> HFMeta:
             if m.arch not in ("llama",):
                 raise ImportError_(f"EXL3 import takes dense llama checkpoints, not '{m.arch}'")
             return m
-        if m.quant_method not in ("awq", "gptq"):
-            raise ImportError_(f"unsupported quant_method '{m.quant_method}' (awq | gptq | exl3)")
-        if m.bits != 4:
+        if m.quant_method == "fp8":
+            block = q.get("weight_block_size")
+            if str(q.get("activation_scheme", "dynamic")).lower() != "dynamic" or not isinstance(block, list) or len(block) != 2:
+                raise ImportError_("FP8 import takes block-quantised checkpoints with dynamic activation scales (weight_block_size)")
+            m.fp8_block = (int(block[0]), int(block[1]))
+            if m.fp8_block[0] < 1 or m.fp8_block[0] % 16 or m.fp8_block[1] < 1 or m.fp8_block[1] % 128:
+                raise ImportError_(f"FP8 blocks of {m.fp8_block[0]} x {m.fp8_block[1]}: whole multiples of 16 x 128 are taken")
+        elif m.quant_method not in ("awq", "gptq"):
+            raise ImportError_(f"unsupported quant_method '{m.quant_method}' (awq | gptq | exl3 | fp8)")
+        if m.quant_method in ("awq", "gptq") and m.bits != 4:
             raise ImportError_(f"4-bit only (got {m.bits})")
         if m.quant_method == "awq" and m.version != "gemm":
             raise ImportError_(f"AWQ pack order '{m.version}' is not supported (only 'gemm')")
@@ -256,6 +265,8 @@ def import_to_gguf(hf_dir: str, out_path: str, tokenizer_gguf: Optional[str] = N
         kv.update(_tokenizer_kv_from_json(tj, emb_rows))
     else:
         raise ImportError_("no tokenizer: pass --tokenizer-gguf <file.gguf> or put tokenizer.json next to the weights")
+    if m.quant_method == "fp8":
+        kv[FP8_BLOCK_ROWS], kv[FP8_BLOCK_COLS] = m.fp8_block
     for k, v in kv.items():
         w.add_kv(k, v)
 
@@ -271,7 +282,17 @@ def import_to_gguf(hf_dir: str, out_path: str, tokenizer_gguf: Optional[str] = N
         g = hf_to_gguf_name(n)
         if not g or n in done:
             continue
-        if n.endswith((".qzeros", ".scales", ".g_idx")):
+        if n.endswith((".qzeros", ".scales", ".g_idx", ".weight_scale_inv")):
+            continue
+        if st.dtype(n) == "F8_E4M3":
+            # kept as they are, in the Hugging Face row order (the graph skips its llama re-ordering for these layers)
+            shp, sc = st.shape(n), n + "_scale_inv"
+            if m.quant_method != "fp8" or not n.endswith(".weight") or len(shp) != 2 or not st.has(sc):
+                raise ImportError_(f"{n}: an FP8 matrix is missing its weight_scale_inv")
+            bn, bk = m.fp8_block
+            if tuple(st.shape(sc)) != (-(-shp[0] // bn), -(-shp[1] // bk)):
+                raise ImportError_(f"{n}: scales {tuple(st.shape(sc))} do not fit {tuple(shp)} in blocks of {bn} x {bk}")
+            plan.append((g, "fp8", n, (shp[1], shp[0])))
             continue
         if n.endswith(".qweight"):
             base = n[:-len(".qweight")]
@@ -309,7 +330,13 @@ def import_to_gguf(hf_dir: str, out_path: str, tokenizer_gguf: Optional[str] = N
 
     n_t = 0
     for gname, kind, src, dims in plan:
-        if kind == "vec":
+        if kind == "fp8":
+            sc = src + "_scale_inv"
+            w.add_tensor(gname, [int(v) for v in dims], int(GGMLType.I8), (lambda nn=src: np.ascontiguousarray(st.numpy(nn)).view(np.uint8).reshape(-1)))
+            w.add_tensor(gname[:-len(".weight")] + FP8_SCALES, [int(v) for v in reversed(st.shape(sc))], int(GGMLType.F32),
+                         (lambda nn=sc: np.ascontiguousarray(st.float32(nn)).view(np.uint8).reshape(-1)))
+            n_t += 1
+        elif kind == "vec":
             w.add_tensor(gname, [int(np.prod(dims))], int(GGMLType.F32), make(gname, kind, src, dims))
         else:
             k, n_out = dims

@@ -15,7 +15,7 @@ import numpy as np
 from .. import _lib
 
 _DT = {"F64": np.float64, "F32": np.float32, "F16": np.float16, "BF16": np.uint16, "I64": np.int64, "I32": np.int32, "I16": np.int16,
-       "I8": np.int8, "U8": np.uint8, "BOOL": np.uint8, "U16": np.uint16, "U32": np.uint32}
+       "I8": np.int8, "U8": np.uint8, "F8_E4M3": np.uint8, "BOOL": np.uint8, "U16": np.uint16, "U32": np.uint32}
 
 
 def _lib_st():
@@ -72,6 +72,9 @@ class SafetensorsFile:
         a = self.numpy(name)
         if dt == "BF16":
             return (a.astype(np.uint32) << 16).view(np.float32)
+        if dt == "F8_E4M3":      # (the codes' own values; scales are tensors of their own)
+            import torch
+            return torch.from_numpy(np.array(a)).view(torch.float8_e4m3fn).to(torch.float32).numpy()
         return a.astype(np.float32)
 
     def close(self):
@@ -126,7 +129,7 @@ class SafetensorsModel:
 
 def write_safetensors(path: str, tensors: dict, metadata: dict | None = None) -> None:
     """``tensors``: name -> numpy array, or (dtype string, array) to force e.g. "BF16" for a uint16 array."""
-    rev = {np.dtype(v): k for k, v in _DT.items() if k not in ("BOOL", "BF16", "U16")}
+    rev = {np.dtype(v): k for k, v in _DT.items() if k not in ("BOOL", "BF16", "U16", "F8_E4M3")}
     header, blobs, off = {}, [], 0
     if metadata:
         header["__metadata__"] = metadata

@@ -195,6 +195,8 @@ def _matrix_type(name: str, kind: str, K: int, quant: str, n_layers: int) -> int
     fmt = default_policy("", quant)(name)
     if fmt == WFormat.EXL3:
         return GGMLType.EXL3 if kind == "matrix" else GGMLType.BF16        # expert stacks stay dense
+    if fmt == WFormat.FP8:
+        return GGMLType.I8
     t = {WFormat.BF16: GGMLType.BF16, WFormat.Q8: GGMLType.Q8_0, WFormat.Q4K: GGMLType.Q4_K, WFormat.Q6K: GGMLType.Q6_K, WFormat.MXFP4: GGMLType.MXFP4}[fmt]
     if K % block_elems(t):
         t = GGMLType.Q8_0 if K % 32 == 0 else GGMLType.F16
@@ -260,6 +262,25 @@ def _add_exl3(w, name: str, dims: tuple, quant: str, seed: int) -> int:
     return 3
 
 
+def _add_fp8(w, name: str, dims: tuple, seed: int) -> int:
+    """A random FP8 layer the way an imported checkpoint stores it: e4m3 codes as bytes, an fp32 scale per block of 128 x 128 beside them."""
+    from ..ops.weights import quantize_fp8
+    from .names import FP8_SCALES
+    import torch
+    K, N, E = (dims + (1,))[:3]
+    root = name[:-len(".weight")] if name.endswith(".weight") else name
+
+    def layer(e):
+        x = torch.from_numpy((0.02 * _rng(f"{name}#{e}", seed).standard_normal((N, K))).astype(np.float32))
+        return quantize_fp8(x)
+
+    codes = lambda: np.concatenate([layer(e).p0.view(torch.uint8)[0, :, :K].contiguous().numpy().reshape(-1) for e in range(E)])
+    scales = lambda: np.concatenate([layer(e).p1[0, ::8].contiguous().numpy().view(np.uint8).reshape(-1) for e in range(E)])      # (eight runs of 16 rows to a block)
+    w.add_tensor(name, dims, int(GGMLType.I8), codes)
+    w.add_tensor(root + FP8_SCALES, (-(-K // 128), -(-N // 128)) + tuple(dims[2:]), int(GGMLType.F32), scales)
+    return 2
+
+
 def write_synthetic_gguf(cfg: ModelConfig, path: str, quant: str = "q8_0", seed: int = 0, tokenizer: bool = True,
                          extra_kv: Iterable = ()) -> dict:
     """Writes the checkpoint; returns {"tensors": n, "bytes": payload bytes}."""
@@ -284,6 +305,9 @@ def write_synthetic_gguf(cfg: ModelConfig, path: str, quant: str = "q8_0", seed:
             else:
                 n += _add_exl3(w, name, dims, quant, seed)
                 continue
+        if t == GGMLType.I8:
+            n += _add_fp8(w, name, tuple(dims), seed)
+            continue
         w.add_tensor(name, dims, int(t), _payload(name, kind, dims, int(t), seed))
         n += 1
     w.write(path)

@@ -14,7 +14,8 @@ import numpy as np
 import torch
 
 from ..formats.gguf import GGMLType, GGUFReader
-from ..ops.weights import QuantWeight, WFormat, from_dense, from_exl3, from_ggml
+from ..formats.names import FP8_BLOCK_COLS, FP8_BLOCK_ROWS, FP8_SCALES
+from ..ops.weights import QuantWeight, WFormat, from_dense, from_exl3, from_fp8, from_ggml
 
 
 class GGUFSource:
@@ -34,6 +35,9 @@ class GGUFSource:
             root = name[:-len(".weight")] if name.endswith(".weight") else name
             tr = torch.from_numpy(np.frombuffer(np.array(t.raw(), copy=True), dtype=np.int16).reshape(K // 16, N // 16, int(t.dims[0])))
             return from_exl3(tr.to(self.device), self.vector(root + ".suh", K), self.vector(root + ".svh", N))
+        root = name[:-len(".weight")] if name.endswith(".weight") else name
+        if int(t.type) == GGMLType.I8 and self.r.has_tensor(root + FP8_SCALES):
+            return self._fp8(name, root, t, N, K, E, experts)
         want = (K, N) if E == 1 else (K, N, E)
         if tuple(t.dims) != want:
             raise ValueError(f"{name}: expected ggml dims {want}, file has {tuple(t.dims)}")
@@ -43,6 +47,20 @@ class GGUFSource:
             raw = raw[experts[0] * per: experts[1] * per]
             E = experts[1] - experts[0]
         return from_ggml(raw.to(self.device), t.type, N, K, E)
+
+    def _fp8(self, name: str, root: str, t, N: int, K: int, E: int, experts) -> QuantWeight:
+        """e4m3 codes as bytes, and fp32 scales {blocks of K, blocks of N (, E)} beside them (<root>.fp8_scale) that share the block size of the file."""
+        s = self.r.tensor(root + FP8_SCALES)
+        bn, bk = int(self.r.get(FP8_BLOCK_ROWS, 128)), int(self.r.get(FP8_BLOCK_COLS, 128))
+        want, scales = (K, N), (-(-K // bk), -(-N // bn))
+        if E > 1:
+            want, scales = want + (E,), scales + (E,)
+        if tuple(t.dims) != want or tuple(s.dims) != scales:
+            raise ValueError(f"{name}: FP8 codes {tuple(t.dims)} with scales {tuple(s.dims)} do not describe a matrix of {want} in blocks of {bn} x {bk}")
+        lo, hi = experts if experts is not None else (0, E)
+        raw = torch.from_numpy(np.array(t.raw(), copy=True)[lo * N * K:hi * N * K]).view(torch.uint8).reshape(hi - lo, N, K)
+        sc = torch.from_numpy(s.to_float32().reshape(E, *reversed(scales[:2]))[lo:hi].copy())
+        return from_fp8(raw.to(self.device).view(torch.float8_e4m3fn), sc.to(self.device), (bn, bk))
 
     def vector(self, name: str, n: int) -> torch.Tensor:
         t = self.r.tensor(name)
@@ -117,7 +135,8 @@ def default_policy(arch: str, quant: str) -> Callable[[str], WFormat]:
     ``q4_k_m``: Q4_K projections, Q6_K output / half of attn_v and ffn_down (llama.cpp's recipe);
     ``q8_0``: everything Q8; ``mxfp4``: MXFP4 experts, bf16 attention, Q8 embeddings/head (gpt-oss);
     ``bf16``: everything bf16; ``exl3`` / ``exl3-<bits>``: every projection and the head as EXL3 trellis layers (4 bits per
-    weight unless said), embeddings bf16 -- the layout of an imported EXL3 checkpoint (src/loaders/hf_import.cpp:536-592).
+    weight unless said), embeddings bf16 -- the layout of an imported EXL3 checkpoint (src/loaders/hf_import.cpp:536-592); ``fp8``: projections and
+    experts e4m3 with a scale per block of 128 x 128, embeddings, head and routers bf16 -- the layout of block-quantised FP8 checkpoints.
     """
     quant = quant.lower()
     exl3_bits = 0
@@ -134,6 +153,8 @@ def default_policy(arch: str, quant: str) -> Callable[[str], WFormat]:
             return WFormat.Q8
         if quant == "exl3":
             return WFormat.BF16 if name == "token_embd.weight" else WFormat.EXL3
+        if quant == "fp8":
+            return WFormat.BF16 if name in ("token_embd.weight", "output.weight") or "ffn_gate_inp" in name else WFormat.FP8
         if quant == "mxfp4":
             if "_exps" in name:
                 return WFormat.MXFP4
@@ -197,7 +218,7 @@ class SynthSource:
                 tr, suh, svh = exl3.random_layer(N, K, getattr(self.policy, "exl3_bits", 4) or 4, self._gen(name), self.std)
                 return from_exl3(tr, suh, svh).to(self.device)
             fmt = WFormat.BF16            # expert stacks and shapes off the 128-point rotation stay dense
-        gran = {WFormat.BF16: 8, WFormat.Q8: 32, WFormat.Q4K: 256, WFormat.Q6K: 256, WFormat.MXFP4: 32}[fmt]
+        gran = {WFormat.BF16: 8, WFormat.Q8: 32, WFormat.Q4K: 256, WFormat.Q6K: 256, WFormat.MXFP4: 32, WFormat.FP8: 1}[fmt]
         if K % gran:                      # llama.cpp's fallback for ragged rows
             fmt = WFormat.Q8 if K % 32 == 0 else WFormat.BF16
         lo, hi = experts if experts is not None else (0, E)

@@ -137,7 +137,7 @@ class Linear:
             return ops.linear(x, self.w, bias=self.bias, act=self.act, act_alpha=self.act_alpha, act_limit=self.act_limit, out_f32=out_f32, out=out)
         if self.reduce and par is not None and par.enabled:
             # the bias of a row-parallel layer is added once, after the reduction
-            if par.fused is not None and x.is_cuda:
+            if par.fused is not None and x.is_cuda and self.w.fmt != WFormat.FP8:      # (no FP8 product stores into its peers' memory)
                 return par.fused.linear_all_reduce(x, self.w, self.bias)
             y = par.all_reduce(ops.linear(x, self.w, out_f32=True))
             return y if self.bias is None else y + self.bias
@@ -162,7 +162,8 @@ class MultiLinear:
 
 
 def _fuse_rows(ws: list[QuantWeight], biases: list[Optional[torch.Tensor]]):
-    if all(w.fmt == ws[0].fmt for w in ws) and ws[0].fmt != WFormat.EXL3:
+    # (FP8 matrices share scales in runs of 16 rows)
+    if all(w.fmt == ws[0].fmt for w in ws) and ws[0].fmt != WFormat.EXL3 and not (ws[0].fmt == WFormat.FP8 and any(w.N % 16 for w in ws[:-1])):
         b = None
         if any(bb is not None for bb in biases):
             b = torch.cat([bb if bb is not None else torch.zeros(w.N, device=w.device) for w, bb in zip(ws, biases)])
@@ -223,8 +224,8 @@ class AttentionBlock:
                 wv = wk                  # V is the raw K projection (src/model/gemma4.cpp:178-183,660)
             else:
                 wv = src.matrix(f"{p}.attn_v.weight", c.n_kv_heads * hd, H)
-        if c.arch == "llama" and getattr(src, "r", None) is not None and wq.fmt != WFormat.EXL3:
-            # (imported EXL3 layers keep the Hugging Face row order, which is the half-split one: src/model/dense_transformer.cpp:165-212)
+        if c.arch == "llama" and getattr(src, "r", None) is not None and wq.fmt not in (WFormat.EXL3, WFormat.FP8):
+            # (imported EXL3 and FP8 layers keep the Hugging Face row order, which is the half-split one: src/model/dense_transformer.cpp:165-212)
             wq, wk = unpermute_llama_qk(wq, c.n_heads, hd), unpermute_llama_qk(wk, c.n_kv_heads, hd)
         has_bias = c.arch in ("qwen2", "gpt-oss") and src.has(f"{p}.attn_q.bias")
         bq = src.vector(f"{p}.attn_q.bias", c.n_heads * q_rows_per_head) if has_bias else None
@@ -781,7 +782,7 @@ class MoEFFN:
                 from ..ops.cuda import CombineDelta
                 return CombineDelta(y, self._arange[key].pair_to_packed, w)
             out = ops.moe_combine(y, self._arange[key], w)
-        elif T <= self.group_gemv_max_tokens and T * self.K <= 8 * local:
+        elif T <= self.group_gemv_max_tokens and T * self.K <= 8 * local and self.gate_up.fmt != WFormat.FP8:
             # expert-major GEMV over a compact packing: every local expert streams its weights once against all of its rows (token
             # rows are read in place through the packing's index: no gather, no tile padding).  Measured slower than the grouped
             # tensor-core GEMM for gpt-oss-120b at 64 concurrent sequences (75 vs 61 ms per step), so it is off by default.
@@ -790,6 +791,17 @@ class MoEFFN:
             y = ops.expert_group_gemv(a, self.down, pk, bias=self.down_bias, e_lo=self.e_lo)
             if fuse_push:
                 return par.fused.moe_combine_push(y, pk.pair_to_packed, w)
+            out = ops.moe_combine(y, pk, w)
+        elif self.gate_up.fmt == WFormat.FP8:
+            # rows sorted by expert without padding; the token rows are rounded as they are gathered
+            pk = ops.moe_pack(idx, self.E, self.e_lo, self.e_hi, tile=1)
+            a = ops.expert_linear(h, self.gate_up, pk, x_index=pk.packed_token, bias=self.gu_bias, act=self.act, e_lo=self.e_lo)
+            y = ops.expert_linear(a, self.down, pk, bias=self.down_bias, e_lo=self.e_lo)
+            if fuse_push:
+                return par.fused.moe_combine_push(y, pk.pair_to_packed, w)
+            if self._lazy(h):
+                from ..ops.cuda import CombineDelta
+                return CombineDelta(y, pk.pair_to_packed, w)
             out = ops.moe_combine(y, pk, w)
         else:
             pk = ops.moe_pack(idx, self.E, self.e_lo, self.e_hi)
@@ -1053,6 +1065,8 @@ class TransformerModel:
         if sc is None or par.fused is None or state is not None or self.tap is not None or fb.want_hidden or type(self) is not TransformerModel:
             return False
         if not sc.can_shard(fb.T) or fb.T < self.SHARD_MIN_TOKENS:
+            return False
+        if any(L["attn"].o.w.fmt == WFormat.FP8 for L in self.layers):      # (the gathered products take the other formats)
             return False
         return all(("moe" not in L) or (L["moe"].mx is not None and L["moe"].shared is None and not L["moe"].expert_tp and L["moe"]._spill is None)
                    for L in self.layers)
