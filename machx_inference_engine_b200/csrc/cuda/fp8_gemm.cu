@@ -2,23 +2,19 @@
 //   y[m, n] = act(sum_b sx[b][m] sw[n / 16][b] sum_{k in b} x8[m][k] w8[n][k] + bias[n])
 // for dense layers and for rows sorted by expert.
 //
-// A block of K is one stage: 128 rows of x and 128 of w in every CTA, 128 bytes each, and four tcgen05.mma of K = 32.  Its sums have a scale of their own, so they
-// cannot stay in TMEM: sixteen warps read each block's sums and add s_x s_w times them to fp32 sums in registers, a quarter of the columns per thread, while the
+// A block of K is one stage: 128 rows of x and BN of w, 128 bytes each, and four tcgen05.mma of K = 32.  Its sums have a scale of their own, so they cannot
+// stay in TMEM: eight warps read each block's 128 x BN sums and add s_x s_w times them to fp32 sums in registers, BN / 2 columns of a row per thread, while the
 // tensor cores fill the next accumulator.
-// What bounds it is the way from L2 to shared memory, about 60 bytes a cycle and SM: 128 x 128 tiles want 32 KB for 256 cycles of products, and take 540; so does a
-// block of 128 x 256 tiles, 48 KB for 512 cycles: 860.  Hence tiles of 256 x 256 on pairs of SMs (tcgen05.mma.cta_group::2): each CTA loads 128 rows of x and half of the 256 rows
-// of w, 32 KB for 512 cycles.  One SM with 128 x 128 is left for products that have no 256 rows or too few tiles.
-//   warp 0      TMA loads into a ring of NST stages (of a pair: the bytes of both CTAs are counted on the first one's barrier)
-//   warp 1      tcgen05.mma from one thread (of a pair: of the first CTA) into a ring of 512 / BN accumulators
+//   warp 0      TMA loads into a ring of NST stages
+//   warp 1      tcgen05.mma from one thread into a ring of 512 / BN accumulators
 //   warps 2, 3  asynchronous copies of the block's scales (128 of the rows, BN / 16 of the weights) into a ring.  Loads into registers would be waited for one block
 //               ahead at most, whatever the distance: they share the counters by which a warp waits
-//   warps 4-19  sums (warp & 3: rows, warp / 4: quarter of the columns); a finished tile goes through shared memory, so that rows are written in runs
+//   warps 4-11  sums (warp & 3: rows, warp / 8: half of the columns); a finished tile goes through shared memory, so that rows are written in runs of 64 bytes
 // A dense product with fewer tiles than SMs is cut along K: the pieces of a tile leave fp32 sums, and the warp that arrives last adds them in the order of the pieces.
 // Every mbarrier wait is bounded.
 #include "act.cuh"
 #include "common.cuh"
 #include "fp8.cuh"
-#include "cluster.cuh"
 #include "host_util.h"
 
 namespace mx {
@@ -28,20 +24,17 @@ constexpr int FG_BM = 128, FG_SUMS = 16, FG_THREADS = 128 + 32 * FG_SUMS, FG_MAX
 // 4096 x 28672 x 4096 under the power cap: groups of 4, 8, 16 and all 32 m-tiles 643, 595, 586 and 572 us
 __host__ __device__ inline int fg_group(int kb) { return kb >= 256 ? 8 : 2048 / kb; }
 
-// BN = 256: a pair of CTAs has a tile of 256 x 256; BN = 128: a CTA one of 128 x 128
 template <int BN, bool F32> struct Fp8GemmShape {
-  static constexpr bool PAIR = BN == 256;
-  static constexpr int BM = PAIR ? 256 : 128, CTAS = PAIR ? 2 : 1;
-  static constexpr int A = FG_BM * FP8_BLOCK, STAGE = 2 * A;
-  static constexpr int ROW = F32 ? 128 : 64;               // bytes of a staged row of a warp's outputs
+  static constexpr int A = FG_BM * FP8_BLOCK, B = BN * FP8_BLOCK, STAGE = A + B;
+  static constexpr int ROW = BN == 128 && !F32 ? 64 : 128; // bytes of a staged row of a warp's outputs
   static constexpr int OUT = FG_SUMS * 32 * ROW;
-  static constexpr int NST = F32 ? 4 : 5;
+  static constexpr int NST = BN == 256 ? 3 : F32 ? 4 : 5;
   static constexpr int ACC = 512 / BN;
   // A slot of scales is free again when the products of the block NST before are done, since they waited for the sums of the block ACC before them.
   static constexpr int RING = NST + ACC, SC = FG_BM + BN / FP8_ROWS;
   struct Small {                                           // what is not tiles, behind them
     alignas(16) float scale[RING][SC];
-    uint64_t bar[2 * NST + 2 * ACC + RING];
+    uint64_t bar[2 * NST + 2 * ACC];
     int sum[FG_THREADS / 32];
     uint32_t tmem;
     int abort;
@@ -51,39 +44,10 @@ template <int BN, bool F32> struct Fp8GemmShape {
   static_assert(SMEM <= 227 * 1024, "shared memory of a block");
 };
 
-__device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ void mbar_arrive_at(uint32_t bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
-// loads whose bytes are counted on a barrier of the pair's first CTA; none is multicast
-__device__ __forceinline__ void pair_load_2d(uint32_t dst, const void* tmap, uint32_t bar, int x, int y) {
-  asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-               ::"r"(dst), "l"(tmap), "r"(bar), "r"(x), "r"(y) : "memory");
-}
-__device__ __forceinline__ void pair_load_3d(uint32_t dst, const void* tmap, uint32_t bar, int x, int y, int z) {
-  asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-               ::"r"(dst), "l"(tmap), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
-}
-__device__ __forceinline__ void pair_e4m3(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-      "@q tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n"
-      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader)
-      : "memory");
-}
-__device__ __forceinline__ void pair_commit_if(uint32_t leader, uint32_t bar) {            // the barrier at this offset in both CTAs
-  asm volatile(
-      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
-      "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}\n"
-      ::"r"(bar), "h"((uint16_t)3), "r"(leader)
-      : "memory");
-}
-
 // KIND: 0 no activation, 1 gated, 2 element-wise.  The tile's end runs once per tile and is bound by fetching its instructions, so each instance has what it needs only.
 template <int BN, int KIND, bool F32>
-__device__ __forceinline__ void fp8_gemm_body(const CUtensorMap& tm_x, const CUtensorMap& tm_w, const Fp8Params& p) {
+__global__ void __launch_bounds__(FG_THREADS, 1)
+fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, const Fp8Params p) {
   using S = Fp8GemmShape<BN, F32>;
   constexpr int NST = S::NST, ACC = S::ACC;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -99,38 +63,27 @@ __device__ __forceinline__ void fp8_gemm_body(const CUtensorMap& tm_x, const CUt
     return;
   }
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int rank = S::PAIR ? (int)cluster_rank() : 0;
-  const uint32_t bar_full = smem_u32(s_bar), bar_empty = bar_full + 8 * NST, bar_tfull = bar_empty + 8 * NST, bar_tempty = bar_tfull + 8 * ACC, bar_scale = bar_tempty + 8 * ACC;
+  const uint32_t bar_full = smem_u32(s_bar), bar_empty = bar_full + 8 * NST, bar_tfull = bar_empty + 8 * NST, bar_tempty = bar_tfull + 8 * ACC;
   volatile int* abort_flag = &s_abort;
   if (tid == 0) {
-    for (int s = 0; s < NST; ++s) { mbar_init(bar_full + 8 * s, 1); mbar_init(bar_empty + 8 * s, 1); }
-    for (int a = 0; a < ACC; ++a) { mbar_init(bar_tfull + 8 * a, 1); mbar_init(bar_tempty + 8 * a, FG_SUMS * S::CTAS); }
-    for (int r = 0; r < S::RING; ++r) mbar_init(bar_scale + 8 * r, 64);
+    for (int s = 0; s < NST; ++s) { mbar_init(bar_full + 8 * s, 1 + 64); mbar_init(bar_empty + 8 * s, 1); }
+    for (int a = 0; a < ACC; ++a) { mbar_init(bar_tfull + 8 * a, 2); mbar_init(bar_tempty + 8 * a, FG_SUMS); }
     s_abort = 0;
     fence_mbar_init();
   }
   // tensor memory is taken when the launch before has ended: it may still want some, and would wait for a CTA that waits for it
   pdl_wait();
-  if (warp == 1) {
-    if constexpr (S::PAIR) {
-      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)) : "memory");
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-    } else {
-      tmem_alloc(smem_u32(&s_tmem), 512);
-      tmem_relinquish();
-    }
-    pdl_launch_dependents();
-  }
+  if (warp == 1) { tmem_alloc(smem_u32(&s_tmem), 512); tmem_relinquish(); pdl_launch_dependents(); }
 
   // ---- tiles: dense in bands of m-tiles; experts one after the other, their m-tiles under each column of tiles
   const bool banked = p.counts != nullptr;
   const int n_tiles = (p.N + BN - 1) / BN;
-  int m_tiles = (p.M + S::BM - 1) / S::BM;
+  int m_tiles = (p.M + FG_BM - 1) / FG_BM;
   if (banked) {
     int run = 0;
     for (int e0 = 0; e0 < p.E; e0 += FG_THREADS) {
       const int e = e0 + tid;
-      int incl = e < p.E ? (p.counts[e] + S::BM - 1) / S::BM : 0;
+      int incl = e < p.E ? (p.counts[e] + FG_BM - 1) / FG_BM : 0;
       const int mine = incl;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -153,12 +106,10 @@ __device__ __forceinline__ void fp8_gemm_body(const CUtensorMap& tm_x, const CUt
   }
   tc_fence_before();
   __syncthreads();
-  if constexpr (S::PAIR) cluster_sync_all();               // (the other CTA's barriers are there before anything arrives at them)
   tc_fence_after();
   const uint32_t tmem = s_tmem;
   const int cuts = p.cuts, tiles = m_tiles * n_tiles * cuts, sw_groups = (p.N + FP8_ROWS - 1) / FP8_ROWS;
-  // a tile: this CTA's rows of it, how many there are, its column of tiles and its blocks of K
-  struct Tile { int e, row0, rows, nt, k0, k1; };
+  struct Tile { int e, row0, rows, nt, k0, k1; };        // and its blocks of K
   auto tile = [&](int t) {
     Tile r;
     const int piece = cuts > 1 ? t % cuts : 0;
@@ -175,50 +126,41 @@ __device__ __forceinline__ void fp8_gemm_body(const CUtensorMap& tm_x, const CUt
       r.e = lo;
       r.nt = i / mt;
       const int m = i - r.nt * mt;
-      const int at = m * S::BM + rank * FG_BM;
-      r.row0 = p.seg[lo] + at;
-      r.rows = r.row0 < 0 ? 0 : min(min(FG_BM, p.counts[lo] - at), p.M - r.row0);
+      r.row0 = p.seg[lo] + m * FG_BM;
+      r.rows = r.row0 < 0 ? 0 : min(min(FG_BM, p.counts[lo] - m * FG_BM), p.M - r.row0);
     } else {
-      const int band = min(max(1, fg_group(p.kb) / (S::BM / FG_BM)), m_tiles), full = band * n_tiles, g = t / full, i = t - g * full, gm = min(band, m_tiles - g * band);
+      const int band = min(fg_group(p.kb), m_tiles), full = band * n_tiles, g = t / full, i = t - g * full, gm = min(band, m_tiles - g * band);
       r.e = 0;
       r.nt = i / gm;
-      r.row0 = (g * band + i - r.nt * gm) * S::BM + rank * FG_BM;
+      r.row0 = (g * band + i - r.nt * gm) * FG_BM;
       r.rows = min(FG_BM, p.M - r.row0);
     }
     return r;
   };
 
-  const int first = S::PAIR ? blockIdx.x >> 1 : blockIdx.x, step = S::PAIR ? gridDim.x >> 1 : gridDim.x;
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
     if (warp == 0 && lane == 0) {
       prefetch_tmap(&tm_x); prefetch_tmap(&tm_w);
       uint32_t s = 0, ph = 1;
       bool ok = true;
-      for (int t = first; t < tiles && ok; t += step) {
+      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
         const Tile at = tile(t);
         for (int k = at.k0; k < at.k1; ++k) {
           if (!(ok = mbar_wait(bar_empty + 8 * s, ph, p.status, ERR_MBAR_TIMEOUT_PRODUCER, abort_flag))) break;
           const uint32_t dst = base + s * S::STAGE;
-          if (rank == 0) mbar_expect_tx(bar_full + 8 * s, S::CTAS * S::STAGE);
-          const int col = at.nt * BN + rank * FG_BM;
-          if constexpr (S::PAIR) {
-            const uint32_t full = map_to_rank(bar_full + 8 * s, 0);
-            pair_load_2d(dst, &tm_x, full, k * (FP8_BLOCK / 2), at.row0);
-            pair_load_3d(dst + S::A, &tm_w, full, k * (FP8_BLOCK / 2), col, at.e);
-          } else {
-            tma_load_2d(dst, &tm_x, bar_full + 8 * s, k * (FP8_BLOCK / 2), at.row0);
-            tma_load_3d(dst + S::A, &tm_w, bar_full + 8 * s, k * (FP8_BLOCK / 2), col, at.e);
-          }
+          mbar_expect_tx(bar_full + 8 * s, S::STAGE);
+          tma_load_2d(dst, &tm_x, bar_full + 8 * s, k * (FP8_BLOCK / 2), at.row0);
+          tma_load_3d(dst + S::A, &tm_w, bar_full + 8 * s, k * (FP8_BLOCK / 2), at.nt * BN, at.e);
           if (++s == NST) { s = 0; ph ^= 1; }
         }
       }
-    } else if (warp == 1 && rank == 0) {
+    } else if (warp == 1) {
       const uint32_t leader = elect_one();
-      constexpr uint32_t idesc = umma_idesc_e4m3(S::BM, BN);
+      constexpr uint32_t idesc = umma_idesc_e4m3(FG_BM, BN);
       uint32_t s = 0, ph = 0, a = 0, aph = 1;
       bool ok = true, data = false, room = false;
-      for (int t = first; t < tiles && ok; t += step) {
+      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
         const int piece = cuts > 1 ? t % cuts : 0, n = (int)((long long)p.kb * (piece + 1) / cuts) - (int)((long long)p.kb * piece / cuts);
         for (int k = 0; k < n; ++k) {
           if (!room && !(ok = mbar_wait(bar_tempty + 8 * a, aph, p.status, ERR_MBAR_TIMEOUT_MMA, abort_flag))) break;
@@ -232,23 +174,16 @@ __device__ __forceinline__ void fp8_gemm_body(const CUtensorMap& tm_x, const CUt
           data = mbar_peek(bar_full + 8 * s, ph);
           room = mbar_peek(bar_tempty + 8 * a, aph);
 #pragma unroll
-          for (int kk = 0; kk < FP8_BLOCK / 32; ++kk) {
-            if constexpr (S::PAIR) pair_e4m3(leader, d, dx + 2 * kk, dw + 2 * kk, idesc, kk != 0);
-            else umma_e4m3(leader, d, dx + 2 * kk, dw + 2 * kk, idesc, kk != 0);
-          }
-          if constexpr (S::PAIR) {
-            pair_commit_if(leader, empty);
-            pair_commit_if(leader, tfull);
-          } else {
-            umma_commit_if(leader, empty);
-            umma_commit_if(leader, tfull);
-          }
+          for (int kk = 0; kk < FP8_BLOCK / 32; ++kk) umma_e4m3(leader, d, dx + 2 * kk, dw + 2 * kk, idesc, kk != 0);
+          umma_commit_if(leader, empty);
+          mbar_arrive_if(leader, tfull);                   // (what this thread has seen arrive, the scales among it, is seen by who waits here)
+          umma_commit_if(leader, tfull);
         }
       }
     } else if (warp >= 2) {
       uint32_t s = 0, ph = 1, r = 0;
       bool ok = true;
-      for (int t = first; t < tiles && ok; t += step) {
+      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
         const Tile at = tile(t);
         // warp 2: rows lane, lane + 32, ..; warp 3: runs of 16 weight rows.  What lies past the matrix has a neighbour's scale
         const float* from[4];
@@ -267,7 +202,7 @@ __device__ __forceinline__ void fp8_gemm_body(const CUtensorMap& tm_x, const CUt
           } else if (lane < BN / FP8_ROWS) {
             copy4(to + 4 * FG_BM, from[0] + k);
           }
-          arrive_copies(bar_scale + 8 * r);
+          arrive_copies(bar_full + 8 * s);
           if (++s == NST) { s = 0; ph ^= 1; }
           if (++r == S::RING) r = 0;
         }
@@ -288,16 +223,15 @@ __device__ __forceinline__ void fp8_gemm_body(const CUtensorMap& tm_x, const CUt
     auto turn = [](int r) { return S::ROW == 128 ? r & 7 : r >> 1 & 3; };
     const int on = KIND == 1 ? p.N >> 1 : p.N;
     const bool wide = (((uintptr_t)p.C) & 15) == 0 && (p.ldc * ESZ) % 16 == 0;
-    uint32_t a = 0, aph = 0, ring = 0, rph = 0;
+    uint32_t a = 0, aph = 0, ring = 0;
     bool ok = true;
-    for (int t = first; t < tiles && ok; t += step) {
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
       const Tile at = tile(t);
       const int mine = q * 32 + lane, col0 = at.nt * BN + part * HC;
       float2 acc[HC / 2];
 #pragma unroll
       for (int j = 0; j < HC / 2; ++j) acc[j] = make_float2(0.f, 0.f);
       for (int k = at.k0; k < at.k1; ++k) {
-        if (!(ok = mbar_wait(bar_scale + 8 * ring, rph, p.status, ERR_MBAR_TIMEOUT_EPILOGUE, abort_flag))) break;
         if (!(ok = mbar_wait(bar_tfull + 8 * a, aph, p.status, ERR_MBAR_TIMEOUT_EPILOGUE, abort_flag))) break;
         tc_fence_after();
         const float sx = small.scale[ring][mine];
@@ -313,10 +247,7 @@ __device__ __forceinline__ void fp8_gemm_body(const CUtensorMap& tm_x, const CUt
           if (g + 2 == G) {
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) {
-              if constexpr (S::PAIR) mbar_arrive_at(map_to_rank(bar_tempty + 8 * a, 0));
-              else mbar_arrive(bar_tempty + 8 * a);
-            }
+            if (lane == 0) mbar_arrive(bar_tempty + 8 * a);
           }
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
@@ -325,14 +256,13 @@ __device__ __forceinline__ void fp8_gemm_body(const CUtensorMap& tm_x, const CUt
           }
         }
         if (++a == ACC) { a = 0; aph ^= 1; }
-        if (++ring == S::RING) { ring = 0; rph ^= 1; }
+        if (++ring == S::RING) ring = 0;
       }
       if (!ok) break;
 
       if (cuts > 1) {
         const int w = warp - 4, own = t / cuts;
-        auto slab = [&](int piece) { return reinterpret_cast<float4*>(p.part) + ((size_t)((own * cuts + piece) * S::CTAS + rank) * FG_SUMS + w) * (HC / 4 * 32) + lane; };
-        int* const ticket = p.tickets + (own * S::CTAS + rank) * FG_SUMS + w;
+        auto slab = [&](int piece) { return reinterpret_cast<float4*>(p.part) + ((size_t)(own * cuts + piece) * FG_SUMS + w) * (HC / 4 * 32) + lane; };
         float4* to = slab(t - own * cuts);
 #pragma unroll
         for (int j = 0; j < HC / 4; ++j) to[j * 32] = make_float4(acc[2 * j].x, acc[2 * j].y, acc[2 * j + 1].x, acc[2 * j + 1].y);
@@ -340,8 +270,8 @@ __device__ __forceinline__ void fp8_gemm_body(const CUtensorMap& tm_x, const CUt
         __syncwarp();
         int prev = 0;
         if (lane == 0) {
-          prev = atomicAdd(ticket, 1);
-          if (prev == cuts - 1) *ticket = 0;
+          prev = atomicAdd(p.tickets + own * FG_SUMS + w, 1);
+          if (prev == cuts - 1) p.tickets[own * FG_SUMS + w] = 0;
         }
         if (__shfl_sync(0xffffffffu, prev, 0) != cuts - 1) continue;
         __threadfence();
@@ -415,49 +345,12 @@ __device__ __forceinline__ void fp8_gemm_body(const CUtensorMap& tm_x, const CUt
     for (int i = 0; i < 200; ++i) __nanosleep(1000);
   tc_fence_before();
   __syncthreads();
-  if constexpr (S::PAIR) {
-    cluster_sync_all();                                    // the pair's loads, products and arrivals use both CTAs' memory
-    if (warp == 1) { tc_fence_after(); asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory"); }
-  } else {
-    if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem, 512); }
-  }
+  if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem, 512); }
 }
 
-template <int KIND, bool F32> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FG_THREADS, 1)
-fp8_gemm_pair(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, const Fp8Params p) {
-  fp8_gemm_body<256, KIND, F32>(tm_x, tm_w, p);
-}
-template <int KIND, bool F32> __global__ void __launch_bounds__(FG_THREADS, 1)
-fp8_gemm_one(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, const Fp8Params p) {
-  fp8_gemm_body<128, KIND, F32>(tm_x, tm_w, p);
-}
-
-template <int KIND, bool F32> static int launch_pair(const CUtensorMap& tx, const CUtensorMap& tw, const Fp8Params& p, long long tiles, cudaStream_t st) {
-  using S = Fp8GemmShape<256, F32>;
-  auto kern = fp8_gemm_pair<KIND, F32>;
-  static std::atomic<int> clusters[64];
-  const int dev = DeviceOnce::ordinal();
-  int most = clusters[dev].load(std::memory_order_acquire);
-  if (!most) {                                             // clusters that are resident at once (a GPC's odd SM has no partner)
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
-    if (e != cudaSuccess) return (int)e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(sm_count() / 2 * 2); cfg.blockDim = dim3(FG_THREADS); cfg.dynamicSmemBytes = S::SMEM;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = 2; at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at; cfg.numAttrs = 1;
-    e = cudaOccupancyMaxActiveClusters(&most, kern, &cfg);
-    if (e != cudaSuccess) return (int)e;
-    if (most < 1) return -116;
-    clusters[dev].store(most, std::memory_order_release);
-  }
-  launch_pdl(kern, dim3(2 * (unsigned)(tiles < most ? tiles : most)), dim3(FG_THREADS), S::SMEM, st, tx, tw, p);
-  return (int)cudaGetLastError();
-}
-template <int KIND, bool F32> static int launch_one(const CUtensorMap& tx, const CUtensorMap& tw, const Fp8Params& p, long long tiles, cudaStream_t st) {
-  using S = Fp8GemmShape<128, F32>;
-  auto kern = fp8_gemm_one<KIND, F32>;
+template <int BN, int KIND, bool F32> static int launch_gemm(const CUtensorMap& tx, const CUtensorMap& tw, const Fp8Params& p, long long tiles, cudaStream_t st) {
+  using S = Fp8GemmShape<BN, F32>;
+  auto kern = fp8_gemm_kernel<BN, KIND, F32>;
   static DeviceOnce configured;
   if (configured.pending()) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
@@ -468,25 +361,24 @@ template <int KIND, bool F32> static int launch_one(const CUtensorMap& tx, const
   return (int)cudaGetLastError();
 }
 
-// Dense (M rows) or experts (counts / seg: from the bank's first expert on; M rows of the packing), tiles of bn x bn = 128 or 256; dense ones in `cuts` pieces along K.
+// Dense (M rows) or experts (counts / seg: from the bank's first expert on; M rows of the packing), tiles of bn = 128 or 256 columns; dense ones in `cuts` pieces along K.
 int fp8_gemm_launch(const Fp8Call& c, cudaStream_t st) {
   Fp8Params p = fp8_params(c);
   p.cuts = c.cuts > 1 ? c.cuts : 1;
-  const int bn = c.bn, ctas = bn == 256 ? 2 : 1;            // (a tile is as high as it is wide)
-  if (c.E > FG_MAX_E || c.slot || (bn != 128 && bn != 256) || (c.counts && (c.M + bn - 1) / bn + c.E > 65535)) return -106;
+  const int bn = c.bn;
+  if (c.E > FG_MAX_E || c.slot || (bn != 128 && bn != 256) || (c.counts && (c.M + FG_BM - 1) / FG_BM + c.E > 65535)) return -106;
   if (((uintptr_t)c.codes | (uintptr_t)c.w) & 15) return -114;
-  const long long tiles = ((c.M + bn - 1) / bn + (c.counts ? (c.E < c.M ? c.E : c.M) : 0)) * (long long)((c.N + bn - 1) / bn);
+  const long long tiles = ((c.M + FG_BM - 1) / FG_BM + (c.counts ? (c.E < c.M ? c.E : c.M) : 0)) * (long long)((c.N + bn - 1) / bn);
   if (tiles >= 1ll << 31) return -106;
-  if (p.cuts > 1 && (c.counts || p.cuts > p.kb || tiles * ctas * FG_SUMS > CUT_TICKETS || tiles * p.cuts > FG_MAX_PIECES || !c.scratch || !c.tickets || ((uintptr_t)c.scratch & 15)))
-    return -106;
+  if (p.cuts > 1 && (c.counts || p.cuts > p.kb || tiles * FG_SUMS > CUT_TICKETS || tiles * p.cuts > FG_MAX_PIECES || !c.scratch || !c.tickets || ((uintptr_t)c.scratch & 15))) return -106;
   CUtensorMap tx, tw;
   int r = fp8_tmap(&tx, c.codes, p.kb, c.rows, 0, FG_BM);
-  if (!r) r = fp8_tmap(&tw, c.w, p.kb, p.N, c.E, FG_BM);
+  if (!r) r = fp8_tmap(&tw, c.w, p.kb, p.N, c.E, bn);
   if (r) return r;
   const int kind = p.act == 0 ? 0 : act_gated(p.act) ? 1 : 2;
-#define MX_FG(KIND_, F32_) if (kind == KIND_ && (p.out_f32 != 0) == F32_) return bn == 256 ? launch_pair<KIND_, F32_>(tx, tw, p, tiles * p.cuts, st) : launch_one<KIND_, F32_>(tx, tw, p, tiles * p.cuts, st)
-  MX_FG(0, false); MX_FG(1, false); MX_FG(2, false);
-  MX_FG(0, true); MX_FG(1, true); MX_FG(2, true);
+#define MX_FG(BN_, KIND_) if (bn == BN_ && kind == KIND_) return p.out_f32 ? launch_gemm<BN_, KIND_, true>(tx, tw, p, tiles * p.cuts, st) : launch_gemm<BN_, KIND_, false>(tx, tw, p, tiles * p.cuts, st)
+  MX_FG(256, 0); MX_FG(256, 1); MX_FG(256, 2);
+  MX_FG(128, 0); MX_FG(128, 1); MX_FG(128, 2);
 #undef MX_FG
   return -106;
 }
@@ -496,7 +388,7 @@ int fp8_gemm_launch(const Fp8Call& c, cudaStream_t st) {
 using namespace mx;
 
 // Bytes of scratch (16-byte aligned) that `pieces` pieces of tiles of bn columns want.
-MX_HOST_API long long mx_fp8_tile_scratch(int pieces, int bn) { return 4ll * pieces * bn * bn; }
+MX_HOST_API long long mx_fp8_tile_scratch(int pieces, int bn) { return 4ll * pieces * FG_BM * bn; }
 
 MX_HOST_API int mx_fp8_call_bytes() { return (int)sizeof(Fp8Call); }
 

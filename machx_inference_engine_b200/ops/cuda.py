@@ -938,7 +938,7 @@ def _fp8_call(x, w: QuantWeight, out, bias, row_scale, act, act_alpha, act_limit
     if nt or cuts > 1:
         tickets = _tickets(dev)
         counters, kept = tickets[0].data_ptr(), tickets[3]
-        work = _fp8_scratch_bytes(nt) if nt else lib.mx_fp8_tile_scratch(-(-out.shape[0] // bn) * -(-w.N // bn) * cuts, bn)
+        work = _fp8_scratch_bytes(nt) if nt else lib.mx_fp8_tile_scratch(-(-out.shape[0] // 128) * -(-w.N // bn) * cuts, bn)
         if kept is None:
             scratch = torch.empty(work, dtype=torch.uint8, device=dev)
         else:
