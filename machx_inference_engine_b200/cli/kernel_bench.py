@@ -194,7 +194,7 @@ def main(argv=None):
     GRAPH_REPS = a.graph_reps
     exl3_bits = int(a.fmt[5:]) if a.fmt.startswith("exl3-") else (4 if a.fmt == "exl3" else 0)
     fmt = WFormat.EXL3 if exl3_bits else {"bf16": WFormat.BF16, "q8": WFormat.Q8, "q4k": WFormat.Q4K, "q6k": WFormat.Q6K, "mxfp4": WFormat.MXFP4,
-                                          "mxf4t": WFormat.MXFP4}[a.fmt]
+                                          "mxf4t": WFormat.MXFP4, "fp8": WFormat.FP8}[a.fmt]
     torch.manual_seed(0)
 
     def weight(N, Kd, E=1):
@@ -215,7 +215,7 @@ def main(argv=None):
         i = [0]
 
         def fn():
-            if a.decode_once:         # the model's `linear`: quantised weight decoded once to bf16, then the TMA-fed kernel
+            if a.decode_once or a.fmt == "fp8":         # the model's `linear`: quantised weight decoded once to bf16, then the TMA-fed kernel; FP8: rows rounded, 8-bit product
                 K.linear(x, ws[i[0] % a.layers])
             else:                     # the tcgen05 kernel with in-kernel weight decode
                 K.gemm(x, ws[i[0] % a.layers], bn=a.bn or None)
@@ -267,6 +267,15 @@ def main(argv=None):
         dn = weight(H, F, E)
         x = torch.randn(T, H, device=dev).to(torch.bfloat16)
         idx, w = K.moe_route(torch.randn(T, E, device=dev), None, k)
+        if a.fmt == "fp8":
+            pk = K.moe_pack(idx, E, tile=1)
+            gate_up = lambda: K.expert_linear(x, gu, pk, x_index=pk.packed_token, act=ref.ACT_SWIGLU_OAI)
+            hmid = gate_up()
+            med, mn = timeit(gate_up, a.iters)
+            report(f"moe gate_up[fp8] T={T} E={E} top{k} {2 * F}x{H}", med, mn, flops=2.0 * T * k * 2 * F * H, bytes_=gu.nbytes)
+            med, mn = timeit(lambda: K.expert_linear(hmid, dn, pk), a.iters)
+            report(f"moe down[fp8] T={T} E={E} top{k} {H}x{F}", med, mn, flops=2.0 * T * k * F * H, bytes_=dn.nbytes)
+            return 0
         pk = K.moe_pack(idx, E)
         f16 = False
         mid = torch.float16 if f16 else torch.bfloat16

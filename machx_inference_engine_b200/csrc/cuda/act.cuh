@@ -39,7 +39,7 @@ __device__ __forceinline__ float gelu_tanh(float z) {
   return z * sigmoid_f<false>(2.f * u);
 }
 __device__ __forceinline__ float relu2(float z) {
-  const float m = fmaxf(z, 0.f);
+  const float m = z < 0.f ? 0.f : z;                       // (a NaN stays one)
   return m * m;
 }
 

@@ -95,6 +95,8 @@ def check_packing(pk, w: QuantWeight, x, x_index, e_lo: int) -> None:
     if pk.counts is None or pk.seg_start is None or pk.max_rows != max(pk.pair_to_packed.numel(), 1):
         raise ValueError("expert_linear takes a compact packing: moe_pack(..., tile=1)")
     E = pk.counts.numel()
+    if w.E > 1024:
+        raise ValueError(f"expert_linear: a bank of {w.E} experts; 1024 are taken")
     if pk.seg_start.numel() != E + 1 or e_lo < 0 or e_lo + w.E > E:
         raise ValueError(f"expert_linear: experts {e_lo} to {e_lo + w.E} of a packing of {E}")
     for t, n in ((pk.counts, E), (pk.seg_start, E + 1)):
@@ -113,6 +115,8 @@ def check_slots(x, w: QuantWeight, slot_expert, x_div: int, bias, act_gated: boo
     """Arguments of :func:`ops.expert_gemv` with an FP8 bank."""
     S = slot_expert.numel()
     check_product(x, w, True, S, bias, act_gated, "expert_gemv")
+    if S >= 1 << 16:
+        raise ValueError(f"expert_gemv: {S} slots; expert_linear takes that many rows")
     if slot_expert.dtype != torch.int32 or not slot_expert.is_contiguous() or slot_expert.device != x.device:
         raise ValueError("expert_gemv: the slots' experts are contiguous int32 on the rows' device")
     if x_div < 1 or x.shape[0] < -(-S // x_div):

@@ -66,6 +66,12 @@ def test_rows_of_odd_strides_and_through_an_index():
     assert ops.fp8_rows(wide[:0]).codes.shape == (0, 1024) and ops.fp8_rows(wide, index=index[:0].to(DEV)).scale.shape == (8, 0)
 
 
+def test_an_index_into_no_rows():
+    none = torch.empty(0, 256, dtype=torch.bfloat16, device=DEV)
+    q = ops.fp8_rows(none, index=torch.tensor([-1, 0, 5], dtype=torch.int32, device=DEV))
+    assert q.scale.isnan().any(0).tolist() == [False, True, True] and float(q.codes.float().abs().max()) == 0
+
+
 def test_rows_at_the_edges_of_the_range():
     inf, nan = float("inf"), float("nan")
     rows = [torch.zeros(256), torch.full((256,), 448.0), torch.full((256,), 449.0), torch.full((256,), 3e38), torch.full((256,), 1e-38), torch.full((256,), -1e-45),
@@ -202,6 +208,9 @@ def test_a_row_that_is_not_finite_stays_alone(M):
     rows[0] |= M > 2
     assert bool(got[rows].isnan().all()) and torch.equal(got[~rows], clean[~rows])
     assert float(ops.linear(torch.zeros_like(x), w).abs().max()) == 0
+    for act in ("swiglu", "swiglu_oai", "geglu", "relu2"):
+        got = ops.linear(bad, w, act=ACTS[act])
+        assert bool(got[rows].isnan().all()) and not bool(got[~rows].isnan().any()), act
 
 
 def test_scales_of_any_size():
@@ -303,7 +312,38 @@ def test_slots_of_experts_elsewhere_are_zero():
     assert torch.equal(got[:3], alone) and float(got[3:].abs().max()) == 0
 
 
+def test_no_tokens_and_no_rows():
+    w, bank3 = bank(64, 256), bank(64, 256, 3)
+    none = torch.empty(0, 256, dtype=torch.bfloat16, device=DEV)
+    assert ops.linear(none, w).shape == (0, 64) and ops.linear(ops.fp8_rows(none), w, act=ops.ACT_SWIGLU).shape == (0, 32)
+    assert ops.expert_gemv(none, bank3, torch.empty(0, dtype=torch.int32, device=DEV), x_div=2).shape == (0, 64)
+    # experts without a token, and a packing whose tokens are all elsewhere
+    idx = torch.tensor([[2], [2], [2]], dtype=torch.int32, device=DEV)
+    pk = ops.moe_pack(idx, 3, 0, 2, tile=1)
+    assert int((pk.pair_to_packed >= 0).sum()) == 0
+    ops.expert_linear(acts(3, 256), bank3.slice_experts(0, 2), pk, x_index=pk.packed_token)
+    torch.cuda.synchronize()
+
+
 # ------------------------------------------------------------------ streams and graphs
+def test_a_stream_of_its_own_and_captured_twice():
+    """Graphs that were captured one after the other and replayed at once; another stream than the tensors' own; the same row many times."""
+    x, w = acts(5, 2048), bank(4096, 2048)
+    want = ops.linear(x, w)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        assert torch.equal(ops.linear(x, w), want)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            a = ops.linear(x, w)
+            b = ops.linear(x[:1].expand(40, 2048), w)
+        x.copy_(x.flip(0))
+        g.replay()
+    side.synchronize()
+    assert torch.equal(a, want.flip(0)) and torch.equal(b, ops.linear(x[:1].expand(40, 2048).contiguous(), w))
+
+
 def test_two_streams_and_a_graph_share_nothing():
     cases = [(1, 6144, 1024), (12, 1024, 4096), (70, 640, 2048), (300, 1024, 512)]
     xs, ws = [acts(M, K) for M, N, K in cases], [bank(N, K) for M, N, K in cases]
