@@ -216,6 +216,14 @@ inline Fp8Params fp8_params(const Fp8Call& c) {
   return p;
 }
 
+// One more arrival at a counter that the pieces of cut work share: what the warp has written before is seen by who counts later, and the other way round.  The fence is
+// the atomic's own, of the one lane that comes here; __threadfence() by every lane costs a sequentially consistent one each.
+__device__ __forceinline__ int arrive_at(int* counter) {
+  int before;
+  asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+  return before;
+}
+
 // Boxes of `rows` rows by one block of codes [E][n][kb * 128] (E = 0: [n][kb * 128]).  Codes travel as two-byte elements: the tile is bytes either way.
 inline int fp8_tmap(CUtensorMap* out, const void* codes, int kb, int n, int E, int rows) {
   const uint64_t row = (uint64_t)kb * FP8_BLOCK;
