@@ -17,6 +17,12 @@ __device__ __forceinline__ float2 cluster_ld2(uint32_t addr, uint32_t rank) {
   asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(remote) : "memory");
   return v;
 }
+// one float to the same address in CTA `rank`
+__device__ __forceinline__ void cluster_st(uint32_t addr, uint32_t rank, float v) {
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"(v) : "memory");
+}
 
 // a channel pair as it was loaded: converted where it is used, so that the loads of the next tile stay in flight
 template <typename T> struct RawPair;

@@ -158,9 +158,11 @@ __device__ __forceinline__ void arrive_copies(uint32_t bar) { asm volatile("cp.a
 
 // What a product multiplies and writes.
 struct Fp8Params {
-  const __nv_bfloat16* xb;   // rows that the streaming kernel rounds itself, `ldx` elements apart, of K
+  const __nv_bfloat16* xb;   // rows that a kernel rounds itself, `ldx` elements apart, of K
   long long ldx;
   int K;
+  const uint8_t* xc;         // rounded rows, and [E][N][kb * 128] of weights, of the kernel that reads them without boxes
+  const uint8_t* w;
   const float* sx;           // [kb][x_rows]
   int x_rows;
   const float* sw;           // [E][ceil(N / 16)][kb]
@@ -205,6 +207,9 @@ struct Fp8Call {
   int unused;
 };
 int fp8_rows_launch(const void* x, int f32, long long ldx, const int* index, int x_rows, int rows, int K, void* codes, float* scale, cudaStream_t st);
+bool fp8_gemv_takes(const Fp8Call& c);
+bool fp8_gemv_rounds(const Fp8Call& c);
+int fp8_gemv_launch(const Fp8Call& c, bool round, cudaStream_t st);
 bool fp8_stream_rounds(const Fp8Call& c);
 int fp8_stream_launch(const Fp8Call& c, bool round, cudaStream_t st);
 int fp8_gemm_launch(const Fp8Call& c, cudaStream_t st);

@@ -403,11 +403,12 @@ MX_HOST_API int mx_fp8_product(const Fp8Call* call, cudaStream_t st) {
   if (c.M <= 0 || c.N <= 0) return 0;
   if (c.K < 1 || c.x_div < 1 || c.E < 1 || c.rows < 1) return -101;
   if (act_gated(c.act) && c.N % 32) return -104;
-  const bool round = fp8_stream_rounds(c);
+  const bool gemv = fp8_gemv_takes(c), round = gemv ? fp8_gemv_rounds(c) : fp8_stream_rounds(c);
   if (c.xb && !round) {
     if (!c.codes) return -130;
     const int r = fp8_rows_launch(c.xb, 0, c.ldx, c.index, c.xb_rows, c.rows, c.K, c.codes, c.scale, st);
     if (r) return r;
   }
+  if (gemv) return fp8_gemv_launch(c, round, st);
   return c.nt ? fp8_stream_launch(c, round, st) : fp8_gemm_launch(c, st);
 }

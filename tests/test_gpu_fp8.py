@@ -388,3 +388,60 @@ def test_a_layer_of_experts_from_router_to_sum():
         return ops.moe_combine(ops.expert_linear(a, dn.to(dev), pk), pk, wt)
 
     assert O.rel(layer(DEV), layer("cpu")) < 2.0 ** -8 + 2.0 ** -8
+
+
+# ------------------------------------------------------------------ few rows of small layers: blocks of K shared by clusters
+@pytest.mark.parametrize("rows", [1, 2, 3, 5, 8])
+@pytest.mark.parametrize("N,K", [(64, 1160), (32, 9000), (1024, 8192), (2080, 2944), (4096, 4096), (8192, 4096), (8224, 4096), (640, 14336), (50, 1025), (30000, 256)])
+def test_few_rows(rows, N, K):
+    x, w, bias, scale = acts(rows, K), bank(N, K), torch.randn(N, generator=gen(N)).to(DEV), torch.rand(rows, generator=gen(rows)).to(DEV)
+    y = O.row_values(x) @ O.weight_values(w)[0].T
+    got = ops.linear(x, w, out_f32=True)
+    assert O.rel(got, y) < tolerance(K)
+    want = torch.relu(y + bias.cpu().double()) ** 2 * scale.cpu().double()[:, None]
+    assert O.rel(ops.linear(x, w, bias=bias, act=ACTS["relu2"], row_scale=scale, out_f32=True), want) < tolerance(K, "relu2")
+    if N % 32 == 0:
+        assert O.rel(ops.linear(x, w, act=ACTS["swiglu"], out_f32=True), O.activate(y, "swiglu")) < tolerance(K, "swiglu")
+    wide = torch.full((rows, K + 3), float("nan"), dtype=torch.bfloat16, device=DEV)
+    wide[:, 1:K + 1] = x                                                           # rows of odd alignment are rounded by a launch before
+    assert torch.equal(ops.linear(wide[:, 1:K + 1], w, out_f32=True), got) and torch.equal(ops.linear(ops.fp8_rows(x), w, out_f32=True), got)
+    out = torch.full((rows, N + 5), 7.0, device=DEV)
+    ops.linear(x, w, out_f32=True, out=out[:, 2:N + 2])
+    assert torch.equal(out[:, 2:N + 2], got) and bool((out[:, :2] == 7).all()) and bool((out[:, N + 2:] == 7).all())
+
+
+@pytest.mark.parametrize("N,K", [(96, 1160), (1024, 8192)])
+def test_few_rows_with_nan_and_infinity(N, K):
+    x, w = acts(4, K), bank(N, K)
+    clean = ops.linear(x, w, out_f32=True)
+    x[1, K - 1], x[3, 5] = float("nan"), float("inf")
+    got = ops.linear(x, w, out_f32=True)
+    assert torch.equal(got[[0, 2]], clean[[0, 2]]) and bool(got[[1, 3]].isnan().all())
+
+
+def test_a_chain_of_few_rows_replays_like_eager_calls():
+    """Each launch starts before the one before has ended; what it reads of that one it reads after it."""
+    ws = [bank(4096, 1024, seed=1), bank(1024, 4096, seed=2), bank(640, 1024, seed=3), bank(1024, 640, seed=4)]
+    x = acts(3, 1024)
+
+    def chain():
+        h = x
+        for w in ws:
+            h = ops.linear(h, w)
+        return h
+
+    want = chain()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            got = chain()
+        for _ in range(20):
+            got.zero_()
+            g.replay()
+            assert torch.equal(got, want)
+        x.copy_(x.flip(0))
+        g.replay()
+    side.synchronize()
+    assert torch.equal(got, want.flip(0))
