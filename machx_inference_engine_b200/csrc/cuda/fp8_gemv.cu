@@ -7,8 +7,8 @@
 // global memory to registers in the layout of mma.m16n8k32: a lane's 16 bytes are four consecutive k of four steps, the rows' codes in shared memory are read the same way, and the
 // order of k within a block is free.  (On B200 these products take a tenth of the time: tcgen05 has them faster, but its accumulators come back through two more waits.)  Every
 // CTA rounds the blocks of the rows that it needs itself.  The first weights are on their way to L2 before the launch before has ended.
-// Measured in a graph of calls, us, with the streaming kernel in brackets: 1 x 512 x 2048 3.2 (5.6), 1 x 1024 x 8192 5.0 (9.5), 1 x 4096 x 4096 5.7 (7.7), 1 x 6144 x 4096 8.9
-// (9.8); gated slots, 10 of 512 of 1024 x 2048, 8.3 (9.3).
+// Measured in a graph of calls, us, with the streaming kernel in brackets: 1 x 512 x 2048 3.0 (5.7), 1 x 1024 x 8192 5.0 (9.3), 1 x 5120 x 2880 6.3 (9.7), 1 x 12288 x 2048 7.9
+// (9.7); gated slots, 10 of 512 of 1024 x 2048, 7.8 (9.2).
 #include "act.cuh"
 #include "cluster.cuh"
 #include "common.cuh"
@@ -34,7 +34,6 @@ __global__ void __launch_bounds__(FV_THREADS, FV_CTAS) fp8_gemv_kernel(const Fp8
   extern __shared__ __align__(16) uint8_t smem_raw[];
   __shared__ __align__(16) float s_red[FV_WARPS][MT * 16][FV_ROWS];
   __shared__ float s_join[FV_MAX_CUTS - 1][MT][FV_THREADS];
-  pdl_launch_dependents();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   const int cuts = p.cuts, cut = cuts > 1 ? (int)cluster_rank() : 0, it = cuts > 1 ? blockIdx.x / cuts : blockIdx.x;
   const int first = (int)((long long)p.kb * cut / cuts), end = (int)((long long)p.kb * (cut + 1) / cuts), blocks = end - first;
@@ -145,6 +144,8 @@ __global__ void __launch_bounds__(FV_THREADS, FV_CTAS) fp8_gemv_kernel(const Fp8
     }
   }
 
+  pdl_launch_dependents();                                                       // (earlier, the next layers' CTAs wait where this one's loads are wanted)
+
   // ---- the warps' sums, joined in their order, then those of the cluster's CTAs in theirs, and the epilogue: a thread has row r of each run and row m of x
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt)
@@ -193,11 +194,12 @@ __global__ void __launch_bounds__(FV_THREADS, FV_CTAS) fp8_gemv_kernel(const Fp8
   }
 }
 
-// Pieces along K and bytes of rounded rows; no cuts: left to the streaming kernel, which has the memory busier once it runs.  us, that -> this one: 1 x 4096 x 4096 7.7 -> 5.7, 1 x
-// 8192 x 4096 10.8 -> 9.5, but 1 x 10240 x 4096 11.2 -> 13.3: up to 8192 items of a block.  With more rows the rounding that every CTA does again counts: 8 x 1024 x 8192 9.8 -> 7.5,
-// 2 x 8192 x 4096 10.7 -> 10.1, but 4 x 6144 x 4096 9.9 -> 11.2, 4 x 2048 x 14336 10.3 -> 11.5: up to twice as many for all rows together.  CTAs past a wave: slots, 10 x
-// 2048 x 512 (640 CTAs of 592 at a time) 8.3 -> 6.9, 16 x 2048 x 768 (1024) 6.5 -> 9.5.  Pieces are powers of two and leave an eighth of the SMs' room: clusters of three that
-// would have filled it (576 CTAs) waited for a place and took twice the time.
+// Pieces along K and bytes of rounded rows; no cuts: left to the streaming kernel, which has the memory busier once it runs.  In a model's chain of launches that kernel fills its
+// rings with weights under the launch before, so long rows want a smaller limit than calls in a loop show.  Decode of one token, ms with the streaming kernel -> with these
+// limits: Qwen3-MoE-30B's shape 3.64 -> 3.12, Qwen3-Next's 4.75 -> 3.98, gpt-oss-20b's 2.71 -> 2.58; Llama-3-8B's (K = 4096, layers of 4096 blocks and up) 2.95 -> 3.21 if it
+// took them, so it does not.  With more rows the rounding that every CTA does again counts, us: 4 x 5120 x 2880 10.3 -> 7.8, 8 x 1024 x 8192 9.8 -> 7.5, but 4 x 6144 x 4096 9.9 ->
+// 11.2, 4 x 2048 x 14336 10.3 -> 11.5.  CTAs past a wave: slots, 10 x 2048 x 512 (640 CTAs, 592 at a time) 8.2 -> 6.8, 16 x 2048 x 768 (1024) 6.5 -> 9.5.  Pieces are powers of two
+// and leave an eighth of the SMs' room: clusters of three that would have filled it (576 CTAs) waited for a place and took twice the time.
 struct GemvPlan { int cuts, smem; long long items; };
 static GemvPlan gemv_plan(const Fp8Call& c) {
   GemvPlan g{};
@@ -205,7 +207,8 @@ static GemvPlan gemv_plan(const Fp8Call& c) {
   const int kb = (c.K + FP8_BLOCK - 1) / FP8_BLOCK, rows = c.slot ? 1 : c.M;
   const long long wave = (long long)FV_CTAS * sm_count();
   g.items = (c.slot ? (long long)c.M : 1) * ((c.N + 16 * MT - 1) / (16 * MT));
-  if (g.items * kb > 8192 || rows * g.items * kb > 2 * 8192 || 4 * g.items > 5 * wave) return g;
+  const long long most = c.slot || kb <= 24 ? 8192 : 3000;
+  if (g.items * kb > most || rows * g.items * kb > 2 * 8192 || 4 * g.items > 5 * wave) return g;
   int cuts = 1;
   while (cuts < FV_MAX_CUTS && 16 * cuts * g.items <= 7 * wave && 2 * cuts * FV_WARPS <= kb) cuts *= 2;
   const int blocks = (kb + cuts - 1) / cuts;
