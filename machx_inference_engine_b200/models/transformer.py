@@ -224,9 +224,9 @@ class AttentionBlock:
                 wv = wk                  # V is the raw K projection (src/model/gemma4.cpp:178-183,660)
             else:
                 wv = src.matrix(f"{p}.attn_v.weight", c.n_kv_heads * hd, H)
-        if c.arch == "llama" and getattr(src, "r", None) is not None and wq.fmt not in (WFormat.EXL3, WFormat.FP8):
-            # (imported EXL3 and FP8 layers keep the Hugging Face row order, which is the half-split one: src/model/dense_transformer.cpp:165-212)
-            wq, wk = unpermute_llama_qk(wq, c.n_heads, hd), unpermute_llama_qk(wk, c.n_kv_heads, hd)
+        if c.arch == "llama" and getattr(src, "r", None) is not None and wq.fmt != WFormat.EXL3:
+            # (imported EXL3 layers and FP8 matrices keep the Hugging Face row order, which is the half-split one: src/model/dense_transformer.cpp:165-212)
+            wq, wk = (w if w.fmt == WFormat.FP8 else unpermute_llama_qk(w, n, hd) for w, n in ((wq, c.n_heads), (wk, c.n_kv_heads)))
         has_bias = c.arch in ("qwen2", "gpt-oss") and src.has(f"{p}.attn_q.bias")
         bq = src.vector(f"{p}.attn_q.bias", c.n_heads * q_rows_per_head) if has_bias else None
         bk = src.vector(f"{p}.attn_k.bias", c.n_kv_heads * hd) if has_bias else None

@@ -45,7 +45,7 @@ def test_matrices_and_experts_of_a_file(tmp_path):
         src.matrix("blk.0.ffn_up_exps.weight", cfg.expert_ffn + 1, cfg.hidden, cfg.n_experts)
 
 
-def hf_directory(d, block=(128, 128), scheme="dynamic"):
+def hf_directory(d, block=(128, 128), scheme="dynamic", kept=()):
     rng = np.random.default_rng(0)
     H, F, L, V, nh, nkv, hd = 256, 384, 2, 320, 4, 2, 64
     json.dump({"model_type": "llama", "architectures": ["LlamaForCausalLM"], "hidden_size": H, "intermediate_size": F, "num_hidden_layers": L, "num_attention_heads": nh,
@@ -55,6 +55,10 @@ def hf_directory(d, block=(128, 128), scheme="dynamic"):
     tensors, dense = {}, {}
 
     def lin(name, n, k):
+        if name.split(".")[-1] in kept:                      # a matrix that was left out of the quantisation
+            w = rng.standard_normal((n, k)).astype(np.float16) * np.float16(0.02)
+            tensors[name + ".weight"], dense[name] = w, torch.from_numpy(w.astype(np.float32))
+            return
         codes = (torch.from_numpy(rng.standard_normal((n, k))).clamp(-4, 4) * 112).to(torch.float8_e4m3fn)
         s = (rng.random((-(-n // 128), -(-k // 128))).astype(np.float32) + 0.5) * np.float32(0.02 / 112)
         tensors[name + ".weight"] = ("F8_E4M3", codes.view(torch.uint8).numpy())
@@ -89,10 +93,26 @@ def test_import_keeps_the_codes(tmp_path):
         w = src.matrix(f"blk.{i}.{gg}.weight", *want.shape)
         assert w.fmt == WFormat.FP8 and torch.equal(w.dequantize()[0], want)
     eng = Engine.load(out, "cpu", EngineOptions(max_ctx=256, max_seqs=1))
-    q = eng.engine.model.layers[0]["attn"].qkv.w if hasattr(eng, "engine") else None
-    if q is not None:                                        # rows in the Hugging Face order: rotated in halves as they are
-        assert torch.equal(q.dequantize()[0][:256], dense["model.layers.0.self_attn.q_proj"])
+    q = eng.model.layers[0]["attn"].qkv.w                    # rows in the Hugging Face order: rotated in halves as they are
+    assert torch.equal(q.dequantize()[0][:256], dense["model.layers.0.self_attn.q_proj"])
     assert eng.generate("hello", SamplingParams(max_tokens=4, temperature=0.0)).completion_tokens >= 1
+
+
+@pytest.mark.parametrize("kept", ["q_proj", "k_proj"])
+def test_queries_and_keys_of_two_kinds_keep_one_row_order(tmp_path, kept):
+    """The matrices that a file stores without quantisation are in the interleaved order of llama files, the e4m3 ones in halves: each is read as what it is."""
+    dense = hf_directory(str(tmp_path), kept=(kept,))
+    out = str(tmp_path / "out.gguf")
+    import_to_gguf(str(tmp_path), out, log=lambda s: None)
+    model = Engine.load(out, "cpu", EngineOptions(max_ctx=256, max_seqs=1)).model
+    x = torch.randn(5, 256, generator=torch.Generator().manual_seed(0)).to(torch.bfloat16)
+    got = model.layers[0]["attn"].qkv(x).float()
+    for lo, name in ((0, "q_proj"), (256, "k_proj")):
+        w = dense[f"model.layers.0.self_attn.{name}"]
+        want = x.float() @ w.t()
+        have = got[:, lo:lo + w.shape[0]]
+        # 2^-4 for codes of the rows, 2^-8 for the output and the file's 8-bit type of the kept matrix: another row order has nothing in common with it (error sqrt(2))
+        assert float((have - want).norm() / want.norm()) < 0.1
 
 
 def test_refusals_of_import(tmp_path):
