@@ -38,21 +38,23 @@ __device__ __forceinline__ float gelu_tanh(float z) {
   if constexpr (PRECISE) return 0.5f * z * (1.f + tanhf(u));
   return z * sigmoid_f<false>(2.f * u);
 }
+// KEEP_NAN: a NaN stays one (a maximum drops it)
+template <bool KEEP_NAN = false>
 __device__ __forceinline__ float relu2(float z) {
-  const float m = z < 0.f ? 0.f : z;                       // (a NaN stays one)
+  const float m = KEEP_NAN ? (z < 0.f ? 0.f : z) : fmaxf(z, 0.f);
   return m * m;
 }
 
-template <bool PRECISE>
+template <bool PRECISE, bool KEEP_NAN = false>
 __device__ __forceinline__ float act_unary(int act, float z, float a, float b) {
   if (act == ACT_CODE_XIELU) return xielu<PRECISE>(z, a, b);
   if (act == ACT_CODE_GELU_TANH) return gelu_tanh<PRECISE>(z);
   if (act == ACT_CODE_TANH) return tanhf(z);
-  return act == ACT_CODE_RELU2 ? relu2(z) : z;
+  return act == ACT_CODE_RELU2 ? relu2<KEEP_NAN>(z) : z;
 }
 
 // the same over a run of values: one branch for the run
-template <bool PRECISE, int N>
+template <bool PRECISE, bool KEEP_NAN = false, int N>
 __device__ __forceinline__ void act_unary_run(int act, float (&v)[N], float a, float b) {
   if (act == ACT_CODE_XIELU) {
 #pragma unroll
@@ -62,7 +64,7 @@ __device__ __forceinline__ void act_unary_run(int act, float (&v)[N], float a, f
     for (int j = 0; j < N; ++j) v[j] = gelu_tanh<PRECISE>(v[j]);
   } else if (act == ACT_CODE_RELU2) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = relu2(v[j]);
+    for (int j = 0; j < N; ++j) v[j] = relu2<KEEP_NAN>(v[j]);
   } else if (act == ACT_CODE_TANH) {
 #pragma unroll
     for (int j = 0; j < N; ++j) v[j] = tanhf(v[j]);

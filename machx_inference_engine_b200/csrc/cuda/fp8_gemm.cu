@@ -312,7 +312,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
             for (int j = 0; j < 32; ++j) v[j] += __ldg(bias + min(col0 + c0 + j, p.N - 1));
           }
           if constexpr (KIND == 1) glu_run<16>(p.act, v, p.act_alpha, p.act_limit);
-          if constexpr (KIND == 2) act_unary_run<false>(p.act, v, p.act_alpha, p.act_limit);
+          if constexpr (KIND == 2) act_unary_run<false, true>(p.act, v, p.act_alpha, p.act_limit);
           constexpr int n = 2 * PIECE;
 #pragma unroll
           for (int j = 0; j < n; j += 16 / ESZ) {

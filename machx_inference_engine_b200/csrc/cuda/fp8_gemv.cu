@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(FV_THREADS, FV_CTAS) fp8_gemv_kernel(const Fp8
   for (int mt = 0; mt < MT; ++mt) {
     if (gated && mt) break;
     float y = v[mt];
-    if (!gated && p.act) y = act_unary<false>(p.act, y, p.act_alpha, p.act_limit);
+    if (!gated && p.act) y = act_unary<false, true>(p.act, y, p.act_alpha, p.act_limit);
     if (p.row_scale) y *= scale;
     if (!owned) y = 0.f;
     const int o = (gated ? n0 / 2 : n0 + mt * 16) + r;

@@ -353,7 +353,7 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] = pair[j];
           } else if (p.act) {
-            act_unary_run<false>(p.act, v, p.act_alpha, p.act_limit);
+            act_unary_run<false, true>(p.act, v, p.act_alpha, p.act_limit);
           }
           if (p.row_scale) {
 #pragma unroll
