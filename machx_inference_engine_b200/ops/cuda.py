@@ -928,17 +928,37 @@ def _fp8_scratch_bytes(nt: int) -> int:
     return _fp8_entry().mx_fp8_stream_scratch(nt)
 
 
+FP8_KEPT = 4 << 20      # bytes of rounded rows that are kept from one call for the next
+_fp8_own = threading.local()
+
+
+def _fp8_room(n: int, dev, stream: int):
+    """``n`` bytes for rounded rows between the two launches of a call.  An allocation takes as much of the host's time as a launch, so up to 4 MB each thread keeps what its calls on a
+    stream share: they follow one another (another thread's may come between the rounding and the product).  Past that, and under capture, an allocation, stream-ordered."""
+    if n > FP8_KEPT or torch.cuda.is_current_stream_capturing():
+        return torch.empty(n, dtype=torch.uint8, device=dev)
+    own = _fp8_own.__dict__
+    t = own.get((dev.index, stream))
+    if t is None or t.numel() < n:
+        if len(own) > STREAM_TICKETS_MAX:
+            own.clear()
+        t = own[dev.index, stream] = torch.empty(n, dtype=torch.uint8, device=dev)
+    return t
+
+
 def _fp8_call(x, w: QuantWeight, out, bias, row_scale, act, act_alpha, act_limit, nt=0, bn=0, cuts=1, counts=None, seg=None, slot=None, x_div=1, e_lo=0, index=None):
     """One product on the current device: ``nt`` rows of a group (csrc/cuda/fp8_stream.cu) or ``bn`` columns of a tile in ``cuts`` pieces along K (csrc/cuda/fp8_gemm.cu).  bf16 rows that the kernel does
-    not round itself are rounded into a scratch buffer first, by the same call: an ordinary allocation, stream-ordered and of the graph's own pool under capture.  Partial sums
-    go to memory that a stream's launches share, since they follow one another, and under capture to an allocation as well."""
+    not round itself are rounded into a scratch buffer first, by the same call.  Partial sums go to memory that a stream's launches share, since they follow one another, and under
+    capture to an allocation of the graph's own pool."""
     lib = _fp8_entry()
     dev = out.device
+    M = out.shape[0]
+    stream = torch._C._cuda_getCurrentRawStream(dev.index)
     part = counters = 0
     if nt or cuts > 1:
         tickets = _tickets(dev)
         counters, kept = tickets[0].data_ptr(), tickets[3]
-        work = _fp8_scratch_bytes(nt) if nt else lib.mx_fp8_tile_scratch(-(-out.shape[0] // 128) * -(-w.N // bn) * cuts, bn)
+        work = _fp8_scratch_bytes(nt) if nt else lib.mx_fp8_tile_scratch(-(-M // 128) * -(-w.N // bn) * cuts, bn)
         if kept is None:
             scratch = torch.empty(work, dtype=torch.uint8, device=dev)
         else:
@@ -950,18 +970,18 @@ def _fp8_call(x, w: QuantWeight, out, bias, row_scale, act, act_alpha, act_limit
         rows, xb, ldx, xb_rows, codes, scale = x.codes.shape[0], 0, 0, 0, x.codes.data_ptr(), x.scale.data_ptr()
     else:
         xb, ldx, xb_rows, codes, scale = x.data_ptr(), x.stride(0), x.shape[0], 0, 0
-        rows = xb_rows if index is None else index.numel()
-    rc = _FP8_WANTS_ROOM if xb and (nt != 16 or counts is not None) else None
+        rows = xb_rows if index is None else M
+    rc = _FP8_WANTS_ROOM if xb and (nt != 16 or counts is not None or (slot is None and M > 8)) else None      # (what the kernels round themselves: at most this)
     while rc is None or rc == _FP8_WANTS_ROOM:
         if rc is not None:                   # (no launch has been made)
             n = rows * -(-w.K // _fp8.FP8_BLOCK)
-            rounded = torch.empty(n * (_fp8.FP8_BLOCK + 4), dtype=torch.uint8, device=dev)
+            rounded = _fp8_room(n * (_fp8.FP8_BLOCK + 4), dev, stream)
             codes = rounded.data_ptr()
             scale = codes + n * _fp8.FP8_BLOCK
         call = _FP8_CALL.pack(xb, ldx, _ptr(index), codes, scale, w.p0.data_ptr(), w.p1.data_ptr(), out.data_ptr(), out.stride(0), _ptr(bias), _ptr(row_scale), _ptr(counts),
-                              _ptr(seg), _ptr(slot), part, counters, xb_rows, rows, out.shape[0], w.N, w.K, w.E, out.dtype == torch.float32, act, x_div, e_lo, nt, bn, cuts, act_alpha,
+                              _ptr(seg), _ptr(slot), part, counters, xb_rows, rows, M, w.N, w.K, w.E, out.dtype == torch.float32, act, x_div, e_lo, nt, bn, cuts, act_alpha,
                               act_limit, 0)
-        rc = lib.mx_fp8_product(call, torch._C._cuda_getCurrentRawStream(dev.index))
+        rc = lib.mx_fp8_product(call, stream)
     _check(rc, "fp8 product")
     _count()
     return out
@@ -1045,7 +1065,7 @@ def expert_linear(x, w: QuantWeight, pk: MoePacking, x_index=None, bias=None, ac
     _fp8.check_product(x, w, True, P, bias, gated, "expert_linear")
     _fp8.check_packing(pk, w, x, x_index, e_lo)
     return _fp8_product(x, w, (P, w.N // 2 if gated else w.N), torch.float32 if out_f32 else torch.bfloat16, None, bias, None, act, act_alpha, act_limit,
-                        counts=pk.counts[e_lo:] if e_lo else pk.counts, seg=pk.seg_start[e_lo:] if e_lo else pk.seg_start, index=None if x_index is None else x_index[:P])
+                        counts=pk.counts[e_lo:] if e_lo else pk.counts, seg=pk.seg_start[e_lo:] if e_lo else pk.seg_start, index=x_index)
 
 
 # ------------------------------------------------------------------ attention

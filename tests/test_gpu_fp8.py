@@ -373,6 +373,27 @@ def test_two_streams_and_a_graph_share_nothing():
         assert all(torch.equal(a, b) for a, b in zip(r, want))
 
 
+def test_threads_on_one_stream_do_not_share_rounded_rows():
+    """Calls of several threads on the same stream: launches of one may come between the two of another."""
+    import threading
+    cases = [(12, 512, 640), (40, 512, 640), (200, 256, 640), (12, 512, 640)]
+    xs, ws = [acts(M, K, seed=i) for i, (M, N, K) in enumerate(cases)], [bank(N, K, seed=i) for i, (M, N, K) in enumerate(cases)]
+    want = [ops.linear(x, w) for x, w in zip(xs, ws)]
+    wrong = []
+
+    def run(i):
+        for _ in range(150):
+            if not torch.equal(ops.linear(xs[i], ws[i]), want[i]):
+                wrong.append(i)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(len(cases))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
 def test_a_layer_of_experts_from_router_to_sum():
     """Route, pack, gate / up, down and sum as a model runs them, against the same steps on the CPU.  The hidden rows are rounded to bf16 and then to e4m3 in
     both; where the two differ by a bf16 step (2^-8) a code may differ by one e4m3 step, 2^-3 of the value.  A hidden value sits so near a border with a
