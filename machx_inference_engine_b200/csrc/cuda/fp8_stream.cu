@@ -12,8 +12,8 @@
 // The work is the list of (group of rows, 128 weight rows, block of K) laid end to end, of which every CTA takes an equal run.  A tile that is cut leaves fp32
 // partials (at most two per CTA); the warp that arrives last adds them in the order of the CTAs, so results do not depend on timing.
 // Bound: memory, and for a token the latencies of one launch.  Two CTAs share an SM: with one and 80 KB of weights under way 8 x 28672 x 4096 took 32 us.
-// Measured in a graph of calls: 8 x 28672 x 4096 gated 25.4 us (4.6 TB/s), 1 x 6144 x 4096 8.9 us, 1 x 28672 x 4096 23.8 us, 1 x 4096 x 14336 14.7 us (about five from launch to the first sums), experts of 64
-// tokens, 8 of 128 of 1536 x 2048, 62.4 us (6.4 TB/s, 0.97 of a copy's rate), slots of four tokens, 4 of 32 of 2880 x 2880, 27 us.
+// Measured in a graph of calls: 8 x 28672 x 4096 gated 25.2 us (4.7 TB/s), 1 x 6144 x 4096 8.4 us, 1 x 28672 x 4096 23.8 us, 1 x 4096 x 14336 14.9 us (about five from launch to the first sums), experts of 64
+// tokens, 8 of 128 of 1536 x 2048, 61.8 us (6.4 TB/s, 0.98 of a copy's rate), slots of four tokens, 4 of 32 of 2880 x 2880, 27 us.
 // Every mbarrier wait is bounded.
 #include "act.cuh"
 #include "common.cuh"
@@ -300,20 +300,20 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
         if (mine_to_finish) {
 #pragma unroll
           for (int j = 0; j < NT / 2; ++j) acc[j] = make_float2(0.f, 0.f);
-          // four parts of sixteen columns at a time are under way; they are added in order
-          constexpr int J = NT / 4 < 4 ? NT / 4 : 4;
+          // P parts of 4 J columns at a time are under way; they are added in order (eight for four of up to eight rows: 8 x 4096 x 14336 17.3 -> 16.9 us, 1 x 4096 x 4096 7.55 -> 7.25; twelve 16.5, 7.5)
+          constexpr int LIVE = ROUND ? 2 : NT / 4, J = LIVE < 4 ? LIVE : 4, P = ROUND ? 8 : 4;
 #pragma unroll
-          for (int j0 = 0; j0 < NT / 4; j0 += J) {
+          for (int j0 = 0; j0 < LIVE; j0 += J) {
             if (4 * j0 < at.rows) {
-              for (int c = c0; c <= c1; c += 4) {
-                float4 v[4][J];
+              for (int c = c0; c <= c1; c += P) {
+                float4 v[P][J];
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < P; ++i)
 #pragma unroll
                   for (int j = 0; j < J; ++j)
                     v[i][j] = c + i <= c1 && 4 * (j0 + j) < at.rows ? __ldcg(slab(c + i) + (j0 + j) * 32) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < P; ++i)
 #pragma unroll
                   for (int j = 0; j < J; ++j) {
                     float2& u = acc[2 * (j0 + j)];
