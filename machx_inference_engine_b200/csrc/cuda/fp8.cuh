@@ -221,12 +221,19 @@ inline Fp8Params fp8_params(const Fp8Call& c) {
   return p;
 }
 
-// One more arrival at a counter that the pieces of cut work share: what the warp has written before is seen by who counts later, and the other way round.  The fence is
-// the atomic's own, of the one lane that comes here; __threadfence() by every lane costs a sequentially consistent one each.
-__device__ __forceinline__ int arrive_at(int* counter) {
-  int before;
-  asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
-  return before;
+// A warp's arrival at a counter that the `pieces` of cut work share; true for the last, which leaves the counter at zero and may read what all of them have written.  The fence
+// is the atomic's own, of one lane (__threadfence() by every lane costs a sequentially consistent one each), so both sides go through a barrier of the warp: the lanes' writes come
+// before that lane's release, and their reads after its acquire.  The shuffle in between orders nothing.
+__device__ __forceinline__ bool warp_arrives_last(int* counter, int pieces) {
+  int before = 0;
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) {
+    asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+    if (before == pieces - 1) *counter = 0;
+  }
+  before = __shfl_sync(0xffffffffu, before, 0);
+  __syncwarp();
+  return before == pieces - 1;
 }
 
 // Boxes of `rows` rows by one block of codes [E][n][kb * 128] (E = 0: [n][kb * 128]).  Codes travel as two-byte elements: the tile is bytes either way.

@@ -272,13 +272,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant_
         float4* to = slab(t - own * cuts);
 #pragma unroll
         for (int j = 0; j < HC / 4; ++j) to[j * 32] = make_float4(acc[2 * j].x, acc[2 * j].y, acc[2 * j + 1].x, acc[2 * j + 1].y);
-        __syncwarp();
-        int prev = 0;
-        if (lane == 0) {
-          prev = arrive_at(p.tickets + own * FG_SUMS + w);
-          if (prev == cuts - 1) p.tickets[own * FG_SUMS + w] = 0;
-        }
-        if (__shfl_sync(0xffffffffu, prev, 0) != cuts - 1) continue;
+        if (!warp_arrives_last(p.tickets + own * FG_SUMS + w, cuts)) continue;
         const float4* from = slab(0);
 #pragma unroll
         for (int j = 0; j < HC / 4; ++j) {

@@ -289,14 +289,7 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
 #pragma unroll
         for (int j = 0; j < NT / 4; ++j)
           if (4 * j < at.rows) mine[j * 32] = make_float4(acc[2 * j].x, acc[2 * j].y, acc[2 * j + 1].x, acc[2 * j + 1].y);
-        __syncwarp();
-        int prev = 0;
-        if (lane == 0) {
-          prev = arrive_at(p.tickets + c0 * 4 + q);
-          if (prev == c1 - c0) p.tickets[c0 * 4 + q] = 0;
-        }
-        prev = __shfl_sync(0xffffffffu, prev, 0);
-        mine_to_finish = prev == c1 - c0;
+        mine_to_finish = warp_arrives_last(p.tickets + c0 * 4 + q, c1 - c0 + 1);
         if (mine_to_finish) {
 #pragma unroll
           for (int j = 0; j < NT / 2; ++j) acc[j] = make_float2(0.f, 0.f);
