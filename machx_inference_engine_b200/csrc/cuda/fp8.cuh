@@ -198,8 +198,9 @@ struct Fp8Call {
   const int* counts;
   const int* seg;
   const int* slot;
-  float* scratch;            // partial sums, and the counters of cut work (host_util.h)
+  float* scratch;            // partial sums, `scratch_bytes` of room, and the counters of cut work (host_util.h)
   int* tickets;
+  long long scratch_bytes;
   int xb_rows, rows;         // rows of xb, and rounded rows
   int M, N, K, E, out_f32, act, x_div, e_lo;
   int nt, bn, cuts;          // rows of a group of the streaming kernel, or 0 and the columns of a tile and its pieces along K of the tiled one

@@ -359,6 +359,9 @@ template <int BN, int KIND, bool F32> static int launch_gemm(const CUtensorMap& 
   return (int)cudaGetLastError();
 }
 
+// bytes of the sums of `pieces` pieces of tiles of bn columns
+static long long tile_scratch(long long pieces, int bn) { return 4 * pieces * FG_BM * bn; }
+
 // Dense (M rows) or experts (counts / seg: from the bank's first expert on; M rows of the packing), tiles of bn = 128 or 256 columns; dense ones in `cuts` pieces along K.
 int fp8_gemm_launch(const Fp8Call& c, cudaStream_t st) {
   Fp8Params p = fp8_params(c);
@@ -368,7 +371,8 @@ int fp8_gemm_launch(const Fp8Call& c, cudaStream_t st) {
   if (((uintptr_t)c.codes | (uintptr_t)c.w) & 15) return -114;
   const long long tiles = ((c.M + FG_BM - 1) / FG_BM + (c.counts ? (c.E < c.M ? c.E : c.M) : 0)) * (long long)((c.N + bn - 1) / bn);
   if (tiles >= 1ll << 31) return -106;
-  if (p.cuts > 1 && (c.counts || p.cuts > p.kb || tiles * FG_SUMS > CUT_TICKETS || tiles * p.cuts > FG_MAX_PIECES || !c.scratch || !c.tickets || ((uintptr_t)c.scratch & 15))) return -106;
+  if (p.cuts > 1 && (c.counts || p.cuts > p.kb || tiles * FG_SUMS > CUT_TICKETS || tiles * p.cuts > FG_MAX_PIECES || ((uintptr_t)c.scratch & 15))) return -106;
+  if (p.cuts > 1 && (!c.scratch || !c.tickets || c.scratch_bytes < tile_scratch(tiles * p.cuts, bn))) return -131;
   CUtensorMap tx, tw;
   int r = fp8_tmap(&tx, c.codes, p.kb, c.rows, 0, FG_BM);
   if (!r) r = fp8_tmap(&tw, c.w, p.kb, p.N, c.E, bn);
@@ -386,12 +390,12 @@ int fp8_gemm_launch(const Fp8Call& c, cudaStream_t st) {
 using namespace mx;
 
 // Bytes of scratch (16-byte aligned) that `pieces` pieces of tiles of bn columns want.
-MX_HOST_API long long mx_fp8_tile_scratch(int pieces, int bn) { return 4ll * pieces * FG_BM * bn; }
+MX_HOST_API long long mx_fp8_tile_scratch(int pieces, int bn) { return tile_scratch(pieces, bn); }
 
 MX_HOST_API int mx_fp8_call_bytes() { return (int)sizeof(Fp8Call); }
 
 // A product (see Fp8Call): rows that are bf16 still are rounded, then the streaming kernel (nt) or the tiled one (bn) runs.
-// -130: bf16 rows that have to be rounded first, and no room for codes; nothing was launched.
+// -130: bf16 rows that have to be rounded first, and no room for codes; nothing was launched.  -131: too little room for partial sums.
 MX_HOST_API int mx_fp8_product(const Fp8Call* call, cudaStream_t st) {
   const Fp8Call& c = *call;
   if (c.M <= 0 || c.N <= 0) return 0;

@@ -425,6 +425,8 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
   if (warp == 1) { tc_fence_after(); tmem_dealloc(s_tmem, S::TMEM); }
 }
 
+// bytes of partial sums of a launch with groups of nt rows, whatever its grid
+static long long stream_scratch(int nt) { return 4ll * FS_MAX_GRID * 2 * FS_TILE * nt; }
 static int stream_grid(int ctas) { return ctas * sm_count() < FS_MAX_GRID ? ctas * sm_count() : FS_MAX_GRID; }
 
 template <int NT, bool ROUND> static int launch_stream(const CUtensorMap& tw, const CUtensorMap& tx, const Fp8Params& p, cudaStream_t st) {
@@ -459,6 +461,7 @@ int fp8_stream_launch(const Fp8Call& c, bool round, cudaStream_t st) {
   const long long groups = c.slot ? c.M : c.counts ? (long long)c.M / nt + (c.E < c.M ? c.E : c.M) + 1 : 1;
   if (c.E > FS_MAX_E || groups >= 65536 || groups * ((p.N + FS_TILE - 1) / FS_TILE) * p.kb >= 1ll << 30 || (!c.slot && !c.counts && c.M > nt)) return -106;      // (units are counted in 32 bits)
   if (((uintptr_t)c.codes | (uintptr_t)c.w | (uintptr_t)c.scratch) & 15) return -114;
+  if (!c.scratch || !c.tickets || c.scratch_bytes < stream_scratch(nt)) return -131;
   CUtensorMap tw, tx;
   int r = fp8_tmap(&tw, c.w, p.kb, p.N, c.E, FS_TILE);
   if (r) return r;
@@ -480,4 +483,4 @@ int fp8_stream_launch(const Fp8Call& c, bool round, cudaStream_t st) {
 }  // namespace mx
 
 // Bytes of scratch (16-byte aligned) that a launch with groups of up to `nt` rows wants.
-MX_HOST_API long long mx_fp8_stream_scratch(int nt) { return 4ll * mx::FS_MAX_GRID * 2 * mx::FS_TILE * nt; }
+MX_HOST_API long long mx_fp8_stream_scratch(int nt) { return mx::stream_scratch(nt); }

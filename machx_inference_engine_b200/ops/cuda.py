@@ -883,7 +883,7 @@ def expert_gemv(x, w: QuantWeight, slot_expert, x_div=1, bias=None, act=ACT_NONE
 
 # ------------------------------------------------------------------ 8-bit floating point (see ops/fp8.py)
 FP8_STREAM_ROWS = (16, 32, 64)           # rows of a group in the weight-streaming kernel
-_FP8_CALL = struct.Struct("<16q13i2fi")   # csrc/cuda/fp8.cuh: Fp8Call
+_FP8_CALL = struct.Struct("<17q13i2fi")   # csrc/cuda/fp8.cuh: Fp8Call
 _FP8_WANTS_ROOM = -130                   # and the answer to bf16 rows without room for rounded ones, where the kernel does not round them itself
 _fp8_lib = None
 
@@ -928,6 +928,20 @@ def _fp8_scratch_bytes(nt: int) -> int:
     return _fp8_entry().mx_fp8_stream_scratch(nt)
 
 
+def _partial_sums(kept, n: int, dev):
+    """``n`` bytes at least for the partial sums of a launch, for as long as the caller holds the tensor.  ``kept``: the list in which a stream's launches keep the largest so far (None
+    under capture: an allocation of the graph's pool).  Threads share a stream's list, and one may put its tensor there while another allocates, so a call uses the tensor whose size it
+    has checked and never reads the list again; the one that is put away later is dropped if it is not larger."""
+    t = kept[0] if kept else None
+    if t is None or t.numel() < n:
+        t = torch.empty(n, dtype=torch.uint8, device=dev)
+        if kept is not None:
+            with _tickets_lock:
+                if not kept or kept[0].numel() < n:
+                    kept[:] = [t]
+    return t
+
+
 FP8_KEPT = 4 << 20      # bytes of rounded rows that are kept from one call for the next
 _fp8_own = threading.local()
 
@@ -954,18 +968,12 @@ def _fp8_call(x, w: QuantWeight, out, bias, row_scale, act, act_alpha, act_limit
     dev = out.device
     M = out.shape[0]
     stream = torch._C._cuda_getCurrentRawStream(dev.index)
-    part = counters = 0
+    part = part_bytes = counters = 0
     if nt or cuts > 1:
         tickets = _tickets(dev)
-        counters, kept = tickets[0].data_ptr(), tickets[3]
-        work = _fp8_scratch_bytes(nt) if nt else lib.mx_fp8_tile_scratch(-(-M // 128) * -(-w.N // bn) * cuts, bn)
-        if kept is None:
-            scratch = torch.empty(work, dtype=torch.uint8, device=dev)
-        else:
-            if not kept or kept[0].numel() < work:
-                kept[:] = [torch.empty(work, dtype=torch.uint8, device=dev)]
-            scratch = kept[0]
-        part = scratch.data_ptr()
+        counters = tickets[0].data_ptr()
+        scratch = _partial_sums(tickets[3], _fp8_scratch_bytes(nt) if nt else lib.mx_fp8_tile_scratch(-(-M // 128) * -(-w.N // bn) * cuts, bn), dev)
+        part, part_bytes = scratch.data_ptr(), scratch.numel()
     if isinstance(x, FP8Rows):
         rows, xb, ldx, xb_rows, codes, scale = x.codes.shape[0], 0, 0, 0, x.codes.data_ptr(), x.scale.data_ptr()
     else:
@@ -979,7 +987,7 @@ def _fp8_call(x, w: QuantWeight, out, bias, row_scale, act, act_alpha, act_limit
             codes = rounded.data_ptr()
             scale = codes + n * _fp8.FP8_BLOCK
         call = _FP8_CALL.pack(xb, ldx, _ptr(index), codes, scale, w.p0.data_ptr(), w.p1.data_ptr(), out.data_ptr(), out.stride(0), _ptr(bias), _ptr(row_scale), _ptr(counts),
-                              _ptr(seg), _ptr(slot), part, counters, xb_rows, rows, M, w.N, w.K, w.E, out.dtype == torch.float32, act, x_div, e_lo, nt, bn, cuts, act_alpha,
+                              _ptr(seg), _ptr(slot), part, counters, part_bytes, xb_rows, rows, M, w.N, w.K, w.E, out.dtype == torch.float32, act, x_div, e_lo, nt, bn, cuts, act_alpha,
                               act_limit, 0)
         rc = lib.mx_fp8_product(call, stream)
     _check(rc, "fp8 product")
