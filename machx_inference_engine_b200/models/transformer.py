@@ -567,7 +567,8 @@ class DenseFFN:
         d = src.matrix(f"{p}.ffn_down{suffix}.weight", H, F)
         if tp > 1:
             gran = max(d.k_granule(), 16)
-            if F % gran or (F // gran) < tp:
+            whole = F % gran == 0 or d.fmt == WFormat.FP8          # (FP8: the last block may be a part of one)
+            if not whole or -(-F // gran) < tp:
                 gran = 32 if F % 32 == 0 else 16          # finer than the weight's blocks: the shard is re-encoded
             lo, hi = _even_chunks(F, tp, gran)[par.rank]
             g, u, d = g.slice_rows(lo, hi), u.slice_rows(lo, hi), d.slice_k(lo, hi, requant=True)
@@ -606,13 +607,13 @@ DenseFFN.forward_gathered = _ffn_gathered
 
 
 def _even_chunks(n: int, parts: int, gran: int) -> list[tuple[int, int]]:
-    """Split n (a multiple of gran) into `parts` contiguous ranges on gran boundaries, sizes differing by <= gran."""
-    blocks = n // gran
+    """Split n into `parts` contiguous ranges on gran boundaries (the last one ends with n), sizes differing by <= gran where that divides n."""
+    blocks = -(-n // gran)
     base, extra = divmod(blocks, parts)
     out, lo = [], 0
     for r in range(parts):
         sz = (base + (1 if r < extra else 0)) * gran
-        out.append((lo, lo + sz))
+        out.append((lo, min(lo + sz, n)))
         lo += sz
     return out
 
@@ -647,7 +648,6 @@ class MoEFFN:
         if self.expert_tp:
             if F % 32 or F // 32 < ep:
                 raise ValueError(f"expert FFN width {F} cannot be cut into {ep} slices of whole 32-element blocks")
-            f_lo, f_hi = _even_chunks(F, ep, 32)[par.rank]
         rw = src.matrix(f"{p}.ffn_gate_inp.weight", E, H)
         self.router = Linear(rw if rw.fmt == ops.WFormat.BF16 else QuantWeight(**_as_bf16(rw)))
         self.router_bias = src.vector(f"{p}.ffn_gate_inp.bias", E) if with_bias else None
@@ -660,6 +660,9 @@ class MoEFFN:
             u = src.matrix(f"{p}.ffn_up_exps.weight", F, H, E, experts=rng)
         d = src.matrix(f"{p}.ffn_down_exps.weight", H, F, E, experts=rng)
         if self.expert_tp:
+            # (FP8: on its blocks, which are those that the hidden rows are rounded in, so that the ranks together compute what one would)
+            gran = d.k_granule() if d.fmt == WFormat.FP8 and -(-F // d.k_granule()) >= ep else 32
+            f_lo, f_hi = _even_chunks(F, ep, gran)[par.rank]
             g, u, d = g.slice_rows(f_lo, f_hi), u.slice_rows(f_lo, f_hi), d.slice_k(f_lo, f_hi, requant=True)
         # MXFP4 banks on a GPU run on the block-scaled tensor-core kernel: gate / up / down stay three banks in its tiled layout
         self.mx = None

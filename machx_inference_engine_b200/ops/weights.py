@@ -136,11 +136,26 @@ class QuantWeight:
         t = self.p1.index_select(1, at).reshape(self.E, groups, FP8_ROWS, -1)
         top = torch.gather(t, 2, t.abs().argmax(dim=2, keepdim=True))
         w = QuantWeight(WFormat.FP8, n, self.K, self.E, codes.view(torch.float8_e4m3fn).contiguous(), top[:, :, 0].contiguous())
-        if not torch.equal(t, top.expand_as(t)):
-            same = (t == top).reshape(self.E, groups * FP8_ROWS, -1)[:, :n].repeat_interleave(FP8_BLOCK, dim=-1)
-            ratio = torch.where(top != 0, t / top, torch.zeros_like(t)).reshape(self.E, groups * FP8_ROWS, -1)[:, :n].repeat_interleave(FP8_BLOCK, dim=-1)
-            again = (w.p0.to(torch.float32) * ratio).to(torch.float8_e4m3fn)
-            w.p0 = torch.where(same, w.p0.view(torch.uint8), again.view(torch.uint8)).view(torch.float8_e4m3fn)
+        w._rescale_fp8(t, top, lambda v: v.reshape(self.E, groups * FP8_ROWS, -1)[:, :n].repeat_interleave(FP8_BLOCK, dim=-1))
+        return w
+
+    def _rescale_fp8(self, t: torch.Tensor, top: torch.Tensor, over) -> None:
+        """Codes that have the scales ``t`` rounded again to those of the runs that they are in now, ``top``; unchanged where the two are equal.  ``over``: scales to codes."""
+        if torch.equal(t, top.expand_as(t)):
+            return
+        again = (self.p0.to(torch.float32) * over(torch.where(top != 0, t / top, torch.zeros_like(t)))).to(torch.float8_e4m3fn)
+        self.p0 = torch.where(over(t == top), self.p0.view(torch.uint8), again.view(torch.uint8)).view(torch.float8_e4m3fn)
+
+    def _slice_k_fp8(self, lo: int, hi: int) -> "QuantWeight":
+        """Columns [lo, hi) that begin or end inside a block, as FP8: a new block that lies over two old ones takes the larger scale, and the other's codes are rounded again."""
+        n = hi - lo
+        blocks = -(-n // FP8_BLOCK)
+        codes = _pad_last(self.p0.view(torch.uint8)[:, :, lo:hi], FP8_BLOCK).view(torch.float8_e4m3fn)
+        at = (lo + torch.arange(blocks * FP8_BLOCK, device=self.device).clamp_(max=n - 1)) // FP8_BLOCK
+        t = self.p1.index_select(2, at).reshape(self.E, -1, blocks, FP8_BLOCK)
+        top = torch.gather(t, 3, t.abs().argmax(dim=3, keepdim=True))
+        w = QuantWeight(WFormat.FP8, self.N, n, self.E, codes, top[..., 0].contiguous())
+        w._rescale_fp8(t, top, lambda v: v.reshape(self.E, -1, blocks * FP8_BLOCK).repeat_interleave(FP8_ROWS, dim=1)[:, :self.N])
         return w
 
     def slice_rows(self, lo: int, hi: int) -> "QuantWeight":
@@ -182,12 +197,15 @@ class QuantWeight:
     def slice_k(self, lo: int, hi: int, requant: bool = False) -> "QuantWeight":
         """Input-dimension slice [lo, hi) (row-parallel shards).  Bounds must sit on block boundaries; with
         ``requant`` a slice that cuts a block is re-encoded instead (Q8 when the slice is a multiple of 32 wide,
-        else bf16) -- the case of a 256-element super-block format sharded finer than its blocks."""
+        else bf16) -- the case of a 256-element super-block format sharded finer than its blocks.  FP8 stays FP8:
+        its products round their activations and have collectives of their own, so all ranks have to hold it or none."""
         self._no_exl3("sliced along K")
         g = self.k_granule()
         if lo % g or (hi % g and not (self.fmt == WFormat.FP8 and hi == self.K)):
             if not requant:
                 raise ValueError(f"K slice [{lo},{hi}) is not aligned to the {g}-element blocks of {self.fmt.name}")
+            if self.fmt == WFormat.FP8:
+                return self._slice_k_fp8(lo, hi)
             dense = self.dequantize(torch.float32)[:, :, lo:hi].contiguous()
             return from_dense(dense, WFormat.Q8 if (hi - lo) % 32 == 0 else WFormat.BF16)
         per_elem = {
