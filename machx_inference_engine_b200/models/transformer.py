@@ -843,6 +843,17 @@ class UnaryMoEFFN(MoEFFN):
         self.router_bias = self.gu_bias = self.down_bias = self.expert_scale = self.shared = self.mx = self._spill = None
         self.act, self.a8, self.reduce, self.group_gemv_max_tokens, self._arange = act, False, False, 0, {}
 
+    def _packed(self, idx, h, w=None, **act):
+        """Experts of pairs that are sorted by expert: (their rows, the row of each pair).  ``w``: factors of what they read.  FP8 banks take the pairs without padding and
+        round a token's row as they gather it."""
+        if self.gate_up.fmt == WFormat.FP8:
+            pk = ops.moe_pack(idx, self.E, tile=1)
+            x, at = (h, pk.packed_token) if w is None else (ops.moe_scale_rows(h, w, pk), None)
+            return ops.expert_linear(ops.expert_linear(x, self.gate_up, pk, x_index=at, **act), self.down, pk), pk.pair_to_packed
+        pk = ops.moe_pack(idx, self.E)
+        a = ops.grouped_linear(ops.moe_gather(h, pk) if w is None else ops.moe_scale_rows(h, w, pk), self.gate_up, pk.tile_expert, pk.num_tiles, **act)
+        return ops.grouped_linear(a, self.down, pk.tile_expert, pk.num_tiles), pk.pair_to_packed
+
 
 class ScaledInputMoEFFN(UnaryMoEFFN):
     """Gated experts without biases, of which each token uses the best K by router score; the weight -- the sigmoid of the chosen score, as it is --
@@ -868,10 +879,7 @@ class ScaledInputMoEFFN(UnaryMoEFFN):
                 self._arange[T, h.device] = torch.arange(T * K, dtype=torch.int32, device=h.device)
             pos = self._arange[T, h.device]
         else:
-            pk = ops.moe_pack(idx, self.E)
-            a = ops.grouped_linear(ops.moe_scale_rows(h, w, pk), self.gate_up, pk.tile_expert, pk.num_tiles, act=self.act)
-            y = ops.grouped_linear(a, self.down, pk.tile_expert, pk.num_tiles)
-            pos = pk.pair_to_packed
+            y, pos = self._packed(idx, h, w, act=self.act)
         return ops.ExpertSum(y, pos, K, None if self.shared is None else self.shared(h))
 
 
@@ -914,10 +922,7 @@ class ClampedMoEFFN(UnaryMoEFFN):
                 self._arange[T, h.device] = torch.arange(T * K, dtype=torch.int32, device=h.device)
             pos = self._arange[T, h.device]
         else:
-            pk = ops.moe_pack(idx, self.E)
-            a = ops.grouped_linear(ops.moe_gather(h, pk), self.gate_up, pk.tile_expert, pk.num_tiles, **self.act_kw)
-            y = ops.grouped_linear(a, self.down, pk.tile_expert, pk.num_tiles)
-            pos = pk.pair_to_packed
+            y, pos = self._packed(idx, h, **self.act_kw)
         if self.shared is None:
             return ops.ExpertSum(y, pos, K, w=w)
         return ops.ExpertSum(y, pos, K, self.shared(h), w, z[:, self.E])
