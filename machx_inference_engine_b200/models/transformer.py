@@ -618,6 +618,13 @@ def _even_chunks(n: int, parts: int, gran: int) -> list[tuple[int, int]]:
     return out
 
 
+def _one_rounding(*banks: QuantWeight) -> tuple:
+    """The banks of an expert layer, which take their rows in one packing: where only some are FP8, those as bf16."""
+    if len({w.fmt == WFormat.FP8 for w in banks}) == 1:
+        return banks
+    return tuple(QuantWeight(**_as_bf16(w)) if w.fmt == WFormat.FP8 else w for w in banks)
+
+
 class MoEFFN:
     """Router -> top-k -> experts -> weighted combine, expert-parallel over the ranks of ``par``.
 
@@ -664,6 +671,7 @@ class MoEFFN:
             gran = d.k_granule() if d.fmt == WFormat.FP8 and -(-F // d.k_granule()) >= ep else 32
             f_lo, f_hi = _even_chunks(F, ep, gran)[par.rank]
             g, u, d = g.slice_rows(f_lo, f_hi), u.slice_rows(f_lo, f_hi), d.slice_k(f_lo, f_hi, requant=True)
+        g, u, d = _one_rounding(g, u, d)
         # MXFP4 banks on a GPU run on the block-scaled tensor-core kernel: gate / up / down stay three banks in its tiled layout
         self.mx = None
         # all-MXFP4 expert banks multiply MXFP8 activations (e4m3 + a power-of-two scale per 32): the arithmetic of the block-scaled
@@ -840,6 +848,7 @@ class UnaryMoEFFN(MoEFFN):
         self.router = Linear((rw if rw.fmt == WFormat.BF16 else QuantWeight(**_as_bf16(rw))).pad_groups(cols=(1, row)))
         self.gate_up = src.matrix(f"{prefix}.e*.up", ffn, hidden, experts).pad_groups(rows=(1, f), cols=(1, row))
         self.down = src.matrix(f"{prefix}.e*.down", hidden, ffn, experts).pad_groups(rows=(1, row), cols=(1, f))
+        self.gate_up, self.down = _one_rounding(self.gate_up, self.down)
         self.router_bias = self.gu_bias = self.down_bias = self.expert_scale = self.shared = self.mx = self._spill = None
         self.act, self.a8, self.reduce, self.group_gemv_max_tokens, self._arange = act, False, False, 0, {}
 
@@ -865,7 +874,8 @@ class ScaledInputMoEFFN(UnaryMoEFFN):
     def __init__(self, src, prefix: str, hidden: int, row: int, experts: int, used: int, ffn: int, shared_ffn: int = 0, act: int = ACT_SWIGLU):
         super().__init__(src, prefix, hidden, row, experts, used, ffn, act)          # (gate_up holds the up rows so far)
         gate = src.matrix(f"{prefix}.e*.gate", ffn, hidden, experts).pad_groups(rows=(1, round_up(ffn, 32)), cols=(1, row))
-        self.gate_up = QuantWeight.interleave_gate_up(gate, self.gate_up)
+        gate, up, self.down = _one_rounding(gate, self.gate_up, self.down)
+        self.gate_up = QuantWeight.interleave_gate_up(gate, up)
         self.shared = GatedFFN(src, f"{prefix}.shared", hidden, row, shared_ffn, act) if shared_ffn else None
 
     def __call__(self, h: torch.Tensor, par: Optional[ParallelCtx] = None):
@@ -896,7 +906,8 @@ class ClampedMoEFFN(UnaryMoEFFN):
                  act: int = ACT_SWIGLU_OAI, alpha: float = 1.702):
         super().__init__(src, prefix, hidden, row, experts, used, ffn, act)          # (gate_up holds the up rows so far)
         gate = src.matrix(f"{prefix}.e*.gate", ffn, hidden, experts).pad_groups(rows=(1, round_up(ffn, 32)), cols=(1, row))
-        self.gate_up = QuantWeight.interleave_gate_up(gate, self.gate_up)
+        gate, up, self.down = _one_rounding(gate, self.gate_up, self.down)
+        self.gate_up = QuantWeight.interleave_gate_up(gate, up)
         if self.gate_up.nbytes <= experts * self.PAIR_GEMV_SMALL_BYTES:
             self.PAIR_GEMV_MAX_TOKENS = 6
         self.act_kw = dict(act=act, act_alpha=alpha, act_limit=limit)

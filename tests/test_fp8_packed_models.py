@@ -1,4 +1,6 @@
 """Expert layers of the layer-list graphs with FP8 banks: the same numbers from pairs in slots (a few tokens) and from pairs sorted by expert (prompts)."""
+from dataclasses import replace
+
 import pytest
 import torch
 
@@ -6,8 +8,9 @@ from machx_inference_engine_b200 import ops
 from machx_inference_engine_b200.formats.model_config import preset
 from machx_inference_engine_b200.models import build_model
 from machx_inference_engine_b200.models.sources import SynthSource, default_policy
-from machx_inference_engine_b200.models.transformer import ClampedMoEFFN, ScaledInputMoEFFN, UnaryMoEFFN
+from machx_inference_engine_b200.models.transformer import ClampedMoEFFN, MoEFFN, ScaledInputMoEFFN, UnaryMoEFFN
 from machx_inference_engine_b200.ops.weights import WFormat
+from machx_inference_engine_b200.parallel.comm import ParallelCtx
 from machx_inference_engine_b200.runtime.engine import EngineOptions, LLMEngine, SamplingParams
 
 H, E, K, F = 160, 6, 2, 96
@@ -59,3 +62,38 @@ def test_other_formats_take_the_padded_packing():
     s = m(h)
     assert m.gate_up.fmt == WFormat.Q8 and s.y.shape[0] % 128 == 0
     assert isinstance(s, ops.ExpertSum) and issubclass(ClampedMoEFFN, UnaryMoEFFN)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("odd", ["down", "gate_up"])
+def test_banks_of_which_one_is_fp8(odd, dev):
+    """A layer's rows come in one packing; where a file has FP8 codes for some of its banks only, those are decoded to bf16 and the layer takes the other formats' paths."""
+    def mixed(quant):
+        def policy(name):
+            down = "down" in name
+            if "gate_inp" in name:
+                return WFormat.BF16
+            return WFormat.FP8 if quant == "fp8" and down == (odd == "down") else WFormat.Q8 if down and quant == "fp8" else WFormat.BF16
+        return policy
+
+    cfg = replace(preset("tiny-qwen3moe"), hidden=128)
+    m = MoEFFN(cfg, 0, SynthSource(dev, mixed("fp8"), seed=7, gen_device="cpu"), ParallelCtx(), act=ops.ACT_SWIGLU, with_bias=False)
+    assert WFormat.FP8 not in (m.gate_up.fmt, m.down.fmt)
+    plain = MoEFFN(cfg, 0, SynthSource(dev, mixed("bf16"), seed=7, gen_device="cpu"), ParallelCtx(), act=ops.ACT_SWIGLU, with_bias=False)
+    for T in (2, 9, 40):
+        h = torch.randn(T, 128, generator=torch.Generator().manual_seed(T)).to(dev, torch.bfloat16)
+        got, want = (x(h, ParallelCtx()) for x in (m, plain))
+        # the same weights but for the rounding of one or two banks to e4m3, half a step of 2^-4 of each value at most, and of the other to bf16 or 8 bits
+        assert float((got - want).norm() / want.norm()) < 2.0 ** -3, T
+
+
+@pytest.mark.parametrize("cls", [ClampedMoEFFN, ScaledInputMoEFFN])
+@pytest.mark.parametrize("which", ["gate up", "down", "up down", "gate"])
+def test_gated_banks_of_which_some_are_fp8(cls, which):
+    policy = lambda fp8: lambda name: WFormat.FP8 if fp8 and name.rsplit(".", 1)[-1] in which.split() else WFormat.BF16
+    m, plain = (cls(SynthSource("cpu", policy(fp8), seed=3), "x", H, H, E, K, F, **({"limit": 1.5} if cls is ClampedMoEFFN else {})) for fp8 in (True, False))
+    assert WFormat.FP8 not in (m.gate_up.fmt, m.down.fmt)
+    for T in (2, 30):
+        h = torch.randn(T, H, generator=torch.Generator().manual_seed(T)).to(torch.bfloat16)
+        got, want = m(h).materialize(), plain(h).materialize()
+        assert 0 < float((got - want).norm() / want.norm()) < 2.0 ** -3      # (as above)
