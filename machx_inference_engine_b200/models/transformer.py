@@ -997,6 +997,13 @@ def _as_bf16(w: QuantWeight) -> dict:
     return dict(fmt=ops.WFormat.BF16, N=w.N, K=w.K, E=w.E, p0=d.contiguous())
 
 
+def _projections(layer: dict) -> list:
+    """The dense products of a layer's attention and feed-forward."""
+    at, ffn = layer["attn"], layer.get("ffn")
+    lins = [at.qkv, at.o] + ([] if ffn is None else [ffn.down, *(ffn.split or [ffn.gate_up])])
+    return [p for lin in lins for p in getattr(lin, "parts", [lin])]
+
+
 # ---------------------------------------------------------------------------------------------
 class TransformerModel:
     def __init__(self, cfg: ModelConfig, src, device, par: Optional[ParallelCtx] = None, max_ctx: int = 8192):
@@ -1085,7 +1092,7 @@ class TransformerModel:
             return False
         if not sc.can_shard(fb.T) or fb.T < self.SHARD_MIN_TOKENS:
             return False
-        if any(L["attn"].o.w.fmt == WFormat.FP8 for L in self.layers):      # (the gathered products take the other formats)
+        if any(lin.w.fmt == WFormat.FP8 for L in self.layers for lin in _projections(L)):      # (the gathered products take the other formats)
             return False
         return all(("moe" not in L) or (L["moe"].mx is not None and L["moe"].shared is None and not L["moe"].expert_tp and L["moe"]._spill is None)
                    for L in self.layers)

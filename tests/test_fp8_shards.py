@@ -7,7 +7,7 @@ import torch
 
 from machx_inference_engine_b200.formats.model_config import preset
 from machx_inference_engine_b200.models.sources import SynthSource, default_policy
-from machx_inference_engine_b200.models.transformer import DenseFFN, MoEFFN, _even_chunks
+from machx_inference_engine_b200.models.transformer import DenseFFN, MoEFFN, TransformerModel, _even_chunks
 from machx_inference_engine_b200.ops import ACT_SWIGLU
 from machx_inference_engine_b200.ops.weights import WFormat, from_fp8
 from machx_inference_engine_b200.parallel.comm import ParallelCtx
@@ -126,3 +126,14 @@ def test_ranks_match_a_single_one(monkeypatch, name, world, within):
     many = _run(world, name, "fp8", "cpu")
     a, b = one["logits"].flatten(), many["logits"].flatten()
     assert many["world"] == world and float(torch.dot(a, b) / (a.norm() * b.norm())) > 0.98
+
+
+@pytest.mark.parametrize("kind", ["attn_q", "attn_v", "attn_output", "ffn_gate", "ffn_down", "none"])
+def test_the_row_sharded_prefill_is_not_taken_with_any_fp8_projection(kind):
+    """Its products read gathered rows and store into their peers' memory, which no FP8 product does; a file may hold codes for some of a layer's matrices only."""
+    cfg = preset("tiny-llama")
+    policy = lambda name: WFormat.FP8 if kind in name and name.startswith("blk.1.") else WFormat.BF16
+    par = ParallelCtx()
+    model = TransformerModel(cfg, SynthSource("cpu", policy, seed=1), "cpu", par, max_ctx=1024)
+    par.fused, par.sharded = object(), type("All", (), {"can_shard": lambda self, T: True})()
+    assert model._can_shard(type("FB", (), {"T": 640, "want_hidden": False})(), None) == (kind == "none")
