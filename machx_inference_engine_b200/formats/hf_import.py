@@ -196,6 +196,27 @@ def _pick_type(name: str, k: int) -> int:
     return int(want)
 
 
+# what an FP8 checkpoint leaves unquantised is kept: its sensitive projections, the embedding and the head
+_KEPT = {"BF16": GGMLType.BF16, "F16": GGMLType.F16, "F32": GGMLType.F32}
+
+
+def _matrix_type(m: HFMeta, st: SafetensorsModel, src: str, gname: str, k: int) -> int:
+    if m.quant_method == "fp8":
+        return int(_KEPT.get(st.dtype(src), GGMLType.F32))
+    return _pick_type(gname, k)
+
+
+def _stored(dense: np.ndarray, t: int) -> np.ndarray:
+    """A matrix in fp32 as the bytes of a tensor of type ``t``."""
+    if t == GGMLType.F32:
+        return np.ascontiguousarray(dense, dtype=np.float32).view(np.uint8).reshape(-1)
+    if t == GGMLType.F16:
+        return dense.astype(np.float16).view(np.uint8).reshape(-1)
+    if t == GGMLType.BF16:       # (its own values: the low halves are zeros)
+        return (np.ascontiguousarray(dense, dtype=np.float32).view(np.uint32) >> 16).astype(np.uint16).view(np.uint8).reshape(-1)
+    return quantize(np.ascontiguousarray(dense), t)
+
+
 def _add_exl3_tensors(w: GGUFWriter, st: SafetensorsModel, names: list, m: HFMeta) -> int:
     """An EXL3 (exllamav3) checkpoint: every quantised linear is ``<module>.trellis`` int16 [K/16, N/16, 16*bits] with ``.suh`` [K] and
     ``.svh`` [N]; they go into the GGUF unchanged (type 37, dims {16*bits, N/16, K/16}, and F16 siblings ``<name>.suh`` / ``.svh``), the
@@ -322,10 +343,7 @@ def import_to_gguf(hf_dir: str, out_path: str, tokenizer_gguf: Optional[str] = N
                 dense = st.float32(src)
             if arch == "llama" and (".attn_q." in gname or ".attn_k." in gname):
                 dense = _llama_permute(dense, m.n_heads if ".attn_q." in gname else m.n_kv_heads)
-            t = _pick_type(gname, dense.shape[1])
-            if t == GGMLType.F16:
-                return dense.astype(np.float16).view(np.uint8).reshape(-1)
-            return quantize(np.ascontiguousarray(dense), t)
+            return _stored(dense, _matrix_type(m, st, src, gname, dense.shape[1]))
         return f
 
     n_t = 0
@@ -341,7 +359,7 @@ def import_to_gguf(hf_dir: str, out_path: str, tokenizer_gguf: Optional[str] = N
         else:
             k, n_out = dims
             f = make(gname, kind, src, dims)
-            w.add_tensor(gname, [k, n_out], _pick_type(gname, k), f if stream else f())
+            w.add_tensor(gname, [k, n_out], _matrix_type(m, st, src, gname, k), f if stream else f())
         n_t += 1
     w.write(out_path)
     log(f"[import] {n_t} tensors -> {out_path} ({os.path.getsize(out_path) / 1e6:.1f} MB), quant source: {m.quant_method or 'none'}")
