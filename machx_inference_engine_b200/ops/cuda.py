@@ -1031,12 +1031,12 @@ def _fp8_expert_plan(rows: int, experts: int, K: int) -> tuple:
     return 0, 256
 
 
-def _fp8_product(x, w: QuantWeight, shape, dtype, out, bias, row_scale, act, act_alpha, act_limit, **kw):
-    """Checked arguments -> the result, on the rows' device, whichever is current."""
+def _fp8_product(x, w: QuantWeight, shape, dtype, out, bias, row_scale, act, act_alpha, act_limit, experts=1, **kw):
+    """Checked arguments -> the result, on the rows' device, whichever is current.  ``experts``: those that the rows of a packing are shared out among; ``w`` may hold some of them."""
     dev = x.device
     if dev.index != torch.cuda.current_device():
         with torch.cuda.device(dev):
-            return _fp8_product(x, w, shape, dtype, out, bias, row_scale, act, act_alpha, act_limit, **kw)
+            return _fp8_product(x, w, shape, dtype, out, bias, row_scale, act, act_alpha, act_limit, experts, **kw)
     if out is None:
         out = w.p0.new_empty(shape, dtype=dtype)
     M = shape[0]
@@ -1045,7 +1045,7 @@ def _fp8_product(x, w: QuantWeight, shape, dtype, out, bias, row_scale, act, act
     if kw.get("slot") is not None:
         nt, bn, cuts = 16, 0, 1
     elif kw.get("counts") is not None:
-        (nt, bn), cuts = _fp8_expert_plan(M, w.E, w.K), 1
+        (nt, bn), cuts = _fp8_expert_plan(M, experts, w.K), 1
     else:
         nt, bn, cuts = _fp8_plan(M, w.N, w.K)
     return _fp8_call(x, w, out, bias, row_scale, act, act_alpha, act_limit, nt, bn, cuts, **kw)
@@ -1072,7 +1072,7 @@ def expert_linear(x, w: QuantWeight, pk: MoePacking, x_index=None, bias=None, ac
     P = pk.max_rows
     _fp8.check_product(x, w, True, P, bias, gated, "expert_linear")
     _fp8.check_packing(pk, w, x, x_index, e_lo)
-    return _fp8_product(x, w, (P, w.N // 2 if gated else w.N), torch.float32 if out_f32 else torch.bfloat16, None, bias, None, act, act_alpha, act_limit,
+    return _fp8_product(x, w, (P, w.N // 2 if gated else w.N), torch.float32 if out_f32 else torch.bfloat16, None, bias, None, act, act_alpha, act_limit, pk.counts.numel(),
                         counts=pk.counts[e_lo:] if e_lo else pk.counts, seg=pk.seg_start[e_lo:] if e_lo else pk.seg_start, index=x_index)
 
 

@@ -1,0 +1,42 @@
+"""FP8 products over packings: which kernel a share of a bank takes, packings without a pair, rows that are not there."""
+import zlib
+
+import pytest
+import torch
+
+import fp8_oracle as O
+from machx_inference_engine_b200 import ops
+from machx_inference_engine_b200.ops.weights import from_fp8
+
+DEVICES = ["cpu", pytest.param("cuda:0", marks=pytest.mark.gpu)]
+
+
+def gen(*key):
+    return torch.Generator().manual_seed(zlib.crc32(repr(key).encode()))
+
+
+def bank(N, K, E, dev):
+    g = gen(N, K, E)
+    codes = (torch.randn(E, N, K, generator=g).clamp(-4, 4) * 112).to(torch.float8_e4m3fn)
+    return from_fp8(codes, (0.5 + torch.rand(E, -(-N // 128), -(-K // 128), generator=g)) * (K ** -0.5 / 112)).to(dev)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,E,k", [(4, 64, 4), (64, 128, 8), (48, 32, 4), (300, 16, 4)])
+def test_a_share_of_a_bank_takes_the_kernel_of_the_whole_one(monkeypatch, T, E, k):
+    """The rule asks for the rows of an expert on average: a rank that holds some of the experts has the same."""
+    from machx_inference_engine_b200.ops import cuda as K
+    plans, call = [], K._fp8_call
+    monkeypatch.setattr(K, "_fp8_call", lambda *a, **kw: (plans.append(a[8:11]), call(*a, **kw))[1])
+    x, w = torch.randn(T, 128, generator=gen(T)).to("cuda:0", torch.bfloat16), bank(64, 128, E, "cuda:0")
+    idx = torch.randn(T, E, generator=gen(T, E)).topk(k, dim=1).indices.to("cuda:0", torch.int32)
+    full = ops.moe_pack(idx, E, tile=1)
+    whole = ops.expert_linear(x, w, full, x_index=full.packed_token)[full.pair_to_packed.long()]
+    for parts in (2, 8):
+        n = E // parts
+        for lo in (0, E - n):
+            pk = ops.moe_pack(idx, E, lo, lo + n, tile=1)
+            got = ops.expert_linear(x, w.slice_experts(lo, lo + n), pk, x_index=pk.packed_token, e_lo=lo)
+            p = pk.pair_to_packed.long()
+            assert torch.equal(got[p[p >= 0]], whole[p >= 0])            # (one kernel; a single block of K is never cut)
+    assert len(set(plans)) == 1
