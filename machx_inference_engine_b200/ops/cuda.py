@@ -1072,7 +1072,10 @@ def expert_linear(x, w: QuantWeight, pk: MoePacking, x_index=None, bias=None, ac
     P = pk.max_rows
     _fp8.check_product(x, w, True, P, bias, gated, "expert_linear")
     _fp8.check_packing(pk, w, x, x_index, e_lo)
-    return _fp8_product(x, w, (P, w.N // 2 if gated else w.N), torch.float32 if out_f32 else torch.bfloat16, None, bias, None, act, act_alpha, act_limit, pk.counts.numel(),
+    shape, dtype = (P, w.N // 2 if gated else w.N), torch.float32 if out_f32 else torch.bfloat16
+    if pk.pair_to_packed.numel() == 0:           # (one row, which is behind the last expert's)
+        return w.p0.new_empty(shape, dtype=dtype)
+    return _fp8_product(x, w, shape, dtype, None, bias, None, act, act_alpha, act_limit, pk.counts.numel(),
                         counts=pk.counts[e_lo:] if e_lo else pk.counts, seg=pk.seg_start[e_lo:] if e_lo else pk.seg_start, index=x_index)
 
 

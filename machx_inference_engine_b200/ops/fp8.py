@@ -107,6 +107,8 @@ def check_packing(pk, w: QuantWeight, x, x_index, e_lo: int) -> None:
             raise ValueError(f"expert_linear: {x.shape[0]} rows for a packing of {pk.pair_to_packed.numel()}")
     elif x_index.dtype != torch.int32 or x_index.numel() < pk.max_rows or not x_index.is_contiguous() or x_index.device != x.device:
         raise ValueError("expert_linear: x_index is a contiguous int32 vector with an entry for every packed row")
+    elif x.shape[0] == 0 and pk.pair_to_packed.numel():
+        raise ValueError(f"expert_linear: no rows for a packing of {pk.pair_to_packed.numel()}")
     if x_index is not None and isinstance(x, FP8Rows):
         raise ValueError("expert_linear: rounded rows come in packed order; fp8_rows(x, index=...) puts them there")
 

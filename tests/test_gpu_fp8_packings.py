@@ -40,3 +40,30 @@ def test_a_share_of_a_bank_takes_the_kernel_of_the_whole_one(monkeypatch, T, E, 
             p = pk.pair_to_packed.long()
             assert torch.equal(got[p[p >= 0]], whole[p >= 0])            # (one kernel; a single block of K is never cut)
     assert len(set(plans)) == 1
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("indexed", [False, True])
+def test_a_packing_without_a_pair(dev, indexed):
+    """One row, which lies behind the last expert's and is nobody's."""
+    w = bank(96, 256, 3, dev)
+    none = torch.empty(0, 256, dtype=torch.bfloat16, device=dev)
+    pk = ops.moe_pack(torch.empty(0, 2, dtype=torch.int32, device=dev), 3, tile=1)
+    assert pk.max_rows == 1 and pk.pair_to_packed.numel() == 0
+    kw = dict(x_index=pk.packed_token) if indexed else {}
+    some = torch.ones(5, 256, dtype=torch.bfloat16, device=dev)
+    for x in (none, some) if indexed else (none, some, ops.fp8_rows(none)):
+        assert ops.expert_linear(x, w, pk, **kw).shape == (1, 96)
+        assert ops.expert_linear(x, w, pk, bias=torch.zeros(3, 96, device=dev), act=ops.ACT_SWIGLU, out_f32=True, **kw).shape == (1, 48)
+    if dev != "cpu":
+        torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_no_rows_for_pairs_are_refused(dev):
+    w = bank(96, 256, 3, dev)
+    pk = ops.moe_pack(torch.zeros(4, 2, dtype=torch.int32, device=dev), 3, tile=1)
+    none = torch.empty(0, 256, dtype=torch.bfloat16, device=dev)
+    for kw in (dict(), dict(x_index=pk.packed_token)):
+        with pytest.raises(ValueError):
+            ops.expert_linear(none, w, pk, **kw)
