@@ -459,7 +459,7 @@ int fp8_stream_launch(const Fp8Call& c, bool round, cudaStream_t st) {
   Fp8Params p = fp8_params(c);
   const int nt = c.nt;
   const long long groups = c.slot ? c.M : c.counts ? (long long)c.M / nt + (c.E < c.M ? c.E : c.M) + 1 : 1;
-  if (c.E > FS_MAX_E || groups >= 65536 || groups * ((p.N + FS_TILE - 1) / FS_TILE) * p.kb >= 1ll << 30 || (!c.slot && !c.counts && c.M > nt)) return -106;      // (units are counted in 32 bits)
+  if ((c.counts && c.E > FS_MAX_E) || groups >= 65536 || groups * ((p.N + FS_TILE - 1) / FS_TILE) * p.kb >= 1ll << 30 || (!c.slot && !c.counts && c.M > nt)) return -106;      // (units are counted in 32 bits)
   if (((uintptr_t)c.codes | (uintptr_t)c.w | (uintptr_t)c.scratch) & 15) return -114;
   if (!c.scratch || !c.tickets || c.scratch_bytes < stream_scratch(nt)) return -131;
   CUtensorMap tw, tx;

@@ -67,3 +67,19 @@ def test_no_rows_for_pairs_are_refused(dev):
     for kw in (dict(), dict(x_index=pk.packed_token)):
         with pytest.raises(ValueError):
             ops.expert_linear(none, w, pk, **kw)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("S,N", [(6, 64), (700, 96)])
+def test_slots_of_more_experts_than_a_packing_takes(S, N, dev):
+    """A packing's tables end at 1024 experts; a slot names its expert itself, in the few-row kernel and in the streaming one."""
+    E, K = 1100, 256
+    w, x = bank(N, K, E, dev), torch.randn(S, K, generator=gen(S)).to(dev, torch.bfloat16)
+    slot = torch.randint(0, E, (S,), generator=gen(S, 1), dtype=torch.int32)
+    slot[:2] = torch.tensor([E - 1, 1024], dtype=torch.int32)
+    want = torch.einsum("pk,pnk->pn", O.row_values(x), O.weight_values(w)[slot.long()])
+    assert O.rel(ops.expert_gemv(x, w, slot.to(dev), out_f32=True), want) < O.fp32_bound(K) + 2.0 ** -22      # (2^-22: the CPU's sums in another order)
+    pk = ops.MoePacking(torch.zeros(E, dtype=torch.int32, device=dev), torch.zeros(E + 1, dtype=torch.int32, device=dev), torch.zeros(S, dtype=torch.int32, device=dev),
+                        torch.zeros(S, dtype=torch.int32, device=dev), None, None, S, 1)
+    with pytest.raises(ValueError):
+        ops.expert_linear(x, w, pk)
