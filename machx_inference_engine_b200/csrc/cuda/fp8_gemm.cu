@@ -3,20 +3,21 @@
 // for dense layers and for rows sorted by expert.
 //
 // A block of K is one stage: 128 rows of x and BN of w, 128 bytes each, and four tcgen05.mma of K = 32.  Its sums have a scale of their own, so they cannot
-// stay in TMEM: eight warps read each block's 128 x BN sums and add s_x s_w times them to fp32 sums in registers, BN / 2 columns of a row per thread, while the
+// stay in TMEM: sixteen warps read each block's 128 x BN sums and add s_x s_w times them to fp32 sums in registers, BN / 4 columns of a row per thread, while the
 // tensor cores fill the next accumulator.
 //   warp 0      TMA loads into a ring of NST stages
 //   warp 1      tcgen05.mma from one thread into a ring of 512 / BN accumulators
 //   warps 2, 3  asynchronous copies of the block's scales (128 of the rows, BN / 16 of the weights) into a ring.  Loads into registers would be waited for one block
 //               ahead at most, whatever the distance: they share the counters by which a warp waits
-//   warps 4-11  sums (warp & 3: rows, warp / 8: half of the columns); a finished tile goes through shared memory, so that rows are written in runs of 64 bytes
+//   warps 4-19  sums (warp & 3: rows, warp / 4 - 1: quarter of the columns); a finished tile goes through shared memory, so that rows are written in runs of 64 or 128 bytes
 // A dense product with fewer tiles than SMs is cut along K: the pieces of a tile leave fp32 sums, and the warp that arrives last adds them in the order of the pieces.
 //
 // What bounds it is the way from L2 to shared memory, about 60 bytes a cycle and SM, and for long prompts the power cap.  A block of a 128 x 256 tile is 48 KB for 512 cycles of
 // products and takes 860; of 128 x 128, 32 KB for 256 cycles, 630.  Without the products a block takes no less; without the loads it takes 540 (256 columns).  Tiles of 256 x
 // 256 on pairs of SMs load a third less and were built: with room for two blocks' sums the signals between the CTAs took what was saved (423 to 500 ns a block, this
 // kernel 455), and under the power cap 4096 x 28672 x 4096 took 574 us, this kernel 544.
-// Measured: 4096 x 28672 x 4096 gated 470 us (2.05 PFLOP/s, 1.22 of the measured bf16 burst; 545 us back to back under the power cap), 512 x 4096 x 14336 42 us (1.43 PFLOP/s).
+// Measured, of rows that were rounded before: 4096 x 28672 x 4096 gated 494 us after a pause (1.95 PFLOP/s, 1.16 of the measured bf16 burst), 538 back to back under the power cap;
+// 512 x 4096 x 14336 44 us back to back (1.38 PFLOP/s).  With the rounding 503, 560 and 52.
 // Every mbarrier wait is bounded.
 #include "act.cuh"
 #include "common.cuh"

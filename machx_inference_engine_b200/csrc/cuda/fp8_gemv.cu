@@ -7,8 +7,8 @@
 // global memory to registers in the layout of mma.m16n8k32: a lane's 16 bytes are four consecutive k of four steps, the rows' codes in shared memory are read the same way, and the
 // order of k within a block is free.  (On B200 these products take a tenth of the time: tcgen05 has them faster, but its accumulators come back through two more waits.)  Every
 // CTA rounds the blocks of the rows that it needs itself.  The first weights are on their way to L2 before the launch before has ended.
-// Measured in a graph of calls, us, with the streaming kernel in brackets: 1 x 512 x 2048 3.0 (5.7), 1 x 1024 x 8192 5.0 (9.3), 1 x 5120 x 2880 6.3 (9.7), 1 x 12288 x 2048 7.9
-// (9.7); gated slots, 10 of 512 of 1024 x 2048, 7.8 (9.2).
+// Measured in a graph of calls over more weights than L2 holds, us, with the streaming kernel in brackets: 1 x 512 x 2048 3.3 (5.3), 1 x 1024 x 8192 5.4 (7.9), 1 x 5120 x 2880 6.7 (9.1), 1 x 12288 x 2048 8.6
+// (9.6); gated slots, 10 of 512 of 1024 x 2048, 7.9 (9.0).  One layer again and again, its weights in L2: 3.2 (5.5), 4.7 (7.7), 5.9 (8.7), 6.3 (9.0) and 7.4 (8.3).
 #include "act.cuh"
 #include "cluster.cuh"
 #include "common.cuh"
@@ -197,9 +197,12 @@ __global__ void __launch_bounds__(FV_THREADS, FV_CTAS) fp8_gemv_kernel(const Fp8
 // Pieces along K and bytes of rounded rows; no cuts: left to the streaming kernel, which has the memory busier once it runs.  In a model's chain of launches that kernel fills its
 // rings with weights under the launch before, so long rows want a smaller limit than calls in a loop show.  Decode of one token, ms with the streaming kernel -> with these
 // limits: Qwen3-MoE-30B's shape 3.64 -> 3.12, Qwen3-Next's 4.75 -> 3.98, gpt-oss-20b's 2.71 -> 2.58; Llama-3-8B's (K = 4096, layers of 4096 blocks and up) 2.95 -> 3.21 if it
-// took them, so it does not.  With more rows the rounding that every CTA does again counts, us: 4 x 5120 x 2880 10.3 -> 7.8, 8 x 1024 x 8192 9.8 -> 7.5, but 4 x 6144 x 4096 9.9 ->
-// 11.2, 4 x 2048 x 14336 10.3 -> 11.5.  CTAs past a wave: slots, 10 x 2048 x 512 (640 CTAs, 592 at a time) 8.2 -> 6.8, 16 x 2048 x 768 (1024) 6.5 -> 9.5.  Pieces are powers of two
-// and leave an eighth of the SMs' room: clusters of three that would have filled it (576 CTAs) waited for a place and took twice the time.
+// took them, so it does not.  The border between the limits lies at 24 blocks of K.  It was looked for in 24 layers of a llama of hidden size H (K of the layers but the last of
+// each, whose rows are 3.5 H long), ms a token with the small limit for every K -> the large one: H of 20 blocks 1.56 -> 1.50, 26 2.27 -> 2.22, 28 1.93 -> 1.94 to 2.19, 30 2.11 ->
+// 2.33, 32 2.15 -> 2.37.
+// With more rows the rounding that every CTA does again counts, us: 4 x 5120 x 2880 10.3 -> 7.8, 8 x 1024 x 8192 9.8 -> 7.5, but 4 x 6144 x 4096 9.9 -> 11.2, 4 x 2048 x 14336
+// 10.3 -> 11.5.  CTAs past a wave: slots, 10 x 2048 x 512 (640 CTAs, 592 at a time) 8.2 -> 6.8, 16 x 2048 x 768 (1024) 6.5 -> 9.5.  Pieces are powers of two and leave an eighth
+// of the SMs' room: clusters of three that would have filled it (576 CTAs) waited for a place and took twice the time.
 struct GemvPlan { int cuts, smem; long long items; };
 static GemvPlan gemv_plan(const Fp8Call& c) {
   GemvPlan g{};

@@ -12,8 +12,9 @@
 // The work is the list of (group of rows, 128 weight rows, block of K) laid end to end, of which every CTA takes an equal run.  A tile that is cut leaves fp32
 // partials (at most two per CTA); the warp that arrives last adds them in the order of the CTAs, so results do not depend on timing.
 // Bound: memory, and for a token the latencies of one launch.  Two CTAs share an SM: with one and 80 KB of weights under way 8 x 28672 x 4096 took 32 us.
-// Measured in a graph of calls: 8 x 28672 x 4096 gated 25.2 us (4.7 TB/s), 1 x 6144 x 4096 8.4 us, 1 x 28672 x 4096 23.8 us, 1 x 4096 x 14336 14.9 us (about five from launch to the first sums), experts of 64
-// tokens, 8 of 128 of 1536 x 2048, 61.8 us (6.4 TB/s, 0.98 of a copy's rate), slots of four tokens, 4 of 32 of 2880 x 2880, 27 us.
+// Measured in a graph of calls over more weights than L2 holds: 8 x 28672 x 4096 gated 25.1 us (4.7 TB/s), 1 x 6144 x 4096 9.6 us, 1 x 28672 x 4096 23.4 us, 1 x 4096 x 14336 14.3 us (about five from launch
+// to the first sums), experts of 64 tokens, 8 of 128 of 1536 x 2048, 63.7 us (6.2 TB/s, 0.95 of a copy's rate), slots of four tokens, 4 of 32 of 2880 x 2880, 23.6 us.  One layer again and again, its weights in
+// L2: 1 x 6144 x 4096 8.3 us, 1 x 4096 x 14336 10.9.
 // Every mbarrier wait is bounded.
 #include "act.cuh"
 #include "common.cuh"
