@@ -1020,6 +1020,8 @@ class TransformerModel:
         self.first_stage, self.last_stage = (not self.pp or par.rank == 0), (not self.pp or par.rank == par.world - 1)
         self.tied = not src.has("output.weight") or c.tie_embeddings
         self.embed_w = self._vocab_matrix(src, "token_embd.weight") if (self.first_stage or (self.last_stage and self.tied)) else None
+        if self.embed_w is not None and self.embed_w.fmt == WFormat.FP8:
+            self.embed_w = QuantWeight(**_as_bf16(self.embed_w))       # (a table of rows to read, which no kernel reads as e4m3)
         head = None
         if self.last_stage:
             head = self.embed_w if self.tied else self._vocab_matrix(src, "output.weight")

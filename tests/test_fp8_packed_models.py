@@ -8,7 +8,7 @@ from machx_inference_engine_b200 import ops
 from machx_inference_engine_b200.formats.model_config import preset
 from machx_inference_engine_b200.models import build_model
 from machx_inference_engine_b200.models.sources import SynthSource, default_policy
-from machx_inference_engine_b200.models.transformer import ClampedMoEFFN, MoEFFN, ScaledInputMoEFFN, UnaryMoEFFN
+from machx_inference_engine_b200.models.transformer import ClampedMoEFFN, MoEFFN, ScaledInputMoEFFN, TransformerModel, UnaryMoEFFN
 from machx_inference_engine_b200.ops.weights import WFormat
 from machx_inference_engine_b200.parallel.comm import ParallelCtx
 from machx_inference_engine_b200.runtime.engine import EngineOptions, LLMEngine, SamplingParams
@@ -97,3 +97,15 @@ def test_gated_banks_of_which_some_are_fp8(cls, which):
         h = torch.randn(T, H, generator=torch.Generator().manual_seed(T)).to(torch.bfloat16)
         got, want = m(h).materialize(), plain(h).materialize()
         assert 0 < float((got - want).norm() / want.norm()) < 2.0 ** -3      # (as above)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("name,tied", [("tiny-llama", False), ("tiny-llama", True)])
+def test_an_embedding_in_fp8_is_decoded_while_loading(dev, name, tied):
+    """Rows of it are read, not multiplied; the head stays FP8 where it is a matrix of its own."""
+    cfg = replace(preset(name), tie_embeddings=tied)
+    model = TransformerModel(cfg, SynthSource(dev, lambda n: WFormat.FP8, seed=1, gen_device="cpu"), dev, max_ctx=512)
+    assert model.embed_w.fmt == WFormat.BF16 and model.lm_head.w.fmt == (WFormat.BF16 if tied else WFormat.FP8)
+    eng = LLMEngine(model, EngineOptions(max_ctx=512, max_batch_tokens=256, max_seqs=2))
+    out, = eng.generate([list(range(40))], SamplingParams(max_tokens=4))
+    assert len(out) == 4
